@@ -340,6 +340,41 @@ int scp_adamw_multi(const ScpAdamTensor* tensors /* host array */, int n, float 
  * (the seed_dev / bc_dev arguments above point into it) that this call rewrites before each replay. */
 int scp_step_state_set(void* state, uint64_t seed_offset, float bias_corr1, float bias_corr2, void* stream);
 
+/* ---- residual trunks (no counterpart in the reference, whose encoders are two hidden layers deep): the norms around a block
+ *      fused with the block's gate and residual scale, forward and backward, one row = one cell:
+ *        n = Norm_post(h)    r = x + s * act(g) * n    y = Norm_pre(r)
+ *      Norm "layer": (t - mean) / sqrt(var + eps) * w + b (biased variance), "rms": t / sqrt(mean t^2 + eps) * w, "none".
+ *      h == NULL: the norm in front of a trunk's first block, y = Norm_pre(x), no r.
+ *      x, r, dr, dx: fp32, or bf16 with x_bf16; h, y, a full gate and their gradients: fp32, or bf16 with h_bf16 (a bf16
+ *      stream needs bf16 blocks).  Inputs have a row stride in elements (>= 0) and contiguous columns, any alignment; outputs
+ *      are contiguous [rows][cols].  Everything else is fp32.  w1 / w2 null: ones, b1 / b2 null: zeros. ---- */
+typedef struct {
+  const void* x;       /* [rows][ldx] */
+  const void* h;       /* [rows][ldh], nullable */
+  const void* gate;    /* gate_mode 1: [rows][ldg] of h's type, 2: fp32 [rows], 3: fp32 [cols] */
+  const float* scale;  /* scale_mode 1: [1], 2: [cols] */
+  const float *w1, *b1, *w2, *b2;   /* post and pre norm, [cols] */
+  void *r, *y;
+  float* stats;        /* [rows][4] mean1, 1/spread1, mean2, 1/spread2: written forward (nullable there), read backward */
+  const void *dr, *dy; /* nullable: zero */
+  void *dx, *dh, *dgate;            /* each nullable; dgate like gate */
+  float *dscale, *dw1, *db1, *dw2, *db2;   /* each nullable */
+  float* ws;           /* backward: scp_residual_norm_bwd_ws_floats(rows, cols) floats if any parameter gradient or a column
+                          gate's gradient is asked for */
+  long ldx, ldh, ldg, lddr, lddy, rows;
+  int cols, x_bf16, h_bf16;
+  int post, pre;       /* 0 none (post only), 1 rms, 2 layer */
+  int gate_mode;       /* 0 none, 1 per element, 2 per row, 3 per column */
+  int gate_act;        /* 0 none, 1 sigmoid, 2 tanh */
+  int scale_mode;      /* 0 scale_value, 1 one learned number, 2 per column */
+  float scale_value, eps;
+  int want1, want2;    /* set by the backward itself */
+} ScpResidualNorm;
+int scp_residual_norm_max_cols(void);
+int scp_residual_norm_fwd(const ScpResidualNorm* args /* host */, void* stream);
+long scp_residual_norm_bwd_ws_floats(long rows, int cols);
+int scp_residual_norm_bwd(const ScpResidualNorm* args /* host */, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,6 +51,15 @@ class EncTail(C.Structure):
                 ("dbn1_w", P), ("dbn1_b", P), ("dbn2_w", P), ("dbn2_b", P)]
 
 
+class ResidualNorm(C.Structure):
+    _fields_ = [("x", P), ("h", P), ("gate", P), ("scale", P), ("w1", P), ("b1", P), ("w2", P), ("b2", P),
+                ("r", P), ("y", P), ("stats", P), ("dr", P), ("dy", P), ("dx", P), ("dh", P), ("dgate", P),
+                ("dscale", P), ("dw1", P), ("db1", P), ("dw2", P), ("db2", P), ("ws", P),
+                ("ldx", L), ("ldh", L), ("ldg", L), ("lddr", L), ("lddy", L), ("rows", L),
+                ("cols", I), ("x_bf16", I), ("h_bf16", I), ("post", I), ("pre", I), ("gate_mode", I), ("gate_act", I),
+                ("scale_mode", I), ("scale_value", F), ("eps", F), ("want1", I), ("want2", I)]
+
+
 _SIGS = {
     "scp_last_error": (C.c_char_p, []),
     "scp_version": (I, []),
@@ -113,6 +122,10 @@ _SIGS = {
     "scp_raw_rows_feat_bwd": (I, [P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, P, L, P, L, P, P, P, P, P]),
     "scp_fos_counts": (I, [P, L, P, L, I, I, P, P, P, P, P]),
     "scp_adamw_multi": (I, [C.POINTER(AdamTensor), I, F, F, F, P]),
+    "scp_residual_norm_max_cols": (I, []),
+    "scp_residual_norm_fwd": (I, [C.POINTER(ResidualNorm), P]),
+    "scp_residual_norm_bwd_ws_floats": (L, [L, I]),
+    "scp_residual_norm_bwd": (I, [C.POINTER(ResidualNorm), P]),
     "scp_step_state_set": (I, [P, U64, F, F, P]),
 }
 

@@ -2026,3 +2026,229 @@ class NbLogLikFn(torch.autograd.Function):
 
 def nb_loglik(x, mu, theta, pi=None):
     return NbLogLikFn.apply(x, mu, theta, pi)
+
+
+# ------------------------------------------------------------------------------------------------
+# Residual trunks: norms around a block, fused with the block's gate and residual scale
+# ------------------------------------------------------------------------------------------------
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+_GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _same_device(what, *tensors):
+    """Refuses CPU tensors and tensors of several GPUs in one call (None entries are skipped)."""
+    _lib.require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devices))}")
+
+
+class _on:
+    """Makes `dev` the current device for a launch (and its stream the one that is used); free of cost where it is already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, dev):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows_of(t, cols):
+    """2-D view [rows, cols] with contiguous columns of a [..., cols] tensor (a copy only if its strides allow no such view)."""
+    t = t.reshape(-1, cols) if t.ndim != 2 else t
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < 0):
+        t = t.contiguous()
+    return t
+
+
+class GatedResidualNormFn(torch.autograd.Function):
+    """scp_residual_norm_fwd / _bwd (csrc/residual_norm.hip); arguments as gated_residual_norm checked and laid them out."""
+
+    @staticmethod
+    def forward(ctx, x, h, gate, scale, w1, b1, w2, b2, cfg):
+        r, y, stats = _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, True)
+        ctx.save_for_backward(x, h, gate, scale, w1, b1, w2, b2, stats)
+        ctx.cfg = cfg
+        ctx.set_materialize_grads(False)
+        return r, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dr, dy):
+        x, h, gate, scale, w1, b1, w2, b2, stats = ctx.saved_tensors
+        cfg = ctx.cfg
+        if dr is None and dy is None:
+            return (None,) * 9
+        need = ctx.needs_input_grad
+        rows, cols = x.shape
+
+        def out(i, like, dtype=None):
+            if not need[i] or like is None:
+                return None
+            return torch.empty(like.shape, dtype=dtype or like.dtype, device=x.device)
+
+        dx, dh, dgate, dscale = out(0, x), out(1, h), out(2, gate), out(3, scale)
+        dw1, db1, dw2, db2 = out(4, w1), out(5, b1), out(6, w2), out(7, b2)
+        grads = (dx, dh, dgate, dscale, dw1, db1, dw2, db2)
+        if rows == 0:                        # no cell: nothing to launch, the parameters' sums are empty
+            return tuple(None if t is None else t.zero_() for t in grads) + (None,)
+        with _on(x.device):
+            L = _lib.lib()
+            a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
+            a.stats = stats.data_ptr()
+            if dr is not None:
+                dr = _rows_of(dr, cols)
+                a.dr, a.lddr = dr.data_ptr(), dr.stride(0)
+            if dy is not None:
+                dy = _rows_of(dy, cols)
+                a.dy, a.lddy = dy.data_ptr(), dy.stride(0)
+            for name, t in zip(("dx", "dh", "dgate", "dscale", "dw1", "db1", "dw2", "db2"), grads):
+                if t is not None:
+                    setattr(a, name, t.data_ptr())
+            ws = None
+            if dscale is not None or dw1 is not None or db1 is not None or dw2 is not None or db2 is not None \
+                    or (dgate is not None and cfg["gate_mode"] == 3):
+                ws = torch.empty(L.scp_residual_norm_bwd_ws_floats(rows, cols), dtype=torch.float32, device=x.device)
+                a.ws = ws.data_ptr()
+            _lib.check(L.scp_residual_norm_bwd(C.byref(a), _lib.stream()), "scp_residual_norm_bwd")
+        return grads + (None,)
+
+
+def _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg):
+    rows, cols = x.shape
+    a = _lib.ResidualNorm()
+    a.x, a.ldx, a.rows, a.cols = x.data_ptr(), x.stride(0), rows, cols
+    a.x_bf16, a.h_bf16 = x.dtype == torch.bfloat16, cfg["y_type"] == torch.bfloat16
+    a.post, a.pre, a.eps, a.scale_value = cfg["post"], cfg["pre"], cfg["eps"], cfg["scale_value"]
+    a.gate_mode, a.gate_act, a.scale_mode = cfg["gate_mode"], cfg["gate_act"], cfg["scale_mode"]
+    if h is not None:
+        a.h, a.ldh = h.data_ptr(), h.stride(0)
+    if gate is not None:
+        a.gate = gate.data_ptr()
+        if cfg["gate_mode"] == 1:
+            a.ldg = gate.stride(0)
+    if scale is not None:
+        a.scale = scale.data_ptr()
+    if w1 is not None:
+        a.w1 = w1.data_ptr()
+    if b1 is not None:
+        a.b1 = b1.data_ptr()
+    if w2 is not None:
+        a.w2 = w2.data_ptr()
+    if b2 is not None:
+        a.b2 = b2.data_ptr()
+    return a
+
+
+def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, want_stats):
+    rows, cols = x.shape
+    with _on(x.device):
+        r = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if h is not None else None
+        y = torch.empty((rows, cols), dtype=cfg["y_type"], device=x.device)
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
+        if rows == 0:
+            return r, y, stats
+        a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
+        a.y = y.data_ptr()
+        if r is not None:
+            a.r = r.data_ptr()
+        if stats is not None:
+            a.stats = stats.data_ptr()
+        _lib.check(_lib.lib().scp_residual_norm_fwd(C.byref(a), _lib.stream()), "scp_residual_norm_fwd")
+    return r, y, stats
+
+
+def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight=None, post_bias=None, pre="layer",
+                        pre_weight=None, pre_bias=None, gate_act="sigmoid", eps=1e-5, out_dtype=None):
+    """What lies between two blocks of a residual trunk, in one pass over the data in each direction:
+
+        n = Norm_post(h)      r = x + scale * act(gate) * n      y = Norm_pre(r)          returns (r, y)
+
+    x [..., D]: the residual stream, float32 or bfloat16.  h: the block's output, x's shape; float32, or bfloat16 (always
+    bfloat16 where x is).  h None: the norm in front of the first block -- y = Norm_pre(x), and r is x itself.
+    gate: None, [..., D] (an element each, h's type), [..., 1] (a row each) or [D] (a column each); gate_act 'sigmoid',
+    'tanh' or 'none'.  scale: None, a number, a tensor of one element, or [D].  post: None, 'rms' or 'layer'; pre: 'rms' or
+    'layer'.  'layer' takes the biased variance about the mean, 'rms' the mean square and has no bias; both add eps (> 0)
+    under the root.  Weights default to ones, biases to zeros.  y has h's type (h None: out_dtype, x's by default).  At most
+    16384 columns, which lie next to each other (other layouts are copied); rows may have any stride.
+    Sums and statistics are fp32, every output is rounded once, y is the norm of r before r's rounding; results are bitwise
+    reproducible.  Gradients flow to every tensor given; a second derivative is refused."""
+    if not isinstance(x, torch.Tensor) or x.ndim == 0:
+        raise ValueError("gated_residual_norm: x must be a tensor of at least one dimension")
+    shape, cols = x.shape, x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    if x.dtype not in _FLOATS:
+        raise ValueError(f"gated_residual_norm: x must be float32 or bfloat16, got {x.dtype}")
+    if post not in _NORMS or pre not in ("rms", "layer"):
+        raise ValueError(f"gated_residual_norm: post must be None, 'rms' or 'layer' and pre 'rms' or 'layer', got {post!r}, {pre!r}")
+    if gate_act not in _GATE_ACTS:
+        raise ValueError(f"gated_residual_norm: gate_act must be one of {sorted(_GATE_ACTS)}, got {gate_act!r}")
+    if not (eps > 0 and math.isfinite(eps)):
+        raise ValueError(f"gated_residual_norm: eps must be positive, got {eps}")
+    if not 1 <= cols <= 16384:
+        raise ValueError(f"gated_residual_norm: 1 to 16384 columns, got {cols}")
+    cfg = {"post": _NORMS[post], "pre": _NORMS[pre], "gate_mode": 0, "gate_act": _GATE_ACTS[gate_act], "scale_mode": 0,
+           "scale_value": 1.0, "eps": float(eps)}
+    if h is None:
+        if gate is not None or scale is not None or post is not None or post_weight is not None or post_bias is not None:
+            raise ValueError("gated_residual_norm: gate, scale and post norm belong to a block's output h")
+        y_type = out_dtype or x.dtype
+    else:
+        if h.shape != shape:
+            raise ValueError(f"gated_residual_norm: h has shape {tuple(h.shape)}, x {tuple(shape)}")
+        if out_dtype not in (None, h.dtype):
+            raise ValueError("gated_residual_norm: y has h's type; out_dtype is for calls without h")
+        y_type = h.dtype
+    if y_type not in _FLOATS or (x.dtype == torch.bfloat16 and y_type != torch.bfloat16):
+        raise ValueError(f"gated_residual_norm: x {x.dtype} with blocks of {y_type}: float32 or bfloat16 beside float32, "
+                         "bfloat16 beside bfloat16")
+    cfg["y_type"] = y_type
+    if post is None and (post_weight is not None or post_bias is not None):
+        raise ValueError("gated_residual_norm: post_weight / post_bias without a post norm")
+
+    def column(name, t, norm):
+        if t is None:
+            return None
+        if norm == "rms" and name.endswith("bias"):
+            raise ValueError(f"gated_residual_norm: {name} with an rms norm, which has none")
+        if t.shape != (cols,) or not t.is_floating_point():
+            raise ValueError(f"gated_residual_norm: {name} must be a floating-point tensor of shape ({cols},), got "
+                             f"{t.dtype} {tuple(t.shape)}")
+        return _f32c(t)
+
+    w1, b1 = column("post_weight", post_weight, post), column("post_bias", post_bias, post)
+    w2, b2 = column("pre_weight", pre_weight, pre), column("pre_bias", pre_bias, pre)
+    if scale is not None:
+        if not isinstance(scale, torch.Tensor):
+            cfg["scale_value"], scale = float(scale), None
+        elif scale.numel() == 1 and scale.is_floating_point():
+            cfg["scale_mode"], scale = 1, _f32c(scale.reshape(1))
+        else:
+            cfg["scale_mode"], scale = 2, column("scale", scale, None)
+    if gate is not None:
+        if gate.shape == shape and gate.dtype == h.dtype:
+            cfg["gate_mode"], gate = 1, _rows_of(gate, cols)
+        elif gate.shape == (*shape[:-1], 1) and gate.is_floating_point() and len(shape) > 1:
+            cfg["gate_mode"], gate = 2, _f32c(gate.reshape(rows))
+        elif gate.shape == (cols,) and gate.is_floating_point():
+            cfg["gate_mode"], gate = 3, _f32c(gate)
+        else:
+            raise ValueError(f"gated_residual_norm: a gate is {tuple(shape)} of {y_type}, {(*shape[:-1], 1)} or ({cols},), got "
+                             f"{gate.dtype} {tuple(gate.shape)}")
+    _same_device("gated_residual_norm", x, h, gate, scale, w1, b1, w2, b2)
+    x2 = _rows_of(x, cols)
+    h2 = None if h is None else _rows_of(h, cols)
+    tensors = (x2, h2, gate, scale, w1, b1, w2, b2)
+    track = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if track:
+        r, y = GatedResidualNormFn.apply(*tensors, cfg)
+    else:
+        r, y, _ = _residual_norm_fwd(*tensors, cfg, False)
+    return x if h is None else r.reshape(shape), y.reshape(shape)
