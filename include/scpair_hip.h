@@ -375,6 +375,32 @@ int scp_residual_norm_fwd(const ScpResidualNorm* args /* host */, void* stream);
 long scp_residual_norm_bwd_ws_floats(long rows, int cols);
 int scp_residual_norm_bwd(const ScpResidualNorm* args /* host */, void* stream);
 
+/* ---- 8-bit activation checkpoints (no counterpart in the reference, which keeps every activation in fp32): 64 columns of a
+ *      row share a step 2^k, the smallest with max|x| <= 127 * 2^k, -126 <= k <= 121; codes int8 [rows][ld], ld = cols rounded up
+ *      to 64 (zeros behind cols); steps uint8 [rows][ld / 64], k + 127 (255: the group held an infinity or a NaN and reads as
+ *      NaN).  x, out, dout, dx: fp32, or bf16 with `bf16`; inputs with a row stride, any alignment, outputs contiguous; codes
+ *      16-byte aligned.  kind 0 gelu (erf), 1 silu, 2 leaky relu; act8_fwd without codes and
+ *      steps (both null) writes only out; act8_bwd: dx = dout * act'(values of the codes). ---- */
+int scp_pack8(const void* x, int bf16, long ldx, long rows, int cols, int8_t* codes, uint8_t* steps, void* stream);
+int scp_unpack8(const int8_t* codes, const uint8_t* steps, long rows, int cols, void* out, int bf16, void* stream);
+int scp_act8_fwd(const void* x, int bf16, long ldx, long rows, int cols, int kind, float slope, void* out, int8_t* codes,
+                 uint8_t* steps, void* stream);
+int scp_act8_bwd(const int8_t* codes, const uint8_t* steps, long rows, int cols, int kind, float slope, const void* dout,
+                 int bf16, long ldd, void* dx, void* stream);
+/* The products of a Linear layer that keeps its input as such a checkpoint.
+ * scp_gemm_bf16_c16: scp_gemm_bf16 (a_col 0, no mask) with a bf16 output; ws of scp_gemm_bf16_ws_floats(M, N, K, ldc) floats.
+ * scp_gemm_q8: C[m][n] = sum_k A[k][m] * value(codes, steps)[k][n], the weight gradient: A bf16 [K][lda] (lda % 8 == 0, 16-byte
+ * aligned), C fp32 or bf16 [M][ldc]; ws of scp_gemm_q8_ws_floats(M, N, K, max(lda, N rounded up to 64), ldc) floats.
+ * scp_pad_bf16: copy with rows padded by zeros to ldd = cols rounded up to 8.  scp_colsum_bf16: fp32 column sums. */
+int scp_gemm_bf16_c16(int a_col, int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb, void* C,
+                      long ldc, const float* bias, float* ws, void* stream);
+long scp_gemm_q8_ws_floats(int M, int N, int K, long ld, long ldc);
+int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const int8_t* codes, const uint8_t* steps, void* C, int c_bf16,
+                long ldc, float* ws, void* stream);
+int scp_pad_bf16(const void* src, long lds, long rows, int cols, void* dst, long ldd, void* stream);
+long scp_colsum_bf16_ws_floats(long rows, int cols);
+int scp_colsum_bf16(const void* x, long ldx, long rows, int cols, float* out, float* ws, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -126,6 +126,16 @@ _SIGS = {
     "scp_residual_norm_fwd": (I, [C.POINTER(ResidualNorm), P]),
     "scp_residual_norm_bwd_ws_floats": (L, [L, I]),
     "scp_residual_norm_bwd": (I, [C.POINTER(ResidualNorm), P]),
+    "scp_pack8": (I, [P, I, L, L, I, P, P, P]),
+    "scp_unpack8": (I, [P, P, L, I, P, I, P]),
+    "scp_act8_fwd": (I, [P, I, L, L, I, I, F, P, P, P, P]),
+    "scp_act8_bwd": (I, [P, P, L, I, I, F, P, I, L, P, P]),
+    "scp_gemm_bf16_c16": (I, [I, I, I, I, I, P, L, P, L, P, L, P, P, P]),
+    "scp_gemm_q8_ws_floats": (L, [I, I, I, L, L]),
+    "scp_gemm_q8": (I, [I, I, I, P, L, P, P, P, I, L, P, P]),
+    "scp_pad_bf16": (I, [P, L, L, I, P, L, P]),
+    "scp_colsum_bf16_ws_floats": (L, [L, I]),
+    "scp_colsum_bf16": (I, [P, L, L, I, P, P, P]),
     "scp_step_state_set": (I, [P, U64, F, F, P]),
 }
 

@@ -20,6 +20,7 @@
 // go round-robin over the 8 XCDs, so the id is remapped to give each XCD a contiguous run of tiles (the tiles that
 // share a B tile sit next to each other in one L2).
 #include <stdlib.h>
+#include "ckpt8.h"
 #include "common.h"
 #include "scpair_hip.h"
 
@@ -43,6 +44,7 @@ struct WgArgs {
   float* adam_m; float* adam_v; __bf16* adam_sh; long adam_ldsh;
   float lr, wd, b1, b2, eps, bc1, bc2, gscale;
   const float* bc_dev;       // optional device words {bias_corr1, bias_corr2} (HIP-graph replays), else bc1 / bc2
+  const uint8_t* steps;      // B in 8-bit checkpoint form: its step bytes [K][ldb / 64]
   unsigned dbg_oor;    // experiments only (SCPAIR_WGEMM_DBG=1): every load in the K loop out of range -> no memory traffic
 };
 
@@ -83,7 +85,12 @@ enum { EPI_SLAB = 0, EPI_DIRECT = 1, EPI_ADAMW = 2 };
 // NW = 8 (default for the plain products): two waves per SIMD, wave tile 128 x 64, one register set of prefetched tiles
 // (256 registers per lane): one wave's MFMA groups cover the other's waits.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
 // elsewhere): one wave per SIMD, wave tile 128 x 128, two register sets (loads two K-steps ahead).
-template <bool A_COL, bool B_COL, int EPI, int NW = 4>
+// BQ: the B operand (col) is an 8-bit activation checkpoint (ckpt8.hip): codes [K][ldb] int8 and one step byte per 64
+// columns.  A thread takes 16 codes with one 16-byte load, half the bytes of the bf16 operand, and takes them apart on the
+// way into LDS (a byte conversion and an fma per element, exact in bf16), where the image is that of a bf16 operand.  The
+// K-ranges are addressed from their own first row, so the operands of a long batch may pass 2 GiB as long as one range does not.
+// CT: type of the output (slabs are fp32 whatever it is).
+template <bool A_COL, bool B_COL, int EPI, int NW = 4, bool BQ = false, typename CT = float>
 __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   constexpr bool DIRECT = EPI == EPI_DIRECT;
   constexpr int NJ = NW == 4 ? 4 : 2, WN = 32 * NJ, CH = 32 / NW, LSTEP = 1024 * NW, NSET = NW == 4 ? 2 : 1;
@@ -104,8 +111,16 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   const int kt0 = z * g.ksteps_per_split;
   const int kt1 = min(nk_all, kt0 + g.ksteps_per_split);
 
-  const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc((void*)g.A, 0, (int)g.a_bytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc((void*)g.B, 0, (int)g.b_bytes, 0x00020000);
+  static_assert(!BQ || (A_COL && B_COL && NW == 8 && EPI != EPI_ADAMW), "8-bit operands: the weight gradient's form only");
+  // BQ: first row and rows of this K-range
+  const long krow0 = BQ ? (long)kt0 * TK : 0;
+  const long krows = min((long)g.K - krow0, (long)(kt1 - kt0) * TK);
+  const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(g.A + krow0 * g.lda), 0, BQ ? (int)(krows * g.lda * 2) : (int)g.a_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc(
+      BQ ? (void*)((const int8_t*)g.B + krow0 * g.ldb) : (void*)g.B, 0, BQ ? (int)(krows * g.ldb) : (int)g.b_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rsS = __builtin_amdgcn_make_buffer_rsrc(
+      BQ ? (void*)(g.steps + krow0 * (g.ldb >> 6)) : (void*)g.B, 0, BQ ? (int)(krows * (g.ldb >> 6)) : 0, 0x00020000);
   constexpr unsigned OOR = 0x80000000u;     // beyond any operand (host checks bytes < 2 GiB): the load returns zeros
 
   // chunk c = tid + 256 i.  row image: row (tid >> 3) + 32 i, chunk tid & 7; col image: k row (tid >> 5) + 8 i,
@@ -129,14 +144,30 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     offB[i] = baseB + stepB * i;
   }
 
+  // BQ: 16-code chunk i of this thread: row (tid >> 4) + 32 i of the K-step, columns 16 (tid & 15)
+  const int rQ = tid >> 4, cQ = tid & 15;
+  const unsigned baseQ = (unsigned)((long)rQ * g.ldb + n0 + 16 * cQ), baseS = (unsigned)((long)rQ * (g.ldb >> 6) + ((n0 + 16 * cQ) >> 6));
+  unsigned qs[2];
+
   // two register sets: the loads of K-step kt + 2 are issued during step kt and stored to LDS during step kt + 1,
   // so a load has more than a whole K-step (64 MFMAs) to arrive
   u32x4 ra[NSET][CH], rb[NSET][CH];
   auto load_tiles = [&](int kt, int set) {       // kt >= kt1: out of range, zeros
-    const int k0 = kt * TK;
+    const int k0 = (BQ ? kt - kt0 : kt) * TK;
     const unsigned dead = (kt < kt1 ? 0u : OOR) | g.dbg_oor;
     const unsigned kA = (A_COL ? (unsigned)((long)k0 * g.lda * 2) : ((k0 + 8 * cA < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
     const unsigned kB = (B_COL ? (unsigned)((long)k0 * g.ldb * 2) : ((k0 + 8 * cB < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
+    if constexpr (BQ) {
+#pragma unroll
+      for (int i = 0; i < CH; i++) ra[set][i] = ld128(rsA, offA[i] + kA);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const unsigned kq = (unsigned)(k0 + 32 * i);
+        rb[set][i] = ld128(rsB, baseQ + kq * (unsigned)g.ldb | dead);
+        qs[i] = __builtin_amdgcn_raw_buffer_load_b8(rsS, (int)(baseS + kq * (unsigned)(g.ldb >> 6) | dead), 0, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < CH; i++) {
       ra[set][i] = ld128(rsA, offA[i] + kA);
@@ -146,6 +177,27 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   auto store_tiles = [&](int stage, int set) {
     unsigned char* ia = smem + stage * STAGE_BYTES;
     unsigned char* ib = ia + TM * TK * 2;
+    if constexpr (BQ) {
+#pragma unroll
+      for (int i = 0; i < CH; i++) *(u32x4*)(ia + ldsA0 + LSTEP * i) = ra[set][i];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float step = q8_step(qs[i]), off = -128.f * step;
+        bf16x8 v[2];
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const unsigned u = rb[set][i][w] ^ 0x80808080u;      // code + 128: unsigned bytes convert in one instruction
+#pragma unroll
+          for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = (__bf16)fmaf((float)((u >> (8 * b)) & 0xffu), step, off);
+        }
+        // odd lanes write their second half first: the 16 lanes of a row then cover all banks in each of the two stores
+        unsigned char* p = ib + col_off(rQ + 32 * i, 16 * cQ);
+        const int odd = cQ & 1;
+        *(bf16x8*)(p + 16 * odd) = odd ? v[1] : v[0];
+        *(bf16x8*)(p + 16 - 16 * odd) = odd ? v[0] : v[1];
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < CH; i++) {
       *(u32x4*)(ia + ldsA0 + LSTEP * i) = ra[set][i];
@@ -315,6 +367,24 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     }
     return;
   }
+  if constexpr (sizeof(CT) == 2) {
+    static_assert(DIRECT, "slabs are fp32");
+    CT* C16 = (CT*)(void*)g.C;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int n = n0 + wn * WN + 32 * j + (lane & 31);
+      const float bn = (g.bias && n < g.N) ? g.bias[n] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int m = m0 + wm * 128 + 32 * i + acc_row(e, lane);
+          if (m < g.M && n < g.N) C16[(long)m * g.ldc + n] = (CT)(acc[i][j][e] + bn);
+        }
+      }
+    }
+    return;
+  }
   float* Cz = g.C + (DIRECT ? 0 : (long)z * g.M * g.ldc);
   if (m0 + TM <= g.M && n0 + TN <= g.N && !(DIRECT && g.mask)) {
     // interior tile: no tests; one store instruction writes two 128-byte row segments
@@ -386,9 +456,11 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
 }
 
 // C = sum of the K-range slabs in slab order, + bias, masked
+// (slabs and output share the row stride ldc)
+template <typename CT>
 __global__ __launch_bounds__(256) void wgemm_reduce_kernel(const float* __restrict__ slabs, int nsplit, int M, int N, long ldc,
                                                             const float* __restrict__ bias, const __bf16* __restrict__ mask,
-                                                            long ldm, float* __restrict__ C) {
+                                                            long ldm, CT* __restrict__ C) {
   const long n4 = (N + 3) / 4;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= (long)M * n4) return;
@@ -403,14 +475,19 @@ __global__ __launch_bounds__(256) void wgemm_reduce_kernel(const float* __restri
       if (bias) s[t] += bias[c + t];
       if (mask && !((float)mask[(long)m * ldm + c + t] > 0.f)) s[t] = 0.f;
     }
-    *(f32x4*)(C + (long)m * ldc + c) = s;
+    if constexpr (sizeof(CT) == 4) {
+      *(f32x4*)(C + (long)m * ldc + c) = s;
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; t++) C[(long)m * ldc + c + t] = (CT)s[t];
+    }
   } else {
     for (int t = 0; t < 4 && c + t < N; t++) {
       float s = p[t];
       for (int zz = 1; zz < nsplit; zz++) s += p[t + zz * slab];
       if (bias) s += bias[c + t];
       if (mask && !((float)mask[(long)m * ldm + c + t] > 0.f)) s = 0.f;
-      C[(long)m * ldc + c + t] = s;
+      C[(long)m * ldc + c + t] = (CT)s;
     }
   }
 }
@@ -470,6 +547,39 @@ int launch(const WgArgs& g, hipStream_t st) {
   }
   SCP_LAUNCH_CHECK();
   return SCP_OK;
+}
+
+// eight-wave forms with a bf16 output and / or an 8-bit B operand
+template <bool AC, bool BC, int EPI, bool BQ, typename CT>
+int launch8(const WgArgs& g, hipStream_t st) {
+  static uint64_t done = 0;
+  const void* fn = (const void*)wgemm_kernel<AC, BC, EPI, 8, BQ, CT>;
+  if (int rc = scp_set_smem(fn, 2 * STAGE_BYTES, &done)) return rc;
+  const int total = g.tiles_m * g.tiles_n * g.nsplit;
+  hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI, 8, BQ, CT>), dim3((unsigned)(((total + 7) / 8) * 8)), dim3(512), 2 * STAGE_BYTES,
+                     st, g);
+  SCP_LAUNCH_CHECK();
+  return SCP_OK;
+}
+
+template <typename CT>
+int reduce_slabs(const WgArgs& g, const float* ws, const float* bias, CT* C, hipStream_t st) {
+  const long n = (long)g.M * ((g.N + 3) / 4);
+  hipLaunchKernelGGL((wgemm_reduce_kernel<CT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, ws, g.nsplit, g.M, g.N,
+                     g.ldc, bias, nullptr, 0L, C);
+  SCP_LAUNCH_CHECK();
+  return SCP_OK;
+}
+
+// K-ranges of a product with an 8-bit operand: at least as many as keep a range's bytes below 1 GiB
+int q8_nsplit(int M, int N, int K, long lda) {
+  const int nk = (K + TK - 1) / TK;
+  long ns = pick_nsplit(M, N, K);
+  const long need = ((long)nk * TK * lda * 2 + (1L << 30) - 1) >> 30;
+  if (need > ns) ns = need;
+  // whole K-steps per range, no empty range
+  const long per = (nk + ns - 1) / ns;
+  return (int)((nk + per - 1) / per);
 }
 
 }  // namespace
@@ -591,9 +701,88 @@ extern "C" int scp_gemm_bf16(int a_col, int b_col, int M, int N, int K, const vo
   if (rc) return rc;
   if (g.nsplit > 1) {
     const long n = (long)M * ((N + 3) / 4);
-    hipLaunchKernelGGL(wgemm_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, ws, g.nsplit, M, N, ldc, bias,
+    hipLaunchKernelGGL((wgemm_reduce_kernel<float>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, ws, g.nsplit, M, N, ldc, bias,
                        (const __bf16*)mask, ldm, C);
     SCP_LAUNCH_CHECK();
   }
   return SCP_OK;
+}
+
+extern "C" int scp_gemm_bf16_c16(int a_col, int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb,
+                                 void* C, long ldc, const float* bias, float* ws, void* stream_) {
+  SCP_CHECK(M > 0 && N > 0 && K > 0, SCP_ERR_ARG, "scp_gemm_bf16_c16: M, N, K must be positive (%d, %d, %d)", M, N, K);
+  SCP_CHECK(A && B && C, SCP_ERR_ARG, "scp_gemm_bf16_c16: null pointer");
+  SCP_CHECK(a_col == 0 && (b_col == 0 || b_col == 1), SCP_ERR_ARG, "scp_gemm_bf16_c16: a_col must be 0, b_col 0 or 1");
+  const long b_rows = b_col ? K : N, b_cols = b_col ? N : K;
+  SCP_CHECK(lda >= ((K + 7) & ~7L) && ldb >= ((b_cols + 7) & ~7L) && ldc >= N, SCP_ERR_ARG,
+            "scp_gemm_bf16_c16: leading dimension too small (operands are padded to a multiple of 8 columns)");
+  SCP_CHECK(lda % 8 == 0 && ldb % 8 == 0 && ((uintptr_t)A & 15) == 0 && ((uintptr_t)B & 15) == 0, SCP_ERR_ARG,
+            "scp_gemm_bf16_c16: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
+  // the slack of scp_gemm_bf16: offset + dead-load mark must not carry out of 32 bits
+  SCP_CHECK((long)M * lda * 2 + 4096 < (1L << 31) && (b_rows + (b_col ? 3 * TK : 0)) * ldb * 2 + 4096 < (1L << 31), SCP_ERR_SHAPE,
+            "scp_gemm_bf16_c16: an operand within 3 K-steps of 2 GiB (or larger) is not supported");
+  WgArgs g = {};
+  g.A = (const __bf16*)A; g.B = (const __bf16*)B;
+  g.lda = lda; g.ldb = ldb; g.ldc = ldc;
+  g.M = M; g.N = N; g.K = K;
+  g.tiles_m = (M + TM - 1) / TM; g.tiles_n = (N + TN - 1) / TN;
+  g.nsplit = pick_nsplit(M, N, K);
+  g.ksteps_per_split = ((K + TK - 1) / TK + g.nsplit - 1) / g.nsplit;
+  g.a_bytes = (unsigned)((long)M * lda * 2);
+  g.b_bytes = (unsigned)(b_rows * ldb * 2);
+  SCP_CHECK((long)g.tiles_m * g.tiles_n * g.nsplit < (1L << 30), SCP_ERR_SHAPE, "scp_gemm_bf16_c16: too many tiles");
+  hipStream_t st = (hipStream_t)stream_;
+  if (g.nsplit == 1) {
+    g.C = (float*)C;
+    g.bias = bias;
+    return b_col ? launch8<false, true, EPI_DIRECT, false, __bf16>(g, st) : launch8<false, false, EPI_DIRECT, false, __bf16>(g, st);
+  }
+  SCP_CHECK(ws, SCP_ERR_ARG, "scp_gemm_bf16_c16: this shape runs as %d K-ranges and needs the workspace of scp_gemm_bf16_ws_floats",
+            g.nsplit);
+  g.C = ws;
+  const int rc = b_col ? launch8<false, true, EPI_SLAB, false, float>(g, st) : launch8<false, false, EPI_SLAB, false, float>(g, st);
+  return rc ? rc : reduce_slabs(g, ws, bias, (__bf16*)C, st);
+}
+
+extern "C" long scp_gemm_q8_ws_floats(int M, int N, int K, long lda, long ldc) {
+  if (M <= 0 || N <= 0 || K <= 0 || lda <= 0) return 0;
+  const int ns = q8_nsplit(M, N, K, lda);
+  return ns > 1 ? (long)ns * M * ldc : 0;
+}
+
+extern "C" int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const int8_t* codes, const uint8_t* steps, void* C,
+                           int c_bf16, long ldc, float* ws, void* stream_) {
+  SCP_CHECK(M > 0 && N > 0 && K > 0, SCP_ERR_ARG, "scp_gemm_q8: M, N, K must be positive (%d, %d, %d)", M, N, K);
+  SCP_CHECK(A && codes && steps && C, SCP_ERR_ARG, "scp_gemm_q8: null pointer");
+  const long ldb = (N + 63) / 64 * 64L;
+  SCP_CHECK(lda >= ((M + 7) & ~7L) && lda % 8 == 0 && ldc >= N, SCP_ERR_ARG,
+            "scp_gemm_q8: leading dimension too small or not a multiple of 8");
+  SCP_CHECK((((uintptr_t)A | (uintptr_t)codes) & 15) == 0, SCP_ERR_ARG, "scp_gemm_q8: operands must be 16-byte aligned");
+  WgArgs g = {};
+  g.A = (const __bf16*)A; g.B = (const __bf16*)(const void*)codes; g.steps = steps;
+  g.lda = lda; g.ldb = ldb; g.ldc = ldc;
+  g.M = M; g.N = N; g.K = K;
+  g.tiles_m = (M + TM - 1) / TM; g.tiles_n = (N + TN - 1) / TN;
+  g.nsplit = q8_nsplit(M, N, K, lda > ldb ? lda : ldb);
+  g.ksteps_per_split = ((K + TK - 1) / TK + g.nsplit - 1) / g.nsplit;
+  // offsets are formed in 32 bits within a K-range, up to three K-steps past its end, and the dead-load mark is bit 31
+  const long range = ((long)g.ksteps_per_split + 3) * TK;
+  SCP_CHECK(range * lda * 2 + 4096 < (1L << 31) && range * ldb + 4096 < (1L << 31), SCP_ERR_SHAPE,
+            "scp_gemm_q8: a K-range of %ld rows of %ld columns passes 2 GiB", range, lda > ldb ? lda : ldb);
+  SCP_CHECK((long)g.tiles_m * g.tiles_n * g.nsplit < (1L << 30), SCP_ERR_SHAPE, "scp_gemm_q8: too many tiles");
+  hipStream_t st = (hipStream_t)stream_;
+  if (g.nsplit == 1) {
+    g.C = (float*)C;
+    if (c_bf16) return launch8<true, true, EPI_DIRECT, true, __bf16>(g, st);
+    const long cb = (long)M * ldc * 4;
+    g.c_bytes = cb < (1L << 31) ? (unsigned)cb : 0u;
+    return launch8<true, true, EPI_DIRECT, true, float>(g, st);
+  }
+  SCP_CHECK(ws, SCP_ERR_ARG, "scp_gemm_q8: this shape runs as %d K-ranges and needs the workspace of scp_gemm_q8_ws_floats", g.nsplit);
+  g.C = ws;
+  const long cb = (long)M * ldc * 4;
+  g.c_bytes = cb < (1L << 31) ? (unsigned)cb : 0u;
+  const int rc = launch8<true, true, EPI_SLAB, true, float>(g, st);
+  if (rc) return rc;
+  return c_bf16 ? reduce_slabs(g, ws, nullptr, (__bf16*)C, st) : reduce_slabs(g, ws, nullptr, (float*)C, st);
 }

@@ -2252,3 +2252,251 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
     else:
         r, y, _ = _residual_norm_fwd(*tensors, cfg, False)
     return x if h is None else r.reshape(shape), y.reshape(shape)
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit activation checkpoints: an activation kept for the backward pass in 1 + 1/64 byte per element
+# ------------------------------------------------------------------------------------------------
+class Packed8:
+    """An activation in 8-bit checkpoint form: codes int8 [rows, ld] (ld = columns rounded up to 64), steps uint8
+    [rows, ld / 64].  The value of a code is code * 2**(step - 127); a step of 255 marks a group that held an infinity or a
+    NaN, whose 64 values read as NaN.  shape, dtype: those of the packed tensor."""
+    __slots__ = ("codes", "steps", "shape", "dtype")
+
+    def __init__(self, codes, steps, shape, dtype):
+        self.codes, self.steps, self.shape, self.dtype = codes, steps, shape, dtype
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.steps.numel()
+
+
+def _check_floats(what, t):
+    if not isinstance(t, torch.Tensor) or t.ndim == 0 or t.dtype not in _FLOATS:
+        raise ValueError(f"{what}: expected a float32 or bfloat16 tensor of at least one dimension, got "
+                         f"{f'{t.dtype} {tuple(t.shape)}' if isinstance(t, torch.Tensor) else type(t).__name__}")
+
+
+def _empty_packed(rows, cols, dev):
+    ld = (cols + 63) // 64 * 64
+    return (torch.empty((rows, ld), dtype=torch.int8, device=dev), torch.empty((rows, ld // 64), dtype=torch.uint8, device=dev))
+
+
+def _pack8_rows(x):
+    rows, cols = x.shape
+    codes, steps = _empty_packed(rows, cols, x.device)
+    if x.numel():
+        with _on(x.device):
+            _lib.check(_lib.lib().scp_pack8(x.data_ptr(), x.dtype == torch.bfloat16, x.stride(0), rows, cols, codes.data_ptr(),
+                                            steps.data_ptr(), _lib.stream()), "scp_pack8")
+    return codes, steps
+
+
+def _unpack8_rows(codes, steps, rows, cols, dtype):
+    out = torch.empty((rows, cols), dtype=dtype, device=codes.device)
+    if out.numel():
+        with _on(codes.device):
+            _lib.check(_lib.lib().scp_unpack8(codes.data_ptr(), steps.data_ptr(), rows, cols, out.data_ptr(),
+                                              dtype == torch.bfloat16, _lib.stream()), "scp_unpack8")
+    return out
+
+
+def pack8(x):
+    """The 8-bit checkpoint of a float32 or bfloat16 tensor [..., D] (a Packed8).  Every 64 columns of a row share a step
+    2^k, the smallest power of two with max|x| <= 127 * 2^k (k >= -126; k <= 121, where codes saturate); a code is x / 2^k
+    rounded to nearest even, so a value is off by at most max|x| / 127 of its group.  For autograd Functions of your own: no gradient flows through."""
+    _check_floats("pack8", x)
+    _same_device("pack8", x)
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else math.prod(x.shape[:-1])
+    codes, steps = _pack8_rows(_rows_of(x.detach(), cols)) if x.numel() else _empty_packed(rows, cols, x.device)
+    return Packed8(codes, steps, x.shape, x.dtype)
+
+
+def unpack8(p, dtype=None):
+    """The tensor that a Packed8 stands for, in `dtype` (float32 or bfloat16: both hold every value exactly, down to
+    bfloat16's subnormals; the packed tensor's own type by default)."""
+    if not isinstance(p, Packed8):
+        raise ValueError(f"unpack8: expected a Packed8, got {type(p).__name__}")
+    dtype = dtype or p.dtype
+    if dtype not in _FLOATS:
+        raise ValueError(f"unpack8: float32 or bfloat16, got {dtype}")
+    _same_device("unpack8", p.codes, p.steps)
+    return _unpack8_rows(p.codes, p.steps, p.codes.shape[0], p.shape[-1], dtype).reshape(p.shape)
+
+
+_ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
+
+
+def _act8_fwd(z, kind, slope, keep):
+    rows, cols = z.shape
+    out = torch.empty((rows, cols), dtype=z.dtype, device=z.device)
+    codes, steps = _empty_packed(rows, cols, z.device) if keep else (None, None)
+    with _on(z.device):
+        _lib.check(_lib.lib().scp_act8_fwd(z.data_ptr(), z.dtype == torch.bfloat16, z.stride(0), rows, cols, kind, slope,
+                                           out.data_ptr(), _lib.ptr(codes), _lib.ptr(steps), _lib.stream()), "scp_act8_fwd")
+    return out, codes, steps
+
+
+class Act8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, kind, slope):
+        out, codes, steps = _act8_fwd(z, kind, slope, True)
+        ctx.save_for_backward(codes, steps)
+        ctx.cfg = (*z.shape, kind, slope)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        codes, steps = ctx.saved_tensors
+        rows, cols, kind, slope = ctx.cfg
+        dz = torch.empty((rows, cols), dtype=dout.dtype, device=dout.device)
+        dout = _rows_of(dout, cols)
+        with _on(dout.device):
+            _lib.check(_lib.lib().scp_act8_bwd(codes.data_ptr(), steps.data_ptr(), rows, cols, kind, slope, dout.data_ptr(),
+                                               dout.dtype == torch.bfloat16, dout.stride(0), dz.data_ptr(), _lib.stream()),
+                       "scp_act8_bwd")
+        return dz, None, None
+
+
+def act8(z, kind="gelu", slope=0.01):
+    """act(z) for z [..., D] float32 or bfloat16, keeping z for the backward pass as an 8-bit checkpoint that the same launch
+    writes: dz = dout * act'(unpack8(pack8(z))).  kind: 'gelu' (the erf form), 'silu', or 'leaky_relu' (slope; 0 is relu; a
+    value whose code is 0 counts as not positive)."""
+    _check_floats("act8", z)
+    if kind not in _ACTS8:
+        raise ValueError(f"act8: kind must be one of {sorted(_ACTS8)}, got {kind!r}")
+    _same_device("act8", z)
+    if z.numel() == 0:
+        return z.clone()
+    rows = _rows_of(z, z.shape[-1])
+    if torch.is_grad_enabled() and z.requires_grad:
+        return Act8Fn.apply(rows, _ACTS8[kind], float(slope)).reshape(z.shape)
+    return _act8_fwd(rows, _ACTS8[kind], float(slope), False)[0].reshape(z.shape)
+
+
+def _bf16_operand(t):
+    """t [rows, cols] (bfloat16 or float32) as the matrix kernels take it: bfloat16, rows of a multiple of 8 elements from a
+    16-byte boundary, zeros behind the columns.  t itself where it is that already."""
+    rows, cols = t.shape
+    if t.dtype == torch.float32:
+        return cast_bf16(t if t.is_contiguous() else t.contiguous(), rows, cols)
+    if cols % 8 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    out = torch.empty((rows, (cols + 7) // 8 * 8), dtype=torch.bfloat16, device=t.device)
+    _lib.check(_lib.lib().scp_pad_bf16(t.data_ptr(), t.stride(0), rows, cols, out.data_ptr(), out.shape[1], _lib.stream()),
+               "scp_pad_bf16")
+    return out
+
+
+def _rows_gemm(b_col, a, B, n, k, out, bias=None):
+    """out[rows, n] = a B^T (b_col 0) or a B (b_col 1), + bias; bf16 operands of _bf16_operand, bf16 or fp32 out.  The kernels
+    address an operand with 31 bits, so a longer batch runs in pieces."""
+    L = _lib.lib()
+    rows, lda = a.shape
+    piece = ((1 << 31) - 8192) // (2 * lda)
+    for r0 in range(0, rows, piece):
+        m = min(piece, rows - r0)
+        ai, oi = a[r0:r0 + m], out[r0:r0 + m]
+        if out.dtype == torch.float32:
+            gemm_bf16(0, b_col, m, n, k, ai, lda, B, B.shape[1], oi, n, bias=bias)
+            continue
+        nws = L.scp_gemm_bf16_ws_floats(m, n, k, n)
+        ws = torch.empty((nws,), dtype=torch.float32, device=a.device) if nws else None
+        _lib.check(L.scp_gemm_bf16_c16(0, b_col, m, n, k, ai.data_ptr(), lda, B.data_ptr(), B.shape[1], oi.data_ptr(), n,
+                                       _lib.ptr(bias), _lib.ptr(ws), _lib.stream()), "scp_gemm_bf16_c16")
+
+
+def _linear8_fwd(x, W, b, split):
+    M, K = x.shape
+    N = W.shape[0]
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    if M:
+        with _on(x.device):
+            if split:
+                xc, Wc = _f32c(x), _f32c(W)
+                gemm_nt_auto(M, N, K, xc, K, 1, Wc, K, 1, y, bias=b)
+            else:
+                _rows_gemm(0, _bf16_operand(x), _bf16_operand(W), N, K, y, bias=b)
+    return y
+
+
+class Linear8Fn(torch.autograd.Function):
+    """y = x W^T + b for 2-D x; keeps x as an 8-bit checkpoint and W.  bf16 operands: the wide MFMA kernels (csrc/wgemm.hip),
+    the weight gradient reading the codes; fp32 tensors in precision 'fp32': the split products (csrc/gemm.hip)."""
+
+    @staticmethod
+    def forward(ctx, x, W, b, split):
+        ctx.split, ctx.dims = split, (x.shape[0], *W.shape)
+        codes, steps = _pack8_rows(x) if ctx.needs_input_grad[1] else (None, None)
+        ctx.save_for_backward(codes, steps, W)
+        return _linear8_fwd(x, W, b, split)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        codes, steps, W = ctx.saved_tensors
+        M, N, K = ctx.dims
+        L = _lib.lib()
+        dx = dW = db = None
+        dy = _rows_of(dy, N)
+        with _on(dy.device):
+            if ctx.needs_input_grad[0]:
+                dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+            if ctx.needs_input_grad[1]:
+                dW = torch.empty((N, K), dtype=W.dtype, device=dy.device)
+            if ctx.needs_input_grad[2]:
+                db = torch.empty((N,), dtype=torch.float32, device=dy.device)
+            if M == 0:
+                return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_(), None
+            if ctx.split:
+                d, Wc = _f32c(dy), _f32c(W)
+                if dx is not None:
+                    gemm_nt_auto(M, K, N, d, N, 1, Wc, 1, K, dx)
+                if dW is not None:
+                    gemm_nt_auto(N, K, M, d, 1, N, _unpack8_rows(codes, steps, M, K, torch.float32), 1, K, dW)
+            else:
+                d = _bf16_operand(dy)
+                if dx is not None:
+                    _rows_gemm(1, d, _bf16_operand(W), K, N, dx)
+                if dW is not None:
+                    nws = L.scp_gemm_q8_ws_floats(N, K, M, max(d.shape[1], codes.shape[1]), K)
+                    ws = torch.empty((nws,), dtype=torch.float32, device=dy.device) if nws else None
+                    _lib.check(L.scp_gemm_q8(N, K, M, d.data_ptr(), d.shape[1], codes.data_ptr(), steps.data_ptr(), dW.data_ptr(),
+                                             dW.dtype == torch.bfloat16, K, _lib.ptr(ws), _lib.stream()), "scp_gemm_q8")
+            if db is not None:
+                if dy.dtype == torch.bfloat16:
+                    ws = torch.empty((L.scp_colsum_bf16_ws_floats(M, N),), dtype=torch.float32, device=dy.device)
+                    _lib.check(L.scp_colsum_bf16(dy.data_ptr(), dy.stride(0), M, N, db.data_ptr(), ws.data_ptr(), _lib.stream()),
+                               "scp_colsum_bf16")
+                else:
+                    db = colsum(dy, M, N, ld=dy.stride(0))
+        return dx, dW, db, None
+
+
+def linear8(x, W, b=None):
+    """y = x W^T + b for x [..., K], W [N, K], b [N], keeping x for the backward pass as an 8-bit checkpoint: dW = dy^T
+    unpack8(pack8(x)), while y, dx and db are what linear gives.  x float32 with W float32: y float32, products in the
+    precision of set_precision.  x bfloat16 with W bfloat16 or float32 (rounded once per call): y bfloat16, bf16 products
+    with fp32 sums; dW has W's type.  b may have any floating-point type.  W and its gradient stay below 2 GiB of bf16."""
+    _check_floats("linear8", x)
+    _check_floats("linear8", W)
+    K = x.shape[-1]
+    if W.ndim != 2 or W.shape[1] != K or K < 1 or W.shape[0] < 1:
+        raise ValueError(f"linear8: x of {K} columns needs a weight [outputs, {K}], got {tuple(W.shape)}")
+    if x.dtype == torch.float32 and W.dtype != torch.float32:
+        raise ValueError("linear8: a float32 input needs a float32 weight")
+    N = W.shape[0]
+    if b is not None and (b.shape != (N,) or not b.is_floating_point()):
+        raise ValueError(f"linear8: the bias must be a floating-point tensor of shape ({N},), got {b.dtype} {tuple(b.shape)}")
+    if (max(N, K) + 256) * (min(N, K) + 256) * 2 >= (1 << 31) - 4096:
+        raise ValueError(f"linear8: a weight of {N} x {K} passes 2 GiB in bfloat16")
+    _same_device("linear8", x, W, b)
+    x2, W, b = _rows_of(x, K), W if W.is_contiguous() else W.contiguous(), None if b is None else _f32c(b)
+    split = x.dtype == torch.float32 and _ns() == 3
+    if torch.is_grad_enabled() and (x.requires_grad or W.requires_grad or (b is not None and b.requires_grad)):
+        y = Linear8Fn.apply(x2, W, b, split)
+    else:
+        y = _linear8_fwd(x2, W, b, split)
+    return y.reshape(*x.shape[:-1], N)

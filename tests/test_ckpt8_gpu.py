@@ -1,0 +1,333 @@
+"""8-bit activation checkpoints (csrc/ckpt8.hip, the q8 form of csrc/wgemm.hip) against their definition in 64 bits on the
+CPU.
+
+Tolerances.  Packing is exact by its definition (power-of-two steps), so codes, steps and unpacked values are compared bit
+for bit.  Activations: one fp32 evaluation of some 20 operations on values of order |z|, 32 * 2^-24 * max(|z|, 1) * |dout|, and half a step of
+the output's type.  Products of K bf16 terms are exact in fp32, their sum in fp32 is off by at most sqrt-free bound
+K * 2^-24 * sum|terms| in the worst order; the blocked order of the kernels (64-deep tiles into one accumulator) keeps it
+below (K / 16 + 16) * 2^-24 * sum |a b|, which is computed from the operands' absolute values; the fp32 mode's operand
+split leaves 2^-22 per product on top.  Outputs held in bf16: half a step, 2^-8 relative."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, B16 = torch.float32, torch.bfloat16
+E = 2.0 ** -24
+
+
+def pack_ref(x):
+    """codes, steps (as the kernels store them) and values in float64 of a 2-D CPU tensor"""
+    rows, cols = x.shape
+    ld = (cols + 63) // 64 * 64
+    t = torch.zeros(rows, ld, dtype=torch.float64)
+    t[:, :cols] = x.double()
+    t = t.reshape(rows, ld // 64, 64)
+    bad = ~torch.isfinite(t).all(2)
+    top = torch.where(torch.isfinite(t), t.abs(), 0.0).amax(2)
+    k = torch.full_like(top, -126, dtype=torch.int64)
+    for p in range(-126, 121):                       # the smallest k <= 121 with top <= 127 * 2^k
+        k = torch.where(top > 127.0 * 2.0 ** p, p + 1, k)
+    step = ((k + 1023) << 52).view(torch.float64)
+    c = torch.round(t / step[..., None]).clamp(-127, 127)
+    c = torch.where(bad[..., None], 0.0, c)
+    v = torch.where(bad[..., None], float("nan"), c * step[..., None])
+    return (c.reshape(rows, ld).to(torch.int8), torch.where(bad, 255, k + 127).to(torch.uint8), v.reshape(rows, ld)[:, :cols])
+
+
+def rand(rows, cols, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(2 * torch.randn(rows, 1, generator=g))
+    x[:, ::37] *= 20
+    return x.to(dtype)
+
+
+SHAPES = [(1, 1), (1, 64), (3, 7), (5, 63), (5, 65), (2, 128), (130, 200), (33, 901), (257, 1800), (4, 20001), (5000, 64)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [F32, B16])
+def test_pack_and_unpack_are_exact(shape, dtype):
+    from scpair_amd import ops
+    x = rand(*shape, dtype, sum(shape))
+    p = ops.pack8(x.cuda())
+    codes, steps, v = pack_ref(x)
+    assert torch.equal(p.codes.cpu(), codes) and torch.equal(p.steps.cpu(), steps)
+    assert p.nbytes == codes.numel() + steps.numel() and p.shape == x.shape and p.dtype == dtype
+    for t in (F32, B16):
+        out = ops.unpack8(p, t)
+        assert out.dtype == t and torch.equal(out.cpu().double(), v)
+    assert torch.equal(ops.unpack8(p).cpu().double(), v) and ops.unpack8(p).dtype == dtype
+    # packing what was unpacked changes nothing
+    assert torch.equal(ops.unpack8(ops.pack8(ops.unpack8(p))).cpu().double(), v)
+
+
+def test_pack_borders_of_the_step():
+    """Maxima on both sides of 127 * 2^k, ties, zeros, the smallest and largest magnitudes."""
+    from scpair_amd import ops
+    rows = []
+    for top in (127.0, math.nextafter(127.0, 200) and 127.00001, 126.99999, 128.0, 64.0, 1.0, 1.984375, 1.9843751, 3.0e38,
+                3.4028234e38, 1e-38, 1.2e-38, 1e-40, 1e-45, 127 * 2.0 ** -126, 128 * 2.0 ** -126, 0.0):
+        r = torch.linspace(-1, 1, 64) * 0.9
+        r = (r * top).float()
+        r[5], r[6] = top, -top
+        rows.append(r)
+    ties = torch.arange(-64, 0).float() + 0.5
+    ties[0] = 127.0
+    rows.append(ties)
+    x = torch.stack(rows)
+    codes, steps, v = pack_ref(x)
+    p = ops.pack8(x.cuda())
+    assert torch.equal(p.steps.cpu(), steps)
+    assert torch.equal(p.codes.cpu(), codes)
+    assert torch.equal(ops.unpack8(p).cpu().double(), v)
+
+
+def test_non_finite_groups_read_as_nan():
+    from scpair_amd import ops
+    x = rand(6, 200, F32, 3)
+    x[0, 3], x[1, 70], x[2, 199], x[3, 128] = float("nan"), float("inf"), -float("inf"), float("nan")
+    codes, steps, v = pack_ref(x)
+    p = ops.pack8(x.cuda())
+    assert torch.equal(p.codes.cpu(), codes) and torch.equal(p.steps.cpu(), steps)
+    out = ops.unpack8(p).cpu().double()
+    assert torch.equal(out.isnan(), v.isnan()) and torch.equal(out.nan_to_num(), v.nan_to_num())
+
+
+def test_pack_strides_shapes_and_empty():
+    from scpair_amd import ops
+    wide = rand(40, 333, B16, 4)
+    for view in (wide[:, 5:205], wide[::2, 1:], wide.t(), wide[3:4].expand(7, 333), wide.reshape(8, 5, 333), wide[0]):
+        dense = view.contiguous()
+        got = ops.unpack8(ops.pack8(view.cuda() if view.is_contiguous() else _as_laid_out(view)))
+        assert got.shape == view.shape
+        want = pack_ref(dense.reshape(-1, dense.shape[-1]))[2].reshape(dense.shape)
+        assert torch.equal(got.cpu().double(), want)
+    for shape in ((0, 5), (5, 0), (0, 0)):
+        assert ops.unpack8(ops.pack8(torch.empty(shape, device="cuda"))).shape == shape
+
+
+def _as_laid_out(view):
+    """the same view on the GPU (strides kept)"""
+    base = view._base.cuda()
+    return torch.as_strided(base, view.size(), view.stride(), view.storage_offset())
+
+
+def act_ref(z, kind, slope):
+    if kind == "gelu":
+        return z * torch.special.ndtr(z)
+    if kind == "silu":
+        return z * torch.sigmoid(z)
+    return torch.where(z > 0, z, slope * z)
+
+
+def act_slope_ref(v, kind, slope):
+    if kind == "gelu":
+        return torch.special.ndtr(v) + v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+    if kind == "silu":
+        return torch.sigmoid(v) * (1 + v * torch.sigmoid(-v))
+    return torch.where(v > 0, 1.0, slope)
+
+
+def half_step(want, dtype):
+    return want.abs() * (2.0 ** -8 if dtype == B16 else E)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (33, 901), (130, 1024), (2, 5, 70)])
+@pytest.mark.parametrize("kind,slope", [("gelu", 0.0), ("silu", 0.0), ("leaky_relu", 0.01), ("leaky_relu", 0.0)])
+@pytest.mark.parametrize("dtype", [F32, B16])
+def test_act8(shape, kind, slope, dtype):
+    from scpair_amd import ops
+    g = torch.Generator().manual_seed(5)
+    z, up = (3 * torch.randn(shape, generator=g)).to(dtype), torch.randn(shape, generator=g).to(dtype)
+    zg = z.cuda().requires_grad_()
+    a = ops.act8(zg, kind, slope)
+    want = act_ref(z.double(), kind, slope)
+    assert a.dtype == dtype and a.shape == z.shape
+    assert ((a.detach().cpu().double() - want).abs() <= 32 * E * z.double().abs().clamp(min=1) + half_step(want, dtype)).all()
+    dz, = torch.autograd.grad(a, zg, up.cuda())
+    v = pack_ref(z.reshape(-1, shape[-1]))[2].reshape(shape)
+    want = up.double() * act_slope_ref(v, kind, slope)
+    assert dz.dtype == dtype
+    assert ((dz.cpu().double() - want).abs() <= 32 * E * up.double().abs() * v.abs().clamp(min=1) + half_step(want, dtype)).all()
+    with torch.no_grad():
+        assert torch.equal(ops.act8(zg, kind, slope), a)
+
+
+def test_act8_extremes():
+    """Large magnitudes neither overflow nor lose their sign; an infinity gives its own limit forward and NaN backward."""
+    from scpair_amd import ops
+    z = torch.tensor([[-3e38, -1e4, -100.0, -20.0, 0.0, 20.0, 100.0, 1e4, 3e38]])
+    for kind in ("gelu", "silu"):
+        a = ops.act8(z.cuda(), kind).cpu()
+        assert torch.isfinite(a).all() and (a[0, 5:] == z[0, 5:]).all() and (a[0, :4].abs() <= 1e-7).all()
+    x = torch.zeros(2, 64)
+    x[0, 1] = float("inf")
+    xg = x.cuda().requires_grad_()
+    a = ops.act8(xg, "silu")
+    assert a[0, 1] == float("inf")
+    d, = torch.autograd.grad(a.sum(), xg)
+    assert d[0].isnan().all() and torch.isfinite(d[1]).all()
+
+
+def bound(a, b, k):
+    return (k / 16 + 16) * E * (a.abs() @ b.abs())
+
+
+LINEARS = [(1, 1, 1), (1, 8, 5), (3, 65, 7), (64, 64, 64), (130, 901, 33), (257, 300, 517), (777, 1801, 901), (1024, 900, 1800),
+           (2049, 72, 264), (5000, 130, 70)]
+
+
+@pytest.mark.parametrize("M,K,N", LINEARS)
+@pytest.mark.parametrize("xt,wt,mode", [(B16, B16, "fp32"), (B16, F32, "fp32"), (F32, F32, "fp32"), (F32, F32, "bf16")])
+@pytest.mark.parametrize("bias", [True, False])
+def test_linear8(M, K, N, xt, wt, mode, bias):
+    from scpair_amd import ops
+    g = torch.Generator().manual_seed(M + K + N)
+    x, W = rand(M, K, xt, M), (torch.randn(N, K, generator=g) / math.sqrt(K)).to(wt)
+    x = x.clamp(-50, 50)
+    b = 0.1 * torch.randn(N, generator=g) if bias else None
+    up = torch.randn(M, N, generator=g).to(xt)
+    old = ops.get_precision()
+    ops.set_precision(mode)
+    try:
+        leaves = [t.cuda().requires_grad_() for t in (x, W, b) if t is not None]
+        y = ops.linear8(*leaves)
+        grads = torch.autograd.grad(y, leaves, up.cuda())
+        again = torch.autograd.grad(ops.linear8(*leaves), leaves, up.cuda())
+        with torch.no_grad():
+            assert torch.equal(ops.linear8(*leaves), y)
+    finally:
+        ops.set_precision(old)
+    for a, c in zip(grads, again):
+        assert torch.equal(a, c)
+    narrow = xt == B16 or mode == "bf16"                  # products of bf16 operands
+    r = (lambda t: t.to(B16).double()) if narrow else (lambda t: t.double())
+    v = pack_ref(x)[2]
+    split = 0.0 if narrow else 2.0 ** -22
+    xr, Wr, ur = r(x), r(W), r(up)
+
+    def close(name, got, want, err, dtype):
+        assert got.dtype == dtype and got.shape == want.shape, name
+        over = (got.detach().cpu().double() - want).abs() - err - (half_step(want, dtype) if dtype == B16 else E * want.abs())
+        assert over.max().item() <= 0, f"{name}: {(got.detach().cpu().double() - want).abs().max().item()}"
+
+    want = xr @ Wr.t() + (b.double() if bias else 0)
+    close("y", y, want, bound(xr, Wr.t(), K) + split * (xr.abs() @ Wr.t().abs()) + 4 * E, xt)
+    close("dx", grads[0], ur @ Wr, bound(ur, Wr, N) + split * (ur.abs() @ Wr.abs()), xt)
+    close("dW", grads[1], ur.t() @ v, bound(ur.t(), v, M) + split * (ur.t().abs() @ v.abs()), wt)
+    if bias:
+        close("db", grads[2], up.double().sum(0), (M / 16 + 16) * E * up.double().abs().sum(0), F32)
+
+
+def test_linear8_layouts_and_partial_gradients():
+    from scpair_amd import ops
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(60, 150, generator=g).to(B16).cuda()
+    W = torch.randn(40, 96, generator=g).to(B16).cuda()
+    base = ops.linear8(wide[:, 7:103].contiguous(), W)
+    assert torch.equal(ops.linear8(wide[:, 7:103], W), base)
+    assert torch.equal(ops.linear8(wide[:, 7:103].reshape(3, 20, 96), W).reshape(60, 40), base)
+    assert torch.equal(ops.linear8(wide[:, 7:103], W.t().contiguous().t()), base)
+    assert torch.equal(ops.linear8(wide[:, 7:103].t().contiguous().t(), W), base)
+    x = wide[:, 7:103].clone().requires_grad_()
+    Wl, b = W.clone().requires_grad_(), torch.zeros(40, dtype=B16, device="cuda", requires_grad=True)
+    y = ops.linear8(x, Wl, b)
+    dx, dW, db = torch.autograd.grad(y.float().sum(), (x, Wl, b))
+    assert db.dtype == B16 and torch.equal(db.cpu(), torch.full((40,), 60.0, dtype=B16))
+    xs = wide[:, 7:103].clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.linear8(xs, W).float().sum(), xs)[0], dx)
+    assert torch.equal(torch.autograd.grad(ops.linear8(wide[:, 7:103], Wl).float().sum(), Wl)[0], dW)
+
+
+def test_linear8_keeps_one_byte_per_element():
+    from scpair_amd import ops
+    W = torch.zeros(64, 4096, dtype=B16, device="cuda", requires_grad=True)
+    x = torch.zeros(4096, 4096, dtype=B16, device="cuda")
+    y = ops.linear8(x, W)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    del x
+    assert before - torch.cuda.memory_allocated() == 4096 * 4096 * 2       # the input is free to go
+    kept = torch.cuda.memory_allocated()
+    del y
+    assert kept - torch.cuda.memory_allocated() <= 4096 * 4096 * (1 + 1 / 64) + 4096 * 64 * 2 + 4096
+
+
+def test_linear8_empty_batch_and_non_finite():
+    from scpair_amd import ops
+    W = torch.randn(40, 96, device="cuda").to(B16).requires_grad_()
+    x = torch.empty(0, 96, dtype=B16, device="cuda", requires_grad=True)
+    y = ops.linear8(x, W)
+    assert y.shape == (0, 40)
+    dx, dW = torch.autograd.grad(y.sum(), (x, W))
+    assert dx.shape == (0, 96) and not dW.any()
+    x = torch.randn(300, 200, device="cuda").to(B16)
+    W = torch.randn(40, 200, device="cuda").to(B16).requires_grad_()
+    x[123, 70] = float("inf")
+    dW, = torch.autograd.grad(ops.linear8(x, W).float().sum(), W, retain_graph=False)
+    assert dW[:, 64:128].isnan().all() and torch.isfinite(dW[:, :64]).all() and torch.isfinite(dW[:, 128:]).all()
+
+
+def test_linear8_long_batch():
+    """More than 2 GiB of input: forward and dx run in pieces, the weight gradient in K-ranges with their own base."""
+    from scpair_amd import ops
+    M, K, N = 1_100_000, 1024, 24
+    x = torch.zeros(M, K, dtype=B16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for r in (0, 600_000, M - 130):
+        x[r:r + 130] = torch.randn(130, K, generator=g, device="cuda").to(B16)
+    W = torch.randn(N, K, generator=g, device="cuda").to(B16).requires_grad_()
+    up = torch.zeros(M, N, dtype=B16, device="cuda")
+    for r in (0, 600_000, M - 130):
+        up[r:r + 130] = torch.randn(130, N, generator=g, device="cuda").to(B16)
+    x.requires_grad_()
+    y = ops.linear8(x, W)
+    dx, dW = torch.autograd.grad(y, (x, W), up)
+    pick = torch.cat([torch.arange(r, r + 130) for r in (0, 600_000, M - 130)]).cuda()
+    xs, us = x.detach()[pick].cpu(), up[pick].cpu().double()
+    Wd = W.detach().cpu().double()
+    for got, want, err in ((y.detach()[pick], xs.double() @ Wd.t(), bound(xs.double(), Wd.t(), K)),
+                           (dx[pick], us @ Wd, bound(us, Wd, N)),
+                           (dW, us.t() @ pack_ref(xs)[2], bound(us.t(), pack_ref(xs)[2], 390))):
+        got = got.cpu().double()
+        assert ((got - want).abs() <= err + half_step(want, B16)).all()
+    assert not y.detach()[200:600_000].any() and not dx[700_000:M - 130].any()
+
+
+def test_captured_and_replayed():
+    """A residual block's two Linears and its activation, forward and backward, captured once and replayed on new values."""
+    from scpair_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda").to(B16)
+    batches = [(rn(300, 200), rn(300, 200)) for _ in range(3)]
+    params = [rn(520, 200), rn(520).float(), rn(200, 520)]
+
+    def step(x, up, W1, b1, W2):
+        y = ops.linear8(ops.act8(ops.linear8(x, W1, b1), "gelu"), W2)
+        return [y.detach(), *torch.autograd.grad(y, (x, W1, b1, W2), up)]
+
+    def leaves(x, up):
+        return [x.clone().requires_grad_(), up.clone(), *(p.clone().requires_grad_() for p in params)]
+
+    held = leaves(*batches[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*held)
+    for batch in batches:
+        with torch.no_grad():
+            for t, v in zip(held, batch):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        for a, b in zip(got, step(*leaves(*batch))):
+            assert torch.equal(a, b)

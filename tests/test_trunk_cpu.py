@@ -72,3 +72,58 @@ def test_residual_norm_c_entry_refuses():
         assert L.scp_residual_norm_bwd(args(**bad), None) == -1, bad
     assert L.scp_residual_norm_bwd_ws_floats(0, 8) == 0
     assert L.scp_residual_norm_bwd_ws_floats(1, 900) == 5 * 900
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.pack8(torch.zeros(())),
+    lambda: ops.pack8(torch.zeros(3, 4, dtype=torch.float16)),
+    lambda: ops.pack8(3.0),
+    lambda: ops.unpack8(torch.zeros(3)),
+    lambda: ops.unpack8(ops.Packed8(torch.zeros(1, 64, dtype=torch.int8), torch.zeros(1, 1, dtype=torch.uint8), (1, 64),
+                                    torch.float32), torch.float64),
+    lambda: ops.act8(torch.zeros(3, 4, dtype=torch.float64)),
+    lambda: ops.act8(torch.zeros(3, 4), "tanh"),
+    lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(5, 3)),
+    lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(4)),
+    lambda: ops.linear8(torch.zeros(3, 0), torch.zeros(5, 0)),
+    lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(0, 4)),
+    lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(5, 4, dtype=torch.bfloat16)),
+    lambda: ops.linear8(torch.zeros(3, 4, dtype=torch.float16), torch.zeros(5, 4)),
+    lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(4)),
+    lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(5, dtype=torch.int64)),
+    lambda: ops.linear8(torch.zeros(1, 32768), torch.zeros(1).expand(32768, 32768)),
+])
+def test_checkpoint_operators_refuse(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+@pytest.mark.parametrize("call", [lambda: ops.pack8(X), lambda: ops.act8(X), lambda: ops.linear8(X, torch.zeros(5, 8))])
+def test_checkpoint_operators_have_no_cpu_path(call):
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        call()
+
+
+def test_checkpoint_c_entries_refuse():
+    L = _lib.lib()
+    a = 4096
+    assert L.scp_pack8(None, 0, 8, 2, 8, a, a, None) == -1 and L.scp_pack8(a, 0, 8, 0, 8, a, a, None) == -1
+    assert L.scp_pack8(a, 0, 8, 2, 8, a + 1, a, None) == -1 and L.scp_pack8(a, 0, -8, 2, 8, a, a, None) == -1
+    assert L.scp_pack8(a, 0, 8, 2, (1 << 24) + 1, a, a, None) == -2
+    assert L.scp_unpack8(a, None, 2, 8, a, 0, None) == -1 and L.scp_unpack8(a, a, 2, 8, None, 0, None) == -1
+    assert L.scp_act8_fwd(a, 0, 8, 2, 8, 3, 0.0, a, a, a, None) == -1 and L.scp_act8_fwd(a, 0, 8, 2, 8, 0, 0.0, a, a, None, None) == -1
+    assert L.scp_act8_bwd(a, a, 2, 8, -1, 0.0, a, 0, 8, a, None) == -1 and L.scp_act8_bwd(a, a, 2, 8, 0, 0.0, None, 0, 8, a, None) == -1
+    assert L.scp_gemm_bf16_c16(1, 0, 8, 8, 8, a, 8, a, 8, a, 8, None, None, None) == -1
+    assert L.scp_gemm_bf16_c16(0, 0, 8, 8, 9, a, 8, a, 16, a, 8, None, None, None) == -1
+    assert L.scp_gemm_bf16_c16(0, 0, 8, 8, 8, a + 2, 8, a, 8, a, 8, None, None, None) == -1
+    assert L.scp_gemm_bf16_c16(0, 0, 1 << 20, 8, 1024, a, 1024, a, 1024, a, 8, None, None, None) == -2
+    assert L.scp_gemm_q8(8, 8, 8, a, 8, a, None, a, 0, 8, None, None) == -1
+    assert L.scp_gemm_q8(9, 8, 8, a, 8, a, a, a, 0, 8, None, None) == -1
+    assert L.scp_gemm_q8(8, 8, 8, a, 12, a, a, a, 0, 8, None, None) == -1
+    assert L.scp_gemm_q8(8, 8, 8, a, 8, a, a, a, 0, 7, None, None) == -1
+    # a batch of 4 M rows needs K-ranges below 2 GiB, hence slabs
+    assert L.scp_gemm_q8_ws_floats(1024, 1024, 4_000_000, 1024, 1024) >= 8 * 1024 * 1024
+    assert L.scp_gemm_q8(1024, 1024, 4_000_000, a, 1024, a, a, a, 0, 1024, None, None) == -1
+    assert b"workspace" in L.scp_last_error()
+    assert L.scp_pad_bf16(a, 9, 2, 9, a, 9, None) == -1 and L.scp_pad_bf16(None, 9, 2, 9, a, 16, None) == -1
+    assert L.scp_colsum_bf16(a, 8, 2, 8, a, None, None) == -1 and L.scp_colsum_bf16_ws_floats(0, 8) == 0
