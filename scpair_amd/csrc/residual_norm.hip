@@ -17,8 +17,8 @@
 // taken about the mean in a second pass over registers: no cancellation for rows far from zero.
 //
 // Bound: HBM.  One pass over the data in each direction: a row lives in registers, 8 consecutive columns per lane and
-// chunk (16 bytes of bf16, 32 of fp32), and a workgroup walks rows with the column constants and column sums in
-// registers.  Up to 1024 columns a row belongs to one wave (no barriers), above that to a workgroup.  Rows need no
+// chunk (16 bytes of bf16, 32 of fp32), and a workgroup walks rows with the column constants and column sums in registers
+// and the next row's values on their way.  Up to 1024 columns a row belongs to one wave (no barriers), above that to a workgroup.  Rows need no
 // alignment: the vector accesses are declared with the element's alignment, which the hardware takes as they are.
 // Column sums leave a workgroup as one partial row each; a second launch adds them in a fixed order (no atomics).
 #include "common.h"
@@ -37,29 +37,33 @@ enum { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_TANH = 2 };
 enum { SCALE_VALUE = 0, SCALE_ONE = 1, SCALE_COL = 2 };
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
-// 8 columns from `col` of a row of D; columns behind the row's end are zero
-template <typename T>
-__device__ __forceinline__ typename Vec8<T>::v ld8(const T* __restrict__ p, int col, int D) {
+// A lane's chunk: 8 columns from `base` of a row of D.  Chunk q covers columns 8q ..; the one that would run over the
+// row's end starts at D - 8 instead, so every access is one vector access without a test.  Its first `8 q - base` columns
+// are its neighbour's: both lanes compute (and write) the same values there, and only the row's sums leave them out.
+// Rows shorter than a chunk (SMALL) go element by element.
+__device__ __forceinline__ int chunk_base(int q, int D) { return max(0, min(8 * q, D - 8)); }
+__device__ __forceinline__ bool chunk_owns(int q, int i, int D) {
+  return 8 * q < D && chunk_base(q, D) + i >= 8 * q && chunk_base(q, D) + i < D;
+}
+template <bool SMALL, typename T>
+__device__ __forceinline__ typename Vec8<T>::v ld8(const T* __restrict__ p, int base, int D) {
+  if constexpr (!SMALL) return *(const typename Vec8<T>::vu*)(p + base);
   typename Vec8<T>::v v;
-  if (col + 8 <= D) {
-    v = *(const typename Vec8<T>::vu*)(p + col);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (col + i < D) ? p[col + i] : (T)0.f;
-  }
+  for (int i = 0; i < 8; i++) v[i] = i < D ? p[i] : (T)0.f;
   return v;
 }
-template <typename T>
-__device__ __forceinline__ void st8(T* __restrict__ p, int col, int D, const float* f) {
+template <bool SMALL, typename T>
+__device__ __forceinline__ void st8(T* __restrict__ p, int base, int D, const float* f) {
   typename Vec8<T>::v v;
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = (T)f[i];
-  if (col + 8 <= D) {
-    *(typename Vec8<T>::vu*)(p + col) = v;
+  if constexpr (!SMALL) {
+    *(typename Vec8<T>::vu*)(p + base) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
-      if (col + i < D) p[col + i] = v[i];
+      if (i < D) p[i] = v[i];
   }
 }
 
@@ -95,139 +99,230 @@ __device__ __forceinline__ float wsum(float v) {
   v = xor16_sum(v);
   return xor32_sum(v);
 }
-// Sums of NV values over the TPR threads of a row, in every thread.  Above one wave: one barrier per call; calls
-// alternate between two LDS slots, and a slot's next write comes after the barrier of the call between.
+// columns of wave w of a workgroup that holds a row in NCH rounds of blockDim.x chunks
+template <int NCH>
+__device__ __forceinline__ int wave_cols(int w, int D) {
+  int n = 0;
+  if (64 * w >= (int)blockDim.x) return 0;
+#pragma unroll
+  for (int c = 0; c < NCH; c++) n += max(0, min(512, D - 8 * (int)blockDim.x * c - 512 * w));
+  return n;
+}
+// sum over groups of 16 neighbouring lanes, in each of them
+__device__ __forceinline__ float sum16(float v) {
+  v += dppf<0xB1>(v);
+  v += dppf<0x4E>(v);
+  v += dppf<0x124>(v);
+  return v + dppf<0x128>(v);
+}
+// Sums of NV values over the threads of a row, in every thread.  TPR > 64 (a workgroup of at most TPR threads): one barrier
+// per call; the lanes of every wave read the waves' sums side by side (slots of absent waves hold zeros) and add them up.
+// Calls alternate between two halves of `red`, and a half's next write comes after the barrier of the call between.
+constexpr int RED = 4 * 16;
 template <int TPR, int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], float* red, int& turn) {
 #pragma unroll
   for (int i = 0; i < NV; i++) v[i] = wsum(v[i]);
   if constexpr (TPR > 64) {
-    constexpr int NWV = TPR / 64;
-    float* s = red + (turn & 1) * (4 * NWV);
+    float* s = red + (turn & 1) * RED;
     turn++;
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-      for (int i = 0; i < NV; i++) s[i * NWV + (threadIdx.x >> 6)] = v[i];
+      for (int i = 0; i < NV; i++) s[i * 16 + (threadIdx.x >> 6)] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      float t = 0.f;
-#pragma unroll
-      for (int w = 0; w < NWV; w++) t += s[i * NWV + w];
-      v[i] = t;
-    }
+    for (int i = 0; i < NV; i++) v[i] = sum16(s[i * 16 + (threadIdx.x & 15)]);
   }
 }
 
-// mean and 1 / spread of a row held as v[NCH][8] (columns >= D hold zeros)
+// Mean and 1 / spread of a row held as v[NCH][8]; own: 1 for the columns of the last chunk that are this lane's, else 0.
+// The squares are taken about a mean, never about zero.  A workgroup's row needs one exchange for both: each wave takes its
+// squares about its own mean, and M2 = sum_w M2_w + (sum_w - n_w mean)^2 / n_w, n_w the columns of wave w.
 template <int TPR, int NCH>
-__device__ __forceinline__ void row_stats(const float (&v)[NCH][8], int kind, int t, int D, float inv_d, float eps,
+__device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const float (&own)[8], int kind, int D, float inv_d, float eps,
                                           float* red, int& turn, float& mean, float& rstd) {
   mean = 0.f;
+  float s = 0.f;
   if (kind == NORM_LAYER) {
-    float s[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < NCH; c++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) s[0] += v[c][i];
-    row_sum<TPR, 1>(s, red, turn);
-    mean = s[0] * inv_d;
+      for (int i = 0; i < 8; i++) s += c == NCH - 1 ? v[c][i] * own[i] : v[c][i];
+    s = wsum(s);
+    if constexpr (TPR > 64) {
+      mean = s * __builtin_amdgcn_rcpf((float)max(wave_cols<NCH>(threadIdx.x >> 6, D), 1));
+    } else {
+      mean = s * inv_d;
+    }
   }
   float q[1] = {0.f};
 #pragma unroll
-  for (int c = 0; c < NCH; c++) {
-    const int col = (t + TPR * c) * 8;
+  for (int c = 0; c < NCH; c++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float e = col + i < D ? v[c][i] - mean : 0.f;
-      q[0] += e * e;
+      const float e = v[c][i] - mean;
+      q[0] += (c == NCH - 1 ? e * own[i] : e) * e;
     }
+  if (TPR > 64 && kind == NORM_LAYER) {
+    q[0] = wsum(q[0]);
+    float* r = red + (turn & 1) * RED;
+    turn++;
+    if ((threadIdx.x & 63) == 0) {
+      r[threadIdx.x >> 6] = s;
+      r[16 + (threadIdx.x >> 6)] = q[0];
+    }
+    __syncthreads();
+    const int w = threadIdx.x & 15, n = wave_cols<NCH>(w, D);
+    const float sw = r[w];
+    mean = sum16(sw) * inv_d;
+    const float d = sw - (float)n * mean;
+    q[0] = sum16(r[16 + w] + (n > 0 ? d * d * __builtin_amdgcn_rcpf((float)n) : 0.f));
+  } else {
+    row_sum<TPR, 1>(q, red, turn);
   }
-  row_sum<TPR, 1>(q, red, turn);
   rstd = 1.f / sqrtf(q[0] * inv_d + eps);
 }
 
-// threads per workgroup: rows of one wave are handled by several independent waves
-template <int TPR> constexpr int fwd_threads() { return TPR == 64 ? 256 : TPR; }
-template <int TPR> constexpr int bwd_threads() { return TPR == 64 ? 512 : TPR; }
+// Rows of one wave share a workgroup of four (independent in the forward; in the backward they add their column sums).
+template <int TPR> constexpr int threads() { return TPR == 64 ? 256 : TPR; }
 
-// column constants of one chunk
-template <int FWD>
-__device__ __forceinline__ void fold(const ScpResidualNorm& a, int col, float* A1, float* B1, float* W2, float* B2) {
+// column constants of one chunk: vector loads behind uniform tests
+template <bool SMALL>
+__device__ __forceinline__ void fold(const ScpResidualNorm& a, int base, float* A1, float* B1, float* W2) {
   const int D = a.cols;
-  float s = a.scale_mode == SCALE_ONE ? a.scale[0] : a.scale_value;
+  float S[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const bool ok = col + i < D;
-    float S = s;
-    if (a.scale_mode == SCALE_COL) S = ok ? a.scale[col + i] : 0.f;
-    if (a.gate_mode == GATE_COL) S *= ok ? gate_value(((const float*)a.gate)[col + i], a.gate_act) : 0.f;
-    A1[i] = !ok ? 0.f : a.w1 ? a.w1[col + i] * S : S;
-    B1[i] = ok && a.b1 ? a.b1[col + i] * S : 0.f;
-    W2[i] = !ok ? 0.f : a.w2 ? a.w2[col + i] : 1.f;
-    if (FWD) B2[i] = ok && a.b2 ? a.b2[col + i] : 0.f;
+    S[i] = a.scale_value;
+    B1[i] = 0.f;
+    W2[i] = 1.f;
+  }
+  if (a.scale_mode == SCALE_ONE) {
+    const float s = a.scale[0];
+#pragma unroll
+    for (int i = 0; i < 8; i++) S[i] = s;
+  } else if (a.scale_mode == SCALE_COL) {
+    const vf8 s = ld8<SMALL, float>(a.scale, base, D);
+#pragma unroll
+    for (int i = 0; i < 8; i++) S[i] = s[i];
+  }
+  if (a.gate_mode == GATE_COL) {
+    const vf8 g = ld8<SMALL, float>((const float*)a.gate, base, D);
+#pragma unroll
+    for (int i = 0; i < 8; i++) S[i] *= gate_value(g[i], a.gate_act);
+  }
+  if (a.b1) {
+    const vf8 b = ld8<SMALL, float>(a.b1, base, D);
+#pragma unroll
+    for (int i = 0; i < 8; i++) B1[i] = b[i] * S[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) A1[i] = S[i];
+  if (a.w1) {
+    const vf8 w = ld8<SMALL, float>(a.w1, base, D);
+#pragma unroll
+    for (int i = 0; i < 8; i++) A1[i] = w[i] * S[i];
+  }
+  if (a.w2) {
+    const vf8 w = ld8<SMALL, float>(a.w2, base, D);
+#pragma unroll
+    for (int i = 0; i < 8; i++) W2[i] = w[i];
   }
 }
 
-template <typename XT, typename HT, int TPR, int NCH>
-__global__ __launch_bounds__(fwd_threads<TPR>()) void rnorm_fwd_kernel(ScpResidualNorm a) {
-  constexpr int RPW = fwd_threads<TPR>() / TPR;
-  __shared__ float red[TPR > 64 ? 2 * 4 * (TPR / 64) : 1];
-  const int t = threadIdx.x % TPR, D = a.cols;
+// GF: a gate for every element
+template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL>
+__global__ __launch_bounds__(threads<TPR>()) void rnorm_fwd_kernel(ScpResidualNorm a) {
+  constexpr int RPW = threads<TPR>() / TPR;
+  __shared__ float red[TPR > 64 ? 2 * RED : 1];
+  const int t = RPW > 1 ? threadIdx.x & 63 : threadIdx.x, D = a.cols;
+  const int nt = RPW > 1 ? 64 : blockDim.x;      // threads of a row
   const float inv_d = 1.f / (float)D;
   int turn = 0;
+  if constexpr (TPR > 64) {
+    for (int i = threadIdx.x; i < 2 * RED; i += blockDim.x) red[i] = 0.f;
+    __syncthreads();
+  }
+  long row = (long)blockIdx.x * RPW + (RPW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);   // wave-uniform
+  const long stride = (long)gridDim.x * RPW;
+  int base[NCH];
+#pragma unroll
+  for (int c = 0; c < NCH; c++) base[c] = chunk_base(t + nt * c, D);
+  const bool last = 8 * (t + nt * (NCH - 1)) < D;     // this lane's last chunk exists; the others always do
+  float own[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) own[i] = chunk_owns(t + nt * (NCH - 1), i, D) ? 1.f : 0.f;
+
+  // the next row's values are fetched while this one's sums run
+  struct Raw {
+    typename Vec8<XT>::v x[NCH];
+    typename Vec8<HT>::v h[NCH], g[GF ? NCH : 1];
+    float grow;
+  };
+  auto load = [&](long r) {
+    Raw v;
+    v.grow = a.gate_mode == GATE_ROW ? ((const float*)a.gate)[r] : 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; c++) {
+      v.x[c] = ld8<SMALL, XT>((const XT*)a.x + r * a.ldx, base[c], D);
+      if (a.h) v.h[c] = ld8<SMALL, HT>((const HT*)a.h + r * a.ldh, base[c], D);
+      if constexpr (GF) v.g[c] = ld8<SMALL, HT>((const HT*)a.gate + r * a.ldg, base[c], D);
+    }
+    return v;
+  };
+  if (row >= a.rows) return;
+  Raw cur = load(row);
+
   float A1[NCH][8], B1[NCH][8], W2[NCH][8], B2[NCH][8];
 #pragma unroll
-  for (int c = 0; c < NCH; c++) fold<1>(a, (t + TPR * c) * 8, A1[c], B1[c], W2[c], B2[c]);
+  for (int c = 0; c < NCH; c++) {
+    fold<SMALL>(a, base[c], A1[c], B1[c], W2[c]);
+#pragma unroll
+    for (int i = 0; i < 8; i++) B2[c][i] = 0.f;
+    if (a.b2) {
+      const vf8 b = ld8<SMALL, float>(a.b2, base[c], D);
+#pragma unroll
+      for (int i = 0; i < 8; i++) B2[c][i] = b[i];
+    }
+  }
 
-  for (long row = (long)blockIdx.x * RPW + threadIdx.x / TPR; row < a.rows; row += (long)gridDim.x * RPW) {
+  for (; row < a.rows; row += stride) {
+    const Raw v = cur;
+    if (row + stride < a.rows) cur = load(row + stride);
     float r[NCH][8];
-    const XT* xp = (const XT*)a.x + row * a.ldx;
     float m1 = 0.f, s1 = 1.f, m2, s2;
     if (a.h) {
-      const HT* hp = (const HT*)a.h + row * a.ldh;
       float h[NCH][8];
-      typename Vec8<XT>::v xv[NCH];
-      typename Vec8<HT>::v gv[NCH];
+#pragma unroll
+      for (int c = 0; c < NCH; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[c][i] = (float)v.h[c][i];
+      const float grow = a.gate_mode == GATE_ROW ? gate_value(v.grow, a.gate_act) : 1.f;
+      if (a.post != NORM_NONE) row_stats<TPR, NCH>(h, own, a.post, D, inv_d, a.eps, red, turn, m1, s1);
 #pragma unroll
       for (int c = 0; c < NCH; c++) {
-        const int col = (t + TPR * c) * 8;
-        const auto hv = ld8<HT>(hp, col, D);
-        xv[c] = ld8<XT>(xp, col, D);
-        if (a.gate_mode == GATE_FULL) gv[c] = ld8<HT>((const HT*)a.gate + row * a.ldg, col, D);
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[c][i] = (float)hv[i];
-      }
-      const float grow = a.gate_mode == GATE_ROW ? gate_value(((const float*)a.gate)[row], a.gate_act) : 1.f;
-      if (a.post != NORM_NONE) row_stats<TPR, NCH>(h, a.post, t, D, inv_d, a.eps, red, turn, m1, s1);
-#pragma unroll
-      for (int c = 0; c < NCH; c++) {
-        const int col = (t + TPR * c) * 8;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          const float g = a.gate_mode == GATE_FULL ? gate_value((float)gv[c][i], a.gate_act) : grow;
-          const float u = ((h[c][i] - m1) * s1 * A1[c][i] + B1[c][i]) * g;
-          r[c][i] = col + i < D ? (float)xv[c][i] + u : 0.f;
+          float g = grow;
+          if constexpr (GF) g = gate_value((float)v.g[c][i], a.gate_act);
+          r[c][i] = (float)v.x[c][i] + ((h[c][i] - m1) * s1 * A1[c][i] + B1[c][i]) * g;
         }
-        if (col < D) st8<XT>((XT*)a.r + row * D, col, D, r[c]);
+        if (c < NCH - 1 || last) st8<SMALL, XT>((XT*)a.r + row * D, base[c], D, r[c]);
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < NCH; c++) {
-        const auto xv = ld8<XT>(xp, (t + TPR * c) * 8, D);
+      for (int c = 0; c < NCH; c++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) r[c][i] = (float)xv[i];
-      }
+        for (int i = 0; i < 8; i++) r[c][i] = (float)v.x[c][i];
     }
-    row_stats<TPR, NCH>(r, a.pre, t, D, inv_d, a.eps, red, turn, m2, s2);
+    row_stats<TPR, NCH>(r, own, a.pre, D, inv_d, a.eps, red, turn, m2, s2);
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
-      const int col = (t + TPR * c) * 8;
       float y[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) y[i] = (r[c][i] - m2) * s2 * W2[c][i] + B2[c][i];
-      if (col < D) st8<HT>((HT*)a.y + row * D, col, D, y);
+      if (c < NCH - 1 || last) st8<SMALL, HT>((HT*)a.y + row * D, base[c], D, y);
     }
     if (a.stats && t == 0) {
       f32x4 s = {m1, s1, m2, s2};
@@ -236,176 +331,244 @@ __global__ __launch_bounds__(fwd_threads<TPR>()) void rnorm_fwd_kernel(ScpResidu
   }
 }
 
-// partial column sums: ws[block][4][cols], order P, Q, sum dy rhat, sum dy
-template <typename XT, typename HT, int TPR, int NCH>
-__global__ __launch_bounds__(bwd_threads<TPR>()) void rnorm_bwd_kernel(ScpResidualNorm a) {
-  constexpr int RPW = bwd_threads<TPR>() / TPR;
-  __shared__ float red[TPR > 64 ? 2 * 4 * (TPR / 64) : 1];
-  __shared__ float colbuf[RPW > 1 ? NCH * 512 : 1];
-  const int t = threadIdx.x % TPR, D = a.cols;
+// waves per SIMD that the registers have to leave room for (second argument of __launch_bounds__)
+constexpr int bwd_waves(int tpr) { return tpr == 1024 ? 4 : tpr == 768 ? 3 : 2; }
+
+// Partial column sums: ws[block][4][cols], order P, sum dy rhat, Q, sum dy; without BIAS (no post bias, no gradient of a pre
+// bias) the last two stay unwritten.
+template <typename XT, typename HT, int TPR, int NCH, bool GF, bool BIAS, bool SMALL>
+__global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kernel(ScpResidualNorm a) {
+  constexpr int RPW = threads<TPR>() / TPR, NA = BIAS ? 4 : 2;
+  __shared__ float red[TPR > 64 ? 2 * RED : 1];
+  __shared__ float colbuf[RPW > 1 ? 2 * RPW * NCH * 512 : 1];
+  const int t = RPW > 1 ? threadIdx.x & 63 : threadIdx.x, D = a.cols;
+  const int nt = RPW > 1 ? 64 : blockDim.x;      // threads of a row
   const float inv_d = 1.f / (float)D;
   int turn = 0;
+  if constexpr (TPR > 64) {
+    for (int i = threadIdx.x; i < 2 * RED; i += blockDim.x) red[i] = 0.f;
+    __syncthreads();
+  }
+  long row = (long)blockIdx.x * RPW + (RPW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);   // wave-uniform
+  const long stride = (long)gridDim.x * RPW;
+  int base[NCH];
+#pragma unroll
+  for (int c = 0; c < NCH; c++) base[c] = chunk_base(t + nt * c, D);
+  const bool last = 8 * (t + nt * (NCH - 1)) < D;
+  float own[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) own[i] = chunk_owns(t + nt * (NCH - 1), i, D) ? 1.f : 0.f;
+
+  struct Raw {
+    typename Vec8<XT>::v x[NCH], dr[NCH];
+    typename Vec8<HT>::v h[NCH], g[GF ? NCH : 1], dy[NCH];
+    f32x4 st;
+    float grow;
+  };
+  auto load = [&](long r) {
+    Raw v;
+    v.st = *(const f32x4*)(a.stats + r * 4);
+    v.grow = a.gate_mode == GATE_ROW ? ((const float*)a.gate)[r] : 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; c++) {
+      v.x[c] = ld8<SMALL, XT>((const XT*)a.x + r * a.ldx, base[c], D);
+      if (a.h) v.h[c] = ld8<SMALL, HT>((const HT*)a.h + r * a.ldh, base[c], D);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; i++) v.h[c][i] = (HT)0.f;
+      if constexpr (GF) v.g[c] = ld8<SMALL, HT>((const HT*)a.gate + r * a.ldg, base[c], D);
+      if (a.dy) v.dy[c] = ld8<SMALL, HT>((const HT*)a.dy + r * a.lddy, base[c], D);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; i++) v.dy[c][i] = (HT)0.f;
+      if (a.dr) v.dr[c] = ld8<SMALL, XT>((const XT*)a.dr + r * a.lddr, base[c], D);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; i++) v.dr[c][i] = (XT)0.f;
+    }
+    return v;
+  };
   float A1[NCH][8], B1[NCH][8], W2[NCH][8];
-  float acc[4][NCH][8];
+  float acc[NA][NCH][8];
 #pragma unroll
   for (int c = 0; c < NCH; c++) {
-    fold<0>(a, (t + TPR * c) * 8, A1[c], B1[c], W2[c], nullptr);
+    fold<SMALL>(a, base[c], A1[c], B1[c], W2[c]);
+    if constexpr (!BIAS)
 #pragma unroll
-    for (int k = 0; k < 4; k++)
+      for (int i = 0; i < 8; i++) B1[c][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NA; k++)
 #pragma unroll
       for (int i = 0; i < 8; i++) acc[k][c][i] = 0.f;
   }
   const float lay1 = a.post == NORM_LAYER ? inv_d : 0.f, cor1 = a.post == NORM_NONE ? 0.f : inv_d;
   const float lay2 = a.pre == NORM_LAYER ? inv_d : 0.f;
 
-  for (long row = (long)blockIdx.x * RPW + threadIdx.x / TPR; row < a.rows; row += (long)gridDim.x * RPW) {
-    const f32x4 st = *(const f32x4*)(a.stats + row * 4);
-    const float m1 = st[0], s1 = st[1], m2 = st[2], s2 = st[3];
-    float hh[NCH][8], G[NCH][8], dG[NCH][8], rh[NCH][8], du[NCH][8];
-    const float grow = a.h && a.gate_mode == GATE_ROW ? gate_value(((const float*)a.gate)[row], a.gate_act) : 1.f;
+  // Fetching the next row early is worth half of the waves where the registers allow it (32768 x 4096 bf16: 305 us against
+  // 396 us with four waves per SIMD and no early fetch); with 16 columns per lane it spills (1024 x 900 fp32: 21 against 17 us).
+  constexpr bool EARLY = NCH == 1 && TPR < 1024;
+  Raw cur;
+  if (EARLY && row < a.rows) cur = load(row);
+  for (; row < a.rows; row += stride) {
+    const Raw v = EARLY ? cur : load(row);
+    if (EARLY && row + stride < a.rows) cur = load(row + stride);
+    const float m1 = v.st[0], s1 = v.st[1], m2 = v.st[2], s2 = v.st[3];
+    float hh[NCH][8], rh[NCH][8], du[NCH][8], G[GF ? NCH : 1][8], dG[GF ? NCH : 1][8];
+    const float grow = a.gate_mode == GATE_ROW ? gate_value(v.grow, a.gate_act) : 1.f;
     float c12[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
-      const int col = (t + TPR * c) * 8;
-      const auto xv = ld8<XT>((const XT*)a.x + row * a.ldx, col, D);
-      typename Vec8<HT>::v hv, gv, yv;
-      typename Vec8<XT>::v rv;
-      if (a.h) hv = ld8<HT>((const HT*)a.h + row * a.ldh, col, D);
-      if (a.gate_mode == GATE_FULL) gv = ld8<HT>((const HT*)a.gate + row * a.ldg, col, D);
-      if (a.dy) yv = ld8<HT>((const HT*)a.dy + row * a.lddy, col, D);
-      if (a.dr) rv = ld8<XT>((const XT*)a.dr + row * a.lddr, col, D);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        G[c][i] = grow;
-        dG[c][i] = 1.f;
-        float r = (float)xv[i];
-        if (a.h) {
-          if (a.gate_mode == GATE_FULL) G[c][i] = gate_both((float)gv[i], a.gate_act, dG[c][i]);
-          hh[c][i] = ((float)hv[i] - m1) * s1;
-          r += (hh[c][i] * A1[c][i] + B1[c][i]) * G[c][i];
-        }
-        rh[c][i] = col + i < D ? (r - m2) * s2 : 0.f;
-        const float dy = a.dy ? (float)yv[i] : 0.f;
-        du[c][i] = a.dr ? (float)rv[i] : 0.f;
-        const float av = dy * W2[c][i];
-        du[c][i] += s2 * av;
-        c12[0] += av;
-        c12[1] += av * rh[c][i];
-        acc[2][c][i] += dy * rh[c][i];
-        acc[3][c][i] += dy;
+        float g = grow;
+        if constexpr (GF) g = G[c][i] = gate_both((float)v.g[c][i], a.gate_act, dG[c][i]);
+        hh[c][i] = ((float)v.h[c][i] - m1) * s1;
+        // without a block A1 is the scale's default, but the statistics are 0 and 1 and h is zero: nothing is added
+        const float r = (float)v.x[c][i] + (hh[c][i] * A1[c][i] + B1[c][i]) * g;
+        rh[c][i] = (r - m2) * s2;
+        const float dy = (float)v.dy[c][i], av = dy * W2[c][i];
+        du[c][i] = (float)v.dr[c][i] + s2 * av;
+        const float ao = c == NCH - 1 ? av * own[i] : av;
+        c12[0] += ao;
+        c12[1] += ao * rh[c][i];
+        acc[1][c][i] += dy * rh[c][i];
+        if constexpr (BIAS) acc[3][c][i] += dy;
       }
     }
     if (a.dy) row_sum<TPR, 2>(c12, red, turn);
-    const float c1 = c12[0] * lay2, c2 = c12[1] * inv_d;
+    const float c1 = s2 * c12[0] * lay2, c2 = s2 * c12[1] * inv_d;
     float e[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
-      const int col = (t + TPR * c) * 8;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        du[c][i] -= s2 * (c1 + rh[c][i] * c2);
-        if (col + i >= D) du[c][i] = 0.f;
-        if (a.h) {
-          const float dg = du[c][i] * G[c][i], b = dg * A1[c][i];
-          acc[0][c][i] += dg * hh[c][i];
-          acc[1][c][i] += dg;
-          e[0] += b;
-          e[1] += b * hh[c][i];
-          e[2] += du[c][i] * (hh[c][i] * A1[c][i] + B1[c][i]);
-        }
+        du[c][i] -= c1 + rh[c][i] * c2;
+        float g = grow;
+        if constexpr (GF) g = G[c][i];
+        const float dg = du[c][i] * g;
+        acc[0][c][i] += dg * hh[c][i];
+        if constexpr (BIAS) acc[2][c][i] += dg;
+        const float bo = c == NCH - 1 ? dg * A1[c][i] * own[i] : dg * A1[c][i];
+        e[0] += bo;
+        e[1] += bo * hh[c][i];
+        if constexpr (!GF) e[2] += (c == NCH - 1 ? du[c][i] * own[i] : du[c][i]) * (hh[c][i] * A1[c][i] + B1[c][i]);
       }
-      if (a.dx && col < D) st8<XT>((XT*)a.dx + row * D, col, D, du[c]);
+      if (a.dx && (c < NCH - 1 || last)) st8<SMALL, XT>((XT*)a.dx + row * D, base[c], D, du[c]);
     }
-    if (a.h) {
-      row_sum<TPR, 3>(e, red, turn);
-      const float e1 = e[0] * lay1, e2 = e[1] * cor1;
+    if (!a.h) continue;
+    row_sum<TPR, GF ? 2 : 3>((float(&)[GF ? 2 : 3])e, red, turn);
+    const float e1 = e[0] * lay1, e2 = e[1] * cor1;
 #pragma unroll
-      for (int c = 0; c < NCH; c++) {
-        const int col = (t + TPR * c) * 8;
-        float dh[8], dg[8];
+    for (int c = 0; c < NCH; c++) {
+      if (c == NCH - 1 && !last) continue;
+      float dh[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          dh[i] = s1 * (du[c][i] * G[c][i] * A1[c][i] - e1 - hh[c][i] * e2);
-          dg[i] = du[c][i] * (hh[c][i] * A1[c][i] + B1[c][i]) * dG[c][i];
-        }
-        if (a.dh && col < D) st8<HT>((HT*)a.dh + row * D, col, D, dh);
-        if (a.dgate && a.gate_mode == GATE_FULL && col < D) st8<HT>((HT*)a.dgate + row * D, col, D, dg);
+      for (int i = 0; i < 8; i++) {
+        float g = grow;
+        if constexpr (GF) g = G[c][i];
+        dh[i] = s1 * (du[c][i] * g * A1[c][i] - e1 - hh[c][i] * e2);
       }
-      if (a.dgate && a.gate_mode == GATE_ROW && t == 0) {
-        float d;
-        gate_both(((const float*)a.gate)[row], a.gate_act, d);
-        ((float*)a.dgate)[row] = e[2] * d;
+      if (a.dh) st8<SMALL, HT>((HT*)a.dh + row * D, base[c], D, dh);
+      if constexpr (GF) {
+        float dg[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) dg[i] = du[c][i] * (hh[c][i] * A1[c][i] + B1[c][i]) * dG[c][i];
+        if (a.dgate) st8<SMALL, HT>((HT*)a.dgate + row * D, base[c], D, dg);
       }
+    }
+    if (!GF && a.dgate && a.gate_mode == GATE_ROW && t == 0) {
+      float d;
+      gate_both(v.grow, a.gate_act, d);
+      ((float*)a.dgate)[row] = e[2] * d;
     }
   }
 
   if (!a.ws) return;
   float* wsb = a.ws + (long)blockIdx.x * 4 * D;
+  if constexpr (RPW > 1) {
+    // two sums at a time: every wave lays its own into LDS, then the workgroup adds the waves in wave order
+    const int w = threadIdx.x / 64;
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    if (k < 2 ? !a.want1 : !a.want2) continue;
-    if constexpr (RPW > 1) {
-      // add the waves of the workgroup in wave order
-      for (int w = 0; w < RPW; w++) {
-        if ((int)(threadIdx.x / 64) == w) {
+    for (int k0 = 0; k0 < NA; k0 += 2) {
+      if (k0) __syncthreads();
 #pragma unroll
-          for (int c = 0; c < NCH; c++)
+      for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              float* p = colbuf + (c * 8 + i) * 64 + t;
-              *p = w ? *p + acc[k][c][i] : acc[k][c][i];
-            }
-        }
-        __syncthreads();
-      }
-      for (int j = threadIdx.x; j < D; j += bwd_threads<TPR>()) {
-        const int ch = j >> 3;
-        wsb[(long)k * D + j] = colbuf[((ch >> 6) * 8 + (j & 7)) * 64 + (ch & 63)];
-      }
+        for (int c = 0; c < NCH; c++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) colbuf[((k * RPW + w) * NCH * 8 + c * 8 + i) * 64 + t] = acc[k0 + k][c][i];
       __syncthreads();
-    } else {
+      for (int j = threadIdx.x; j < 2 * D; j += 64 * RPW) {
+        const int k = j >= D, col = j - k * D, q = min(col >> 3, (D - 1) >> 3), ch = q >> 6;
+        const int i = col - chunk_base(q, D);
+        float s = 0.f;
 #pragma unroll
-      for (int c = 0; c < NCH; c++) {
-        const int col = (t + TPR * c) * 8;
-        if (col < D) st8<float>(wsb + (long)k * D, col, D, acc[k][c]);
+        for (int ww = 0; ww < RPW; ww++) s += colbuf[((k * RPW + ww) * NCH * 8 + ch * 8 + i) * 64 + (q & 63)];
+        wsb[(long)(k0 + k) * D + col] = s;
       }
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NA; k++)
+#pragma unroll
+      for (int c = 0; c < NCH; c++)
+        if (c < NCH - 1 || last) st8<SMALL, float>(wsb + (long)k * D, base[c], D, acc[k][c]);
   }
 }
 
-// columns' sums of the partial rows (fixed order), and from them the parameters' gradients.  A workgroup takes 16
-// columns; 16 threads share a column.
-__global__ __launch_bounds__(256) void rnorm_cols_kernel(ScpResidualNorm a, int nblk, float* each) {
-  __shared__ double part[4][16][17];
-  const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + cx, D = a.cols;
+// The columns' sums of the partial rows (fixed order, fp64), and from them the parameters' gradients.  A workgroup takes 32
+// columns; 32 threads share a column, four rows of all sums in flight each.
+template <bool BIAS>
+__global__ __launch_bounds__(1024) void rnorm_cols_kernel(ScpResidualNorm a, int nblk, float* each) {
+  constexpr int NA = BIAS ? 4 : 2;
+  __shared__ double part[NA][32][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + cx, D = a.cols;
+  double s[NA];
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    double s = 0.0;
-    if (col < D && (k < 2 ? a.want1 : a.want2))
-      for (int b = ry; b < nblk; b += 16) s += (double)a.ws[((long)b * 4 + k) * D + col];
-    part[k][ry][cx] = s;
+  for (int k = 0; k < NA; k++) s[k] = 0.0;
+  if (col < D) {
+    const float* p = a.ws + col;
+    int b = ry;
+    for (; b + 96 < nblk; b += 128) {
+      float v[4][NA];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int k = 0; k < NA; k++) v[u][k] = p[((long)(b + 32 * u) * 4 + k) * D];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int k = 0; k < NA; k++) s[k] += (double)v[u][k];
+    }
+    for (; b < nblk; b += 32)
+#pragma unroll
+      for (int k = 0; k < NA; k++) s[k] += (double)p[((long)b * 4 + k) * D];
+  }
+#pragma unroll
+  for (int k = 0; k < NA; k++) part[k][ry][cx] = s[k];
+  __syncthreads();
+  // 32 x NA sums of 32: one per thread of the first NA half-waves
+  if (ry < NA) {
+    double q = 0.0;
+#pragma unroll
+    for (int y = 0; y < 32; y++) q += part[ry][y][cx];
+    part[ry][0][cx] = q;      // read by this thread only before the barrier
   }
   __syncthreads();
   if (ry || col >= D) return;
-  double sum[4];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    sum[k] = 0.0;
-    for (int y = 0; y < 16; y++) sum[k] += part[k][y][cx];
-  }
-  if (a.want2) {
-    if (a.dw2) a.dw2[col] = (float)sum[2];
-    if (a.db2) a.db2[col] = (float)sum[3];
-  }
+  const double P = part[0][0][cx], Q = BIAS ? part[NA / 2][0][cx] : 0.0;
+  if (a.dw2) a.dw2[col] = (float)part[1][0][cx];
+  if constexpr (BIAS)
+    if (a.db2) a.db2[col] = (float)part[3][0][cx];
   if (a.want1) {
-    const float s = a.scale_mode == SCALE_COL ? a.scale[col] : a.scale_mode == SCALE_ONE ? a.scale[0] : a.scale_value;
+    const float sc = a.scale_mode == SCALE_COL ? a.scale[col] : a.scale_mode == SCALE_ONE ? a.scale[0] : a.scale_value;
     float g = 1.f, d = 1.f;
     if (a.gate_mode == GATE_COL) g = gate_both(((const float*)a.gate)[col], a.gate_act, d);
-    const double n = (a.w1 ? a.w1[col] : 1.f) * sum[0] + (a.b1 ? a.b1[col] * sum[1] : 0.0);
-    if (a.dw1) a.dw1[col] = (float)(s * g * sum[0]);
-    if (a.db1) a.db1[col] = (float)(s * g * sum[1]);
-    if (a.gate_mode == GATE_COL && a.dgate) ((float*)a.dgate)[col] = (float)(s * d * n);
+    const double n = (a.w1 ? a.w1[col] : 1.f) * P + (BIAS && a.b1 ? a.b1[col] * Q : 0.0);
+    if (a.dw1) a.dw1[col] = (float)(sc * g * P);
+    if (a.db1) a.db1[col] = (float)(sc * g * Q);
+    if (a.gate_mode == GATE_COL && a.dgate) ((float*)a.dgate)[col] = (float)(sc * d * n);
     if (a.dscale && a.scale_mode == SCALE_COL) a.dscale[col] = (float)(g * n);
     if (each) each[col] = (float)(g * n);
   }
@@ -422,45 +585,68 @@ __global__ __launch_bounds__(256) void rnorm_scale_kernel(const float* each, int
 
 constexpr int MAX_COLS = 16384;
 
-// threads per row by width: a wave up to 1024 columns, above that a workgroup with 8 or 16 columns per thread
-int tpr_of(int cols) { return cols <= 1024 ? 64 : cols <= 4096 ? 256 : cols <= 8192 ? 512 : 1024; }
+// Rows up to 1024 columns: a wave each, four to a workgroup.  Wider rows: a workgroup each, of as many waves as 8 columns per
+// lane take (16 where that would not fit its register budget).
+unsigned wg_threads(int cols, int nch) { return cols <= 1024 ? 256u : 64u * ((cols + 512 * nch - 1) / (512 * nch)); }
 
+// Workgroups of the backward: about those that are resident at once, since each leaves a partial row per column sum
 int bwd_grid(long rows, int cols) {
-  const int tpr = tpr_of(cols), rpw = tpr == 64 ? 8 : 1;
-  const long need = (rows + rpw - 1) / rpw;
-  const long cap = tpr == 64 ? 512 : tpr == 256 ? 1024 : 512;
+  const int rpw = cols <= 1024 ? 4 : 1;
+  const long need = (rows + rpw - 1) / rpw, cap = cols <= 2048 ? 512 : 256;
   return (int)(need < cap ? need : cap);
 }
 
-template <typename XT, typename HT, int TPR, int NCH>
-int go(const ScpResidualNorm& a, bool bwd, hipStream_t st) {
-  if (!bwd) {
-    const int rpw = fwd_threads<TPR>() / TPR;
-    const long need = (a.rows + rpw - 1) / rpw, cap = 256L * (2048 / fwd_threads<TPR>());
-    hipLaunchKernelGGL((rnorm_fwd_kernel<XT, HT, TPR, NCH>), dim3((unsigned)(need < cap ? need : cap)),
-                       dim3(fwd_threads<TPR>()), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH>), dim3((unsigned)bwd_grid(a.rows, a.cols)),
-                       dim3(bwd_threads<TPR>()), 0, st, a);
-  }
+template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL = false>
+int go_fwd(const ScpResidualNorm& a, hipStream_t st) {
+  const unsigned T = wg_threads(a.cols, NCH);
+  const long rpw = TPR == 64 ? 4 : 1, need = (a.rows + rpw - 1) / rpw, cap = 256L * (2048 / T);
+  hipLaunchKernelGGL((rnorm_fwd_kernel<XT, HT, TPR, NCH, GF, SMALL>), dim3((unsigned)(need < cap ? need : cap)), dim3(T), 0, st, a);
+  SCP_LAUNCH_CHECK();
+  return SCP_OK;
+}
+template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL = false>
+int go_bwd(const ScpResidualNorm& a, bool bias, hipStream_t st) {
+  const dim3 grid((unsigned)bwd_grid(a.rows, a.cols)), T(wg_threads(a.cols, NCH));
+  if (bias)
+    hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, true, SMALL>), grid, T, 0, st, a);
+  else
+    hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, false, SMALL>), grid, T, 0, st, a);
   SCP_LAUNCH_CHECK();
   return SCP_OK;
 }
 
-template <typename XT, typename HT>
-int by_width(const ScpResidualNorm& a, bool bwd, hipStream_t st) {
-  if (a.cols <= 512) return go<XT, HT, 64, 1>(a, bwd, st);
-  if (a.cols <= 1024) return go<XT, HT, 64, 2>(a, bwd, st);
-  if (a.cols <= 2048) return go<XT, HT, 256, 1>(a, bwd, st);
-  if (a.cols <= 4096) return go<XT, HT, 256, 2>(a, bwd, st);
-  if (a.cols <= 8192) return go<XT, HT, 512, 2>(a, bwd, st);
-  return go<XT, HT, 1024, 2>(a, bwd, st);
+// bwd: 0 forward, 1 backward without bias sums, 2 with them
+template <typename XT, typename HT, bool GF>
+int by_width(const ScpResidualNorm& a, int bwd, hipStream_t st) {
+  const int D = a.cols;
+  if (bwd) {
+    const bool bias = bwd == 2;
+    if (D < 8) return go_bwd<XT, HT, 64, 1, GF, true>(a, bias, st);
+    if (D <= 512) return go_bwd<XT, HT, 64, 1, GF>(a, bias, st);
+    if (D <= 1024) return go_bwd<XT, HT, 64, 2, GF>(a, bias, st);
+    if (D <= 2048) return go_bwd<XT, HT, 256, 1, GF>(a, bias, st);
+    if (D <= 4096) return go_bwd<XT, HT, 512, 1, GF>(a, bias, st);
+    if (D <= 6144) return go_bwd<XT, HT, 768, 1, GF>(a, bias, st);
+    if (D <= 8192) return go_bwd<XT, HT, 512, 2, GF>(a, bias, st);
+    return go_bwd<XT, HT, 1024, 2, GF>(a, bias, st);
+  }
+  if (D < 8) return go_fwd<XT, HT, 64, 1, GF, true>(a, st);
+  if (D <= 512) return go_fwd<XT, HT, 64, 1, GF>(a, st);
+  if (D <= 1024) return go_fwd<XT, HT, 64, 2, GF>(a, st);
+  if (D <= 4096) return go_fwd<XT, HT, 512, 1, GF>(a, st);
+  if (D <= 8192) return go_fwd<XT, HT, 1024, 1, GF>(a, st);
+  return go_fwd<XT, HT, 1024, 2, GF>(a, st);
 }
 
-int by_type(const ScpResidualNorm& a, bool bwd, hipStream_t st) {
-  if (!a.x_bf16 && !a.h_bf16) return by_width<float, float>(a, bwd, st);
-  if (!a.x_bf16) return by_width<float, __bf16>(a, bwd, st);
-  return by_width<__bf16, __bf16>(a, bwd, st);
+template <bool GF>
+int by_type(const ScpResidualNorm& a, int bwd, hipStream_t st) {
+  if (!a.x_bf16 && !a.h_bf16) return by_width<float, float, GF>(a, bwd, st);
+  if (!a.x_bf16) return by_width<float, __bf16, GF>(a, bwd, st);
+  return by_width<__bf16, __bf16, GF>(a, bwd, st);
+}
+
+int launch_rows(const ScpResidualNorm& a, int bwd, hipStream_t st) {
+  return a.gate_mode == GATE_FULL ? by_type<true>(a, bwd, st) : by_type<false>(a, bwd, st);
 }
 
 int check_args(const ScpResidualNorm* a, const char* who) {
@@ -488,7 +674,7 @@ extern "C" int scp_residual_norm_fwd(const ScpResidualNorm* a, void* stream) {
   int rc = check_args(a, "scp_residual_norm_fwd");
   if (rc) return rc;
   SCP_CHECK(a->y && (!a->h || a->r), SCP_ERR_ARG, "scp_residual_norm_fwd: null output");
-  return by_type(*a, false, (hipStream_t)stream);
+  return launch_rows(*a, 0, (hipStream_t)stream);
 }
 
 extern "C" long scp_residual_norm_bwd_ws_floats(long rows, int cols) {
@@ -509,11 +695,15 @@ extern "C" int scp_residual_norm_bwd(const ScpResidualNorm* a_, void* stream) {
                 (!a.dgate || a.gate_mode != GATE_NONE), SCP_ERR_ARG, "scp_residual_norm_bwd: gradient of an absent parameter");
   if (!(a.want1 || a.want2)) a.ws = nullptr;
   hipStream_t st = (hipStream_t)stream;
-  rc = by_type(a, true, st);
+  const bool bias = a.b1 || a.db2;
+  rc = launch_rows(a, bias ? 2 : 1, st);
   if (rc || !a.ws) return rc;
   const int nblk = bwd_grid(a.rows, a.cols);
   float* each = a.dscale && a.scale_mode == SCALE_ONE ? a.ws + (long)nblk * 4 * a.cols : nullptr;
-  hipLaunchKernelGGL(rnorm_cols_kernel, dim3((a.cols + 15) / 16), dim3(256), 0, st, a, nblk, each);
+  if (bias)
+    hipLaunchKernelGGL((rnorm_cols_kernel<true>), dim3((a.cols + 31) / 32), dim3(1024), 0, st, a, nblk, each);
+  else
+    hipLaunchKernelGGL((rnorm_cols_kernel<false>), dim3((a.cols + 31) / 32), dim3(1024), 0, st, a, nblk, each);
   SCP_LAUNCH_CHECK();
   if (each) {
     hipLaunchKernelGGL(rnorm_scale_kernel, dim3(1), dim3(256), 0, st, each, a.cols, a.dscale);
