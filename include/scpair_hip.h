@@ -390,16 +390,35 @@ int scp_act8_bwd(const int8_t* codes, const uint8_t* steps, long rows, int cols,
 /* The products of a Linear layer that keeps its input as such a checkpoint.
  * scp_gemm_bf16_c16: scp_gemm_bf16 (a_col 0, no mask) with a bf16 output; ws of scp_gemm_bf16_ws_floats(M, N, K, ldc) floats.
  * scp_gemm_q8: C[m][n] = sum_k A[k][m] * value(codes, steps)[k][n], the weight gradient: A bf16 [K][lda] (lda % 8 == 0, 16-byte
- * aligned), C fp32 or bf16 [M][ldc]; ws of scp_gemm_q8_ws_floats(M, N, K, max(lda, N rounded up to 64), ldc) floats.
- * scp_pad_bf16: copy with rows padded by zeros to ldd = cols rounded up to 8.  scp_colsum_bf16: fp32 column sums. */
+ * aligned), C fp32 or bf16 [M][ldc]; ws of scp_gemm_q8_ws_floats(M, N, K, max(lda, N rounded up to 64), ldc) floats. */
 int scp_gemm_bf16_c16(int a_col, int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb, void* C,
                       long ldc, const float* bias, float* ws, void* stream);
 long scp_gemm_q8_ws_floats(int M, int N, int K, long ld, long ldc);
 int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const int8_t* codes, const uint8_t* steps, void* C, int c_bf16,
                 long ldc, float* ws, void* stream);
-int scp_pad_bf16(const void* src, long lds, long rows, int cols, void* dst, long ldd, void* stream);
-long scp_colsum_bf16_ws_floats(long rows, int cols);
-int scp_colsum_bf16(const void* x, long ldx, long rows, int cols, float* out, float* ws, void* stream);
+/* The whole layer, everything it launches: y = x W^T + b with x's checkpoint written beside it, and its gradients.  x, y, dy, dx
+ * fp32 or bf16 (x_bf16), W and dW fp32 or bf16 (w_bf16; an fp32 x needs an fp32 W), W contiguous [N][K], b and db fp32.
+ * ns as everywhere (fp32 x only).  codes / steps: forward nullable (no weight gradient to come).  dx, dW, db: nullable.
+ * ws: scp_linear8_fwd_ws / _bwd_ws(args) bytes (-1: bad arguments), 256-byte aligned. */
+typedef struct {
+  const void* x;
+  const void* W;
+  const float* b;
+  void* y;
+  int8_t* codes;
+  uint8_t* steps;
+  const void* dy;
+  void* dx;
+  void* dW;
+  float* db;
+  void* ws;
+  long M, ldx, lddy;
+  int N, K, x_bf16, w_bf16, ns;
+} ScpLinear8;
+long scp_linear8_fwd_ws(const ScpLinear8* args /* host */);
+long scp_linear8_bwd_ws(const ScpLinear8* args /* host */);
+int scp_linear8_fwd(const ScpLinear8* args /* host */, void* stream);
+int scp_linear8_bwd(const ScpLinear8* args /* host */, void* stream);
 
 #ifdef __cplusplus
 }

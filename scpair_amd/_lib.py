@@ -60,6 +60,11 @@ class ResidualNorm(C.Structure):
                 ("scale_mode", I), ("scale_value", F), ("eps", F), ("want1", I), ("want2", I)]
 
 
+class Linear8(C.Structure):
+    _fields_ = [("x", P), ("W", P), ("b", P), ("y", P), ("codes", P), ("steps", P), ("dy", P), ("dx", P), ("dW", P), ("db", P),
+                ("ws", P), ("M", L), ("ldx", L), ("lddy", L), ("N", I), ("K", I), ("x_bf16", I), ("w_bf16", I), ("ns", I)]
+
+
 _SIGS = {
     "scp_last_error": (C.c_char_p, []),
     "scp_version": (I, []),
@@ -133,9 +138,10 @@ _SIGS = {
     "scp_gemm_bf16_c16": (I, [I, I, I, I, I, P, L, P, L, P, L, P, P, P]),
     "scp_gemm_q8_ws_floats": (L, [I, I, I, L, L]),
     "scp_gemm_q8": (I, [I, I, I, P, L, P, P, P, I, L, P, P]),
-    "scp_pad_bf16": (I, [P, L, L, I, P, L, P]),
-    "scp_colsum_bf16_ws_floats": (L, [L, I]),
-    "scp_colsum_bf16": (I, [P, L, L, I, P, P, P]),
+    "scp_linear8_fwd_ws": (L, [C.POINTER(Linear8)]),
+    "scp_linear8_bwd_ws": (L, [C.POINTER(Linear8)]),
+    "scp_linear8_fwd": (I, [C.POINTER(Linear8), P]),
+    "scp_linear8_bwd": (I, [C.POINTER(Linear8), P]),
     "scp_step_state_set": (I, [P, U64, F, F, P]),
 }
 

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   const long krow0 = BQ ? (long)kt0 * TK : 0;
   const long krows = min((long)g.K - krow0, (long)(kt1 - kt0) * TK);
   const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(g.A + krow0 * g.lda), 0, BQ ? (int)(krows * g.lda * 2) : (int)g.a_bytes, 0x00020000);
+      (void*)(g.A + krow0 * g.lda), 0, BQ ? (int)(((krows - 1) * g.lda + ((g.M + 7) & ~7)) * 2) : (int)g.a_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc(
       BQ ? (void*)((const int8_t*)g.B + krow0 * g.ldb) : (void*)g.B, 0, BQ ? (int)(krows * g.ldb) : (int)g.b_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rsS = __builtin_amdgcn_make_buffer_rsrc(

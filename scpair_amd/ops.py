@@ -2044,28 +2044,24 @@ def _same_device(what, *tensors):
         raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devices))}")
 
 
-class _on:
-    """Makes `dev` the current device for a launch (and its stream the one that is used); free of cost where it is already."""
-    __slots__ = ("guard",)
+def _call(index, fn, *args):
+    """fn(*args, stream) on GPU `index`, which becomes the current device for the launch if it is not; checks the result."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, fn.__name__)
 
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _rows_of(t, cols):
     """2-D view [rows, cols] with contiguous columns of a [..., cols] tensor (a copy only if its strides allow no such view)."""
     t = t.reshape(-1, cols) if t.ndim != 2 else t
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < 0):
-        t = t.contiguous()
-    return t
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
 
 
 class GatedResidualNormFn(torch.autograd.Function):
@@ -2080,45 +2076,61 @@ class GatedResidualNormFn(torch.autograd.Function):
         return r, y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dr, dy):
-        x, h, gate, scale, w1, b1, w2, b2, stats = ctx.saved_tensors
-        cfg = ctx.cfg
-        if dr is None and dy is None:
-            return (None,) * 9
-        need = ctx.needs_input_grad
-        rows, cols = x.shape
+        return _residual_norm_bwd_once(ctx, dr, dy) if torch.is_grad_enabled() else _residual_norm_bwd(ctx, dr, dy)
 
-        def out(i, like, dtype=None):
-            if not need[i] or like is None:
-                return None
-            return torch.empty(like.shape, dtype=dtype or like.dtype, device=x.device)
 
-        dx, dh, dgate, dscale = out(0, x), out(1, h), out(2, gate), out(3, scale)
-        dw1, db1, dw2, db2 = out(4, w1), out(5, b1), out(6, w2), out(7, b2)
-        grads = (dx, dh, dgate, dscale, dw1, db1, dw2, db2)
-        if rows == 0:                        # no cell: nothing to launch, the parameters' sums are empty
-            return tuple(None if t is None else t.zero_() for t in grads) + (None,)
-        with _on(x.device):
-            L = _lib.lib()
-            a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
-            a.stats = stats.data_ptr()
-            if dr is not None:
-                dr = _rows_of(dr, cols)
-                a.dr, a.lddr = dr.data_ptr(), dr.stride(0)
-            if dy is not None:
-                dy = _rows_of(dy, cols)
-                a.dy, a.lddy = dy.data_ptr(), dy.stride(0)
-            for name, t in zip(("dx", "dh", "dgate", "dscale", "dw1", "db1", "dw2", "db2"), grads):
-                if t is not None:
-                    setattr(a, name, t.data_ptr())
-            ws = None
-            if dscale is not None or dw1 is not None or db1 is not None or dw2 is not None or db2 is not None \
-                    or (dgate is not None and cfg["gate_mode"] == 3):
-                ws = torch.empty(L.scp_residual_norm_bwd_ws_floats(rows, cols), dtype=torch.float32, device=x.device)
-                a.ws = ws.data_ptr()
-            _lib.check(L.scp_residual_norm_bwd(C.byref(a), _lib.stream()), "scp_residual_norm_bwd")
-        return grads + (None,)
+def _residual_norm_bwd(ctx, dr, dy):
+    x, h, gate, scale, w1, b1, w2, b2, stats = ctx.saved_tensors
+    if dr is None and dy is None:
+        return (None,) * 9
+    cfg, need = ctx.cfg, ctx.needs_input_grad
+    rows, cols = x.shape
+    dx = x.new_empty((rows, cols)) if need[0] else None
+    dh = h.new_empty((rows, cols)) if need[1] else None
+    dgate = torch.empty_like(gate, memory_format=torch.contiguous_format) if need[2] else None
+    dscale = torch.empty_like(scale) if need[3] else None
+    # the norms' parameter gradients: rows of one small tensor
+    n = need[4] + need[5] + need[6] + need[7]
+    small = iter(x.new_empty((n, cols), dtype=torch.float32).unbind(0)) if n else None
+    dw1, db1, dw2, db2 = (next(small) if need[i] else None for i in (4, 5, 6, 7))
+    grads = dx, dh, dgate, dscale, dw1, db1, dw2, db2, None
+    if rows == 0:                        # no cell: nothing to launch, the parameters' sums are empty
+        return tuple(None if t is None else t.zero_() for t in grads)
+    L = _lib.lib()
+    a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
+    a.stats = stats.data_ptr()
+    if dr is not None:
+        dr = _rows_of(dr, cols)
+        a.dr, a.lddr = dr.data_ptr(), dr.stride(0)
+    if dy is not None:
+        dy = _rows_of(dy, cols)
+        a.dy, a.lddy = dy.data_ptr(), dy.stride(0)
+    if dx is not None:
+        a.dx = dx.data_ptr()
+    if dh is not None:
+        a.dh = dh.data_ptr()
+    if dgate is not None:
+        a.dgate = dgate.data_ptr()
+    if dscale is not None:
+        a.dscale = dscale.data_ptr()
+    if dw1 is not None:
+        a.dw1 = dw1.data_ptr()
+    if db1 is not None:
+        a.db1 = db1.data_ptr()
+    if dw2 is not None:
+        a.dw2 = dw2.data_ptr()
+    if db2 is not None:
+        a.db2 = db2.data_ptr()
+    ws = None
+    if n or dscale is not None or (dgate is not None and cfg["gate_mode"] == 3):
+        ws = x.new_empty((L.scp_residual_norm_bwd_ws_floats(rows, cols),), dtype=torch.float32)
+        a.ws = ws.data_ptr()
+    _call(x.get_device(), L.scp_residual_norm_bwd, C.byref(a))
+    return grads
+
+
+_residual_norm_bwd_once = torch.autograd.function.once_differentiable(_residual_norm_bwd)      # a second derivative is refused
 
 
 def _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg):
@@ -2149,19 +2161,17 @@ def _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg):
 
 def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, want_stats):
     rows, cols = x.shape
-    with _on(x.device):
-        r = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if h is not None else None
-        y = torch.empty((rows, cols), dtype=cfg["y_type"], device=x.device)
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
-        if rows == 0:
-            return r, y, stats
+    r = x.new_empty((rows, cols)) if h is not None else None
+    y = x.new_empty((rows, cols), dtype=cfg["y_type"])
+    stats = x.new_empty((rows, 4), dtype=torch.float32) if want_stats else None
+    if rows:
         a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
         a.y = y.data_ptr()
         if r is not None:
             a.r = r.data_ptr()
         if stats is not None:
             a.stats = stats.data_ptr()
-        _lib.check(_lib.lib().scp_residual_norm_fwd(C.byref(a), _lib.stream()), "scp_residual_norm_fwd")
+        _call(x.get_device(), _lib.lib().scp_residual_norm_fwd, C.byref(a))
     return r, y, stats
 
 
@@ -2229,14 +2239,14 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
         if not isinstance(scale, torch.Tensor):
             cfg["scale_value"], scale = float(scale), None
         elif scale.numel() == 1 and scale.is_floating_point():
-            cfg["scale_mode"], scale = 1, _f32c(scale.reshape(1))
+            cfg["scale_mode"], scale = 1, _f32c(scale)
         else:
             cfg["scale_mode"], scale = 2, column("scale", scale, None)
     if gate is not None:
         if gate.shape == shape and gate.dtype == h.dtype:
             cfg["gate_mode"], gate = 1, _rows_of(gate, cols)
         elif gate.shape == (*shape[:-1], 1) and gate.is_floating_point() and len(shape) > 1:
-            cfg["gate_mode"], gate = 2, _f32c(gate.reshape(rows))
+            cfg["gate_mode"], gate = 2, _f32c(gate)
         elif gate.shape == (cols,) and gate.is_floating_point():
             cfg["gate_mode"], gate = 3, _f32c(gate)
         else:
@@ -2251,7 +2261,9 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
         r, y = GatedResidualNormFn.apply(*tensors, cfg)
     else:
         r, y, _ = _residual_norm_fwd(*tensors, cfg, False)
-    return x if h is None else r.reshape(shape), y.reshape(shape)
+    if x.ndim != 2:
+        r, y = None if h is None else r.reshape(shape), y.reshape(shape)
+    return x if h is None else r, y
 
 
 # ------------------------------------------------------------------------------------------------
@@ -2277,28 +2289,9 @@ def _check_floats(what, t):
                          f"{f'{t.dtype} {tuple(t.shape)}' if isinstance(t, torch.Tensor) else type(t).__name__}")
 
 
-def _empty_packed(rows, cols, dev):
-    ld = (cols + 63) // 64 * 64
-    return (torch.empty((rows, ld), dtype=torch.int8, device=dev), torch.empty((rows, ld // 64), dtype=torch.uint8, device=dev))
-
-
-def _pack8_rows(x):
-    rows, cols = x.shape
-    codes, steps = _empty_packed(rows, cols, x.device)
-    if x.numel():
-        with _on(x.device):
-            _lib.check(_lib.lib().scp_pack8(x.data_ptr(), x.dtype == torch.bfloat16, x.stride(0), rows, cols, codes.data_ptr(),
-                                            steps.data_ptr(), _lib.stream()), "scp_pack8")
-    return codes, steps
-
-
-def _unpack8_rows(codes, steps, rows, cols, dtype):
-    out = torch.empty((rows, cols), dtype=dtype, device=codes.device)
-    if out.numel():
-        with _on(codes.device):
-            _lib.check(_lib.lib().scp_unpack8(codes.data_ptr(), steps.data_ptr(), rows, cols, out.data_ptr(),
-                                              dtype == torch.bfloat16, _lib.stream()), "scp_unpack8")
-    return out
+def _empty_packed(rows, cols, ref):
+    groups = (cols + 63) // 64
+    return ref.new_empty((rows, 64 * groups), dtype=torch.int8), ref.new_empty((rows, groups), dtype=torch.uint8)
 
 
 def pack8(x):
@@ -2308,8 +2301,11 @@ def pack8(x):
     _check_floats("pack8", x)
     _same_device("pack8", x)
     cols = x.shape[-1]
-    rows = x.numel() // cols if cols else math.prod(x.shape[:-1])
-    codes, steps = _pack8_rows(_rows_of(x.detach(), cols)) if x.numel() else _empty_packed(rows, cols, x.device)
+    codes, steps = _empty_packed(math.prod(x.shape[:-1]), cols, x)
+    if x.numel():
+        t = _rows_of(x.detach(), cols)
+        _call(t.get_device(), _lib.lib().scp_pack8, t.data_ptr(), t.dtype == torch.bfloat16, t.stride(0), t.shape[0], cols,
+              codes.data_ptr(), steps.data_ptr())
     return Packed8(codes, steps, x.shape, x.dtype)
 
 
@@ -2322,7 +2318,11 @@ def unpack8(p, dtype=None):
     if dtype not in _FLOATS:
         raise ValueError(f"unpack8: float32 or bfloat16, got {dtype}")
     _same_device("unpack8", p.codes, p.steps)
-    return _unpack8_rows(p.codes, p.steps, p.codes.shape[0], p.shape[-1], dtype).reshape(p.shape)
+    out = p.codes.new_empty(p.shape, dtype=dtype)
+    if out.numel():
+        _call(out.get_device(), _lib.lib().scp_unpack8, p.codes.data_ptr(), p.steps.data_ptr(), p.codes.shape[0], p.shape[-1],
+              out.data_ptr(), dtype == torch.bfloat16)
+    return out
 
 
 _ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
@@ -2330,11 +2330,10 @@ _ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
 
 def _act8_fwd(z, kind, slope, keep):
     rows, cols = z.shape
-    out = torch.empty((rows, cols), dtype=z.dtype, device=z.device)
-    codes, steps = _empty_packed(rows, cols, z.device) if keep else (None, None)
-    with _on(z.device):
-        _lib.check(_lib.lib().scp_act8_fwd(z.data_ptr(), z.dtype == torch.bfloat16, z.stride(0), rows, cols, kind, slope,
-                                           out.data_ptr(), _lib.ptr(codes), _lib.ptr(steps), _lib.stream()), "scp_act8_fwd")
+    out = z.new_empty((rows, cols))
+    codes, steps = _empty_packed(rows, cols, z) if keep else (None, None)
+    _call(z.get_device(), _lib.lib().scp_act8_fwd, z.data_ptr(), z.dtype == torch.bfloat16, z.stride(0), rows, cols, kind, slope,
+          out.data_ptr(), _lib.ptr(codes), _lib.ptr(steps))
     return out, codes, steps
 
 
@@ -2343,21 +2342,25 @@ class Act8Fn(torch.autograd.Function):
     def forward(ctx, z, kind, slope):
         out, codes, steps = _act8_fwd(z, kind, slope, True)
         ctx.save_for_backward(codes, steps)
-        ctx.cfg = (*z.shape, kind, slope)
+        ctx.cfg = kind, slope
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        codes, steps = ctx.saved_tensors
-        rows, cols, kind, slope = ctx.cfg
-        dz = torch.empty((rows, cols), dtype=dout.dtype, device=dout.device)
-        dout = _rows_of(dout, cols)
-        with _on(dout.device):
-            _lib.check(_lib.lib().scp_act8_bwd(codes.data_ptr(), steps.data_ptr(), rows, cols, kind, slope, dout.data_ptr(),
-                                               dout.dtype == torch.bfloat16, dout.stride(0), dz.data_ptr(), _lib.stream()),
-                       "scp_act8_bwd")
-        return dz, None, None
+        return _act8_bwd_once(ctx, dout) if torch.is_grad_enabled() else _act8_bwd(ctx, dout)
+
+
+def _act8_bwd(ctx, dout):
+    codes, steps = ctx.saved_tensors
+    rows, cols = dout.shape
+    dout = _rows_of(dout, cols)
+    dz = dout.new_empty((rows, cols))
+    _call(dz.get_device(), _lib.lib().scp_act8_bwd, codes.data_ptr(), steps.data_ptr(), rows, cols, *ctx.cfg, dout.data_ptr(),
+          dout.dtype == torch.bfloat16, dout.stride(0), dz.data_ptr())
+    return dz, None, None
+
+
+_act8_bwd_once = torch.autograd.function.once_differentiable(_act8_bwd)      # a second derivative is refused
 
 
 def act8(z, kind="gelu", slope=0.01):
@@ -2370,109 +2373,88 @@ def act8(z, kind="gelu", slope=0.01):
     _same_device("act8", z)
     if z.numel() == 0:
         return z.clone()
-    rows = _rows_of(z, z.shape[-1])
+    t = _rows_of(z, z.shape[-1])
     if torch.is_grad_enabled() and z.requires_grad:
-        return Act8Fn.apply(rows, _ACTS8[kind], float(slope)).reshape(z.shape)
-    return _act8_fwd(rows, _ACTS8[kind], float(slope), False)[0].reshape(z.shape)
+        out = Act8Fn.apply(t, _ACTS8[kind], float(slope))
+    else:
+        out = _act8_fwd(t, _ACTS8[kind], float(slope), False)[0]
+    return out if z.ndim == 2 else out.reshape(z.shape)
 
 
-def _bf16_operand(t):
-    """t [rows, cols] (bfloat16 or float32) as the matrix kernels take it: bfloat16, rows of a multiple of 8 elements from a
-    16-byte boundary, zeros behind the columns.  t itself where it is that already."""
-    rows, cols = t.shape
-    if t.dtype == torch.float32:
-        return cast_bf16(t if t.is_contiguous() else t.contiguous(), rows, cols)
-    if cols % 8 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    out = torch.empty((rows, (cols + 7) // 8 * 8), dtype=torch.bfloat16, device=t.device)
-    _lib.check(_lib.lib().scp_pad_bf16(t.data_ptr(), t.stride(0), rows, cols, out.data_ptr(), out.shape[1], _lib.stream()),
-               "scp_pad_bf16")
-    return out
+def _linear8_args(x, W, split):
+    a = _lib.Linear8()
+    a.M, a.K, a.N = x.shape[0], x.shape[1], W.shape[0]
+    a.W, a.x_bf16, a.w_bf16, a.ns = W.data_ptr(), x.dtype == torch.bfloat16, W.dtype == torch.bfloat16, 3 if split else 1
+    return a
 
 
-def _rows_gemm(b_col, a, B, n, k, out, bias=None):
-    """out[rows, n] = a B^T (b_col 0) or a B (b_col 1), + bias; bf16 operands of _bf16_operand, bf16 or fp32 out.  The kernels
-    address an operand with 31 bits, so a longer batch runs in pieces."""
+def _linear8_run(what, a, index, ref):
+    """One of the two C entries with its workspace (none where the shape needs none)."""
     L = _lib.lib()
-    rows, lda = a.shape
-    piece = ((1 << 31) - 8192) // (2 * lda)
-    for r0 in range(0, rows, piece):
-        m = min(piece, rows - r0)
-        ai, oi = a[r0:r0 + m], out[r0:r0 + m]
-        if out.dtype == torch.float32:
-            gemm_bf16(0, b_col, m, n, k, ai, lda, B, B.shape[1], oi, n, bias=bias)
-            continue
-        nws = L.scp_gemm_bf16_ws_floats(m, n, k, n)
-        ws = torch.empty((nws,), dtype=torch.float32, device=a.device) if nws else None
-        _lib.check(L.scp_gemm_bf16_c16(0, b_col, m, n, k, ai.data_ptr(), lda, B.data_ptr(), B.shape[1], oi.data_ptr(), n,
-                                       _lib.ptr(bias), _lib.ptr(ws), _lib.stream()), "scp_gemm_bf16_c16")
+    nws = getattr(L, what + "_ws")(C.byref(a))
+    if nws < 0:
+        _lib.check(-1, what)
+    ws = ref.new_empty((nws,), dtype=torch.uint8) if nws else None
+    if nws:
+        a.ws = ws.data_ptr()
+    _call(index, getattr(L, what), C.byref(a))
 
 
-def _linear8_fwd(x, W, b, split):
+def _linear8_fwd(x, W, b, split, keep):
     M, K = x.shape
-    N = W.shape[0]
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((M, W.shape[0]))
+    codes, steps = _empty_packed(M, K, x) if keep else (None, None)
+    a = _linear8_args(x, W, split)
     if M:
-        with _on(x.device):
-            if split:
-                xc, Wc = _f32c(x), _f32c(W)
-                gemm_nt_auto(M, N, K, xc, K, 1, Wc, K, 1, y, bias=b)
-            else:
-                _rows_gemm(0, _bf16_operand(x), _bf16_operand(W), N, K, y, bias=b)
-    return y
+        a.x, a.ldx, a.y = x.data_ptr(), x.stride(0), y.data_ptr()
+        if b is not None:
+            a.b = b.data_ptr()
+        if keep:
+            a.codes, a.steps = codes.data_ptr(), steps.data_ptr()
+        _linear8_run("scp_linear8_fwd", a, x.get_device(), x)
+    return y, codes, steps
 
 
 class Linear8Fn(torch.autograd.Function):
-    """y = x W^T + b for 2-D x; keeps x as an 8-bit checkpoint and W.  bf16 operands: the wide MFMA kernels (csrc/wgemm.hip),
-    the weight gradient reading the codes; fp32 tensors in precision 'fp32': the split products (csrc/gemm.hip)."""
+    """scp_linear8_fwd / _bwd (csrc/linear8.hip); keeps x as an 8-bit checkpoint, and W."""
 
     @staticmethod
     def forward(ctx, x, W, b, split):
-        ctx.split, ctx.dims = split, (x.shape[0], *W.shape)
-        codes, steps = _pack8_rows(x) if ctx.needs_input_grad[1] else (None, None)
+        y, codes, steps = _linear8_fwd(x, W, b, split, ctx.needs_input_grad[1])
         ctx.save_for_backward(codes, steps, W)
-        return _linear8_fwd(x, W, b, split)
+        ctx.split, ctx.dims = split, x.shape
+        return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        codes, steps, W = ctx.saved_tensors
-        M, N, K = ctx.dims
-        L = _lib.lib()
-        dx = dW = db = None
-        dy = _rows_of(dy, N)
-        with _on(dy.device):
-            if ctx.needs_input_grad[0]:
-                dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
-            if ctx.needs_input_grad[1]:
-                dW = torch.empty((N, K), dtype=W.dtype, device=dy.device)
-            if ctx.needs_input_grad[2]:
-                db = torch.empty((N,), dtype=torch.float32, device=dy.device)
-            if M == 0:
-                return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_(), None
-            if ctx.split:
-                d, Wc = _f32c(dy), _f32c(W)
-                if dx is not None:
-                    gemm_nt_auto(M, K, N, d, N, 1, Wc, 1, K, dx)
-                if dW is not None:
-                    gemm_nt_auto(N, K, M, d, 1, N, _unpack8_rows(codes, steps, M, K, torch.float32), 1, K, dW)
-            else:
-                d = _bf16_operand(dy)
-                if dx is not None:
-                    _rows_gemm(1, d, _bf16_operand(W), K, N, dx)
-                if dW is not None:
-                    nws = L.scp_gemm_q8_ws_floats(N, K, M, max(d.shape[1], codes.shape[1]), K)
-                    ws = torch.empty((nws,), dtype=torch.float32, device=dy.device) if nws else None
-                    _lib.check(L.scp_gemm_q8(N, K, M, d.data_ptr(), d.shape[1], codes.data_ptr(), steps.data_ptr(), dW.data_ptr(),
-                                             dW.dtype == torch.bfloat16, K, _lib.ptr(ws), _lib.stream()), "scp_gemm_q8")
-            if db is not None:
-                if dy.dtype == torch.bfloat16:
-                    ws = torch.empty((L.scp_colsum_bf16_ws_floats(M, N),), dtype=torch.float32, device=dy.device)
-                    _lib.check(L.scp_colsum_bf16(dy.data_ptr(), dy.stride(0), M, N, db.data_ptr(), ws.data_ptr(), _lib.stream()),
-                               "scp_colsum_bf16")
-                else:
-                    db = colsum(dy, M, N, ld=dy.stride(0))
-        return dx, dW, db, None
+        return _linear8_bwd_once(ctx, dy) if torch.is_grad_enabled() else _linear8_bwd(ctx, dy)
+
+
+def _linear8_bwd(ctx, dy):
+    codes, steps, W = ctx.saved_tensors
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    M, K = ctx.dims
+    dy = _rows_of(dy, W.shape[0])
+    dx = dy.new_empty((M, K)) if need_x else None
+    dW = torch.empty_like(W) if need_w else None
+    db = dy.new_empty((W.shape[0],), dtype=torch.float32) if need_b else None
+    if M == 0:
+        return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_(), None
+    a = _lib.Linear8()
+    a.M, a.K, a.N = M, K, W.shape[0]
+    a.W, a.x_bf16, a.w_bf16, a.ns = W.data_ptr(), dy.dtype == torch.bfloat16, W.dtype == torch.bfloat16, 3 if ctx.split else 1
+    a.dy, a.lddy = dy.data_ptr(), dy.stride(0)
+    if need_x:
+        a.dx = dx.data_ptr()
+    if need_w:
+        a.dW, a.codes, a.steps = dW.data_ptr(), codes.data_ptr(), steps.data_ptr()
+    if need_b:
+        a.db = db.data_ptr()
+    _linear8_run("scp_linear8_bwd", a, dy.get_device(), dy)
+    return dx, dW, db, None
+
+
+_linear8_bwd_once = torch.autograd.function.once_differentiable(_linear8_bwd)
 
 
 def linear8(x, W, b=None):
@@ -2490,13 +2472,16 @@ def linear8(x, W, b=None):
     N = W.shape[0]
     if b is not None and (b.shape != (N,) or not b.is_floating_point()):
         raise ValueError(f"linear8: the bias must be a floating-point tensor of shape ({N},), got {b.dtype} {tuple(b.shape)}")
-    if (max(N, K) + 256) * (min(N, K) + 256) * 2 >= (1 << 31) - 4096:
-        raise ValueError(f"linear8: a weight of {N} x {K} passes 2 GiB in bfloat16")
+    if max(N, K) > 1 << 20 or (N + 256) * (K + 256) * 2 >= (1 << 31) - 65536:
+        raise ValueError(f"linear8: a weight of {N} x {K} passes 2 GiB in bfloat16 or 2^20 in one dimension")
     _same_device("linear8", x, W, b)
-    x2, W, b = _rows_of(x, K), W if W.is_contiguous() else W.contiguous(), None if b is None else _f32c(b)
+    x2 = _rows_of(x, K)
+    if x2.shape[0] >= 1 << 30:
+        raise ValueError(f"linear8: at most 2^30 - 1 rows, got {x2.shape[0]}")
+    W, b = W if W.is_contiguous() else W.contiguous(), None if b is None else _f32c(b)
     split = x.dtype == torch.float32 and _ns() == 3
     if torch.is_grad_enabled() and (x.requires_grad or W.requires_grad or (b is not None and b.requires_grad)):
         y = Linear8Fn.apply(x2, W, b, split)
     else:
-        y = _linear8_fwd(x2, W, b, split)
-    return y.reshape(*x.shape[:-1], N)
+        y = _linear8_fwd(x2, W, b, split, False)[0]
+    return y if x.ndim == 2 else y.reshape(*x.shape[:-1], N)

@@ -125,5 +125,26 @@ def test_checkpoint_c_entries_refuse():
     assert L.scp_gemm_q8_ws_floats(1024, 1024, 4_000_000, 1024, 1024) >= 8 * 1024 * 1024
     assert L.scp_gemm_q8(1024, 1024, 4_000_000, a, 1024, a, a, a, 0, 1024, None, None) == -1
     assert b"workspace" in L.scp_last_error()
-    assert L.scp_pad_bf16(a, 9, 2, 9, a, 9, None) == -1 and L.scp_pad_bf16(None, 9, 2, 9, a, 16, None) == -1
-    assert L.scp_colsum_bf16(a, 8, 2, 8, a, None, None) == -1 and L.scp_colsum_bf16_ws_floats(0, 8) == 0
+
+
+def test_linear8_c_entries_refuse():
+    L = _lib.lib()
+
+    def args(**kw):
+        a = _lib.Linear8()
+        for k, v in (dict(x=4096, W=4096, y=4096, dy=4096, M=5, N=8, K=16, ldx=16, lddy=8, ns=3, ws=4096) | kw).items():
+            setattr(a, k, v)
+        return C.byref(a)
+
+    for bad in (dict(M=0), dict(N=0), dict(K=0), dict(w_bf16=1), dict(ns=2), dict(codes=4096), dict(codes=4097, steps=4096)):
+        assert L.scp_linear8_fwd(args(**bad), None) == -1 and L.scp_linear8_bwd(args(**bad), None) == -1, bad
+        assert L.scp_linear8_fwd_ws(args(**bad)) == -1 and L.scp_linear8_bwd_ws(args(**bad)) == -1, bad
+    for bad in (dict(M=1 << 30), dict(K=(1 << 20) + 1), dict(N=40000, K=40000)):
+        assert L.scp_linear8_fwd(args(**bad), None) == -2 and L.scp_linear8_fwd_ws(args(**bad)) == -1, bad
+    for bad in (dict(x=None), dict(W=None), dict(y=None), dict(ldx=-1), dict(ws=None), dict(ws=4096 + 16)):
+        assert L.scp_linear8_fwd(args(**bad), None) == -1, bad
+    for bad in (dict(dy=None), dict(lddy=-1), dict(dx=4096, W=None), dict(dW=4096), dict(dx=4096, ws=None), dict(db=4096, ws=None)):
+        assert L.scp_linear8_bwd(args(**bad), None) == -1, bad
+    # aligned bf16 operands need no copies: the workspace holds K-range slabs only, none for a large product
+    big = dict(x_bf16=1, w_bf16=1, M=16384, N=4096, K=4096, ldx=4096, lddy=4096, dx=4096, dW=4096, codes=4096, steps=4096)
+    assert L.scp_linear8_fwd_ws(args(**big)) == 0 and L.scp_linear8_bwd_ws(args(**big)) == 0
