@@ -388,11 +388,11 @@ int scp_act8_fwd(const void* x, int bf16, long ldx, long rows, int cols, int kin
 int scp_act8_bwd(const int8_t* codes, const uint8_t* steps, long rows, int cols, int kind, float slope, const void* dout,
                  int bf16, long ldd, void* dx, void* stream);
 /* The products of a Linear layer that keeps its input as such a checkpoint.
- * scp_gemm_bf16_c16: scp_gemm_bf16 (a_col 0, no mask) with a bf16 output; ws of scp_gemm_bf16_ws_floats(M, N, K, ldc) floats.
+ * scp_gemm_rows: scp_gemm_bf16 (a_col 0, no mask) with an fp32 or bf16 output; ws of scp_gemm_bf16_ws_floats(M, N, K, ldc) floats.
  * scp_gemm_q8: C[m][n] = sum_k A[k][m] * value(codes, steps)[k][n], the weight gradient: A bf16 [K][lda] (lda % 8 == 0, 16-byte
  * aligned), C fp32 or bf16 [M][ldc]; ws of scp_gemm_q8_ws_floats(M, N, K, max(lda, N rounded up to 64), ldc) floats. */
-int scp_gemm_bf16_c16(int a_col, int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb, void* C,
-                      long ldc, const float* bias, float* ws, void* stream);
+int scp_gemm_rows(int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb, void* C, int c_bf16, long ldc,
+                  const float* bias, float* ws, void* stream);
 long scp_gemm_q8_ws_floats(int M, int N, int K, long ld, long ldc);
 int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const int8_t* codes, const uint8_t* steps, void* C, int c_bf16,
                 long ldc, float* ws, void* stream);

@@ -128,20 +128,20 @@ _SIGS = {
     "scp_fos_counts": (I, [P, L, P, L, I, I, P, P, P, P, P]),
     "scp_adamw_multi": (I, [C.POINTER(AdamTensor), I, F, F, F, P]),
     "scp_residual_norm_max_cols": (I, []),
-    "scp_residual_norm_fwd": (I, [C.POINTER(ResidualNorm), P]),
+    "scp_residual_norm_fwd": (I, [P, P]),
     "scp_residual_norm_bwd_ws_floats": (L, [L, I]),
-    "scp_residual_norm_bwd": (I, [C.POINTER(ResidualNorm), P]),
+    "scp_residual_norm_bwd": (I, [P, P]),
     "scp_pack8": (I, [P, I, L, L, I, P, P, P]),
     "scp_unpack8": (I, [P, P, L, I, P, I, P]),
     "scp_act8_fwd": (I, [P, I, L, L, I, I, F, P, P, P, P]),
     "scp_act8_bwd": (I, [P, P, L, I, I, F, P, I, L, P, P]),
-    "scp_gemm_bf16_c16": (I, [I, I, I, I, I, P, L, P, L, P, L, P, P, P]),
+    "scp_gemm_rows": (I, [I, I, I, I, P, L, P, L, P, I, L, P, P, P]),
     "scp_gemm_q8_ws_floats": (L, [I, I, I, L, L]),
     "scp_gemm_q8": (I, [I, I, I, P, L, P, P, P, I, L, P, P]),
-    "scp_linear8_fwd_ws": (L, [C.POINTER(Linear8)]),
-    "scp_linear8_bwd_ws": (L, [C.POINTER(Linear8)]),
-    "scp_linear8_fwd": (I, [C.POINTER(Linear8), P]),
-    "scp_linear8_bwd": (I, [C.POINTER(Linear8), P]),
+    "scp_linear8_fwd_ws": (L, [P]),
+    "scp_linear8_bwd_ws": (L, [P]),
+    "scp_linear8_fwd": (I, [P, P]),
+    "scp_linear8_bwd": (I, [P, P]),
     "scp_step_state_set": (I, [P, U64, F, F, P]),
 }
 

@@ -19,15 +19,33 @@ namespace {
 
 enum { ACT_GELU = 0, ACT_SILU = 1, ACT_LEAKY = 2 };
 
-__device__ __forceinline__ float act_value(float x, int kind, float slope) {
-  if (kind == ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678f));
-  if (kind == ACT_SILU) return x / (1.f + expf(-x));
+// FAST (bf16 tensors): the hardware exponential and reciprocal, and erfc by Abramowitz & Stegun 7.1.26 (absolute error below
+// 1.5e-7, far under bf16's half step), which shares its exp(-x^2 / 2) with the derivative; with libm's functions the bf16
+// kernels were bound by instruction issue (16384 x 8192 silu: 165 us forward).  fp32 tensors: libm's functions.
+__device__ __forceinline__ float normal_cdf_fast(float x, float gauss) {      // gauss = exp(-x^2 / 2)
+  const float z = fabsf(x) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float tail = 0.5f * p * gauss;
+  return x < 0.f ? tail : 1.f - tail;
+}
+template <bool FAST> __device__ __forceinline__ float act_value(float x, int kind, float slope) {
+  if (kind == ACT_GELU) {
+    if (FAST) return x * normal_cdf_fast(x, __expf(-0.5f * x * x));
+    return 0.5f * x * (1.f + erff(x * 0.70710678f));
+  }
+  if (kind == ACT_SILU) return FAST ? x * __builtin_amdgcn_rcpf(1.f + __expf(-x)) : x / (1.f + expf(-x));
   return x > 0.f ? x : slope * x;
 }
-__device__ __forceinline__ float act_slope(float x, int kind, float slope) {
-  if (kind == ACT_GELU) return 0.5f * (1.f + erff(x * 0.70710678f)) + x * 0.39894228f * expf(-0.5f * x * x);
+template <bool FAST> __device__ __forceinline__ float act_slope(float x, int kind, float slope) {
+  if (kind == ACT_GELU) {
+    if (FAST) {
+      const float gauss = __expf(-0.5f * x * x);
+      return fmaf(x * 0.39894228f, gauss, normal_cdf_fast(x, gauss));
+    }
+    return 0.5f * (1.f + erff(x * 0.70710678f)) + x * 0.39894228f * expf(-0.5f * x * x);
+  }
   if (kind == ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-x));
+    const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
     return s * (1.f + x * (1.f - s));
   }
   return x > 0.f ? 1.f : slope;
@@ -49,7 +67,7 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T* __restrict__ x, lon
     }
     if (ACT) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) f[j] = act_value(f[j], kind, slope);
+      for (int j = 0; j < 8; j++) f[j] = act_value<sizeof(T) == 2>(f[j], kind, slope);
       if (col < s.cols) store8<T>(out + row * s.cols, col, s.cols, f);
     }
   }
@@ -70,7 +88,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t* __restrict__
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       f[j] = (float)(int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3))) * step;
-      if (GRAD) f[j] = g[j] * act_slope(f[j], kind, slope);
+      if (GRAD) f[j] = g[j] * act_slope<sizeof(T) == 2>(f[j], kind, slope);
     }
     store8<T>(out + row * s.cols, col, s.cols, f);
   }

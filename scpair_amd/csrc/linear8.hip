@@ -74,21 +74,34 @@ __global__ __launch_bounds__(256) void lin_prep_kernel(const T* __restrict__ src
   }
 }
 
-// dy: bf16 blocks (dst null: none) and partial column sums part[gridDim.y][cols] (null: none) in one pass.  A workgroup takes
-// 512 columns, 8 per lane, and every gridDim.y-th group of four rows, a row a wave.
-template <typename T, int LAY>
+// dy: bf16 blocks (DST) and partial column sums part[gridDim.y][cols] (null: none) in one pass.  A workgroup takes 512 columns,
+// 8 per lane, and every gridDim.y-th group of four rows, a row a wave, four rows in flight.
+template <typename T, int LAY, bool DST>
 __global__ __launch_bounds__(256) void lin_dy_kernel(const T* __restrict__ x, long ldx, long rows, int cols,
                                                      __bf16* __restrict__ dst, int w, float* __restrict__ part) {
   __shared__ float buf[3][8][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 512 + lane * 8;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (col < cols) {
-    for (long r = (long)blockIdx.y * 4 + wave; r < rows; r += (long)gridDim.y * 4) {
+    const long step = (long)gridDim.y * 4;
+    long r = (long)blockIdx.y * 4 + wave;
+    for (; r + 3 * step < rows; r += 4 * step) {
+      float f[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; u++) load8<T>(x + (r + u * step) * ldx, col, cols, f[u]);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc[i] += f[u][i];
+        if (DST) put8<LAY>(dst, r + u * step, col, w, 0, f[u]);
+      }
+    }
+    for (; r < rows; r += step) {
       float f[8];
       load8<T>(x + r * ldx, col, cols, f);
 #pragma unroll
       for (int i = 0; i < 8; i++) acc[i] += f[i];
-      if (dst) put8<LAY>(dst, r, col, w, 0, f);
+      if (DST) put8<LAY>(dst, r, col, w, 0, f);
     }
   }
   if (!part) return;
@@ -161,10 +174,14 @@ __device__ __forceinline__ bf16x8 lg_frag(const unsigned char* img, int r0, int 
 
 enum { OP_ROW = 0, OP_COL = 1, OP_Q8 = 2 };
 
-// one operand's tiles: global -> registers -> LDS
+// One operand's tiles: global -> registers -> LDS.  What a lane adds to the descriptor's base does not change from step to
+// step; the step itself moves the scalar offset (row operands) or the descriptor (col operands).
 template <int TS, int OP>
 struct Tile {
-  static constexpr int NC = OP == OP_Q8 ? TS / 64 : TS / 32;      // 16-byte chunks per thread and step
+  static constexpr int EB = OP == OP_Q8 ? 1 : 2;                   // bytes per element
+  static constexpr int NC = TS * 64 * EB / 16 / 256;               // 16-byte chunks per thread and step
+  static constexpr int CPR = OP == OP_ROW ? 8 : TS * EB / 16;      // chunks per image row
+  static constexpr int RPI = 256 / CPR;                            // image rows per round of the 256 threads
   struct Reg {
     u32x4 v[NC];
     unsigned step[OP == OP_Q8 ? NC : 1];
@@ -172,61 +189,60 @@ struct Tile {
   const unsigned char* base;     // first byte of the tile's rows (row) / of k row 0 (col)
   const uint8_t* steps;
   long ld;
-  int r0, rows;                  // tile origin; rows left from there (row operands)
-  long cols;                     // columns that a row holds (col operands): the last k row is read no further
-  int K, tid;
+  int kp, K, tail;               // K rounded up to 8 / K / bytes of a last k row, from the tile's first column on
+  int bytes;                     // row operands: extent of the tile's rows
+  int voff[NC], soff[OP == OP_Q8 ? NC : 1], lds[NC];
 
   __device__ __forceinline__ void init(const void* p, const uint8_t* st, long ld_, int origin, int extent, int K_) {
-    tid = threadIdx.x;
     ld = ld_;
-    r0 = origin;
     K = K_;
-    rows = min(TS, extent - origin);
-    cols = OP == OP_Q8 ? ld : (extent + 7) & ~7;
+    kp = (K + 7) & ~7;
     steps = st;
-    base = (const unsigned char*)p + (OP == OP_ROW ? (long)origin * ld * 2 : OP == OP_COL ? (long)origin * 2 : origin);
+    base = (const unsigned char*)p + (OP == OP_ROW ? (long)origin * ld * 2 : (long)origin * EB);
+    bytes = (int)(min(TS, extent - origin) * ld * 2);
+    // a k row is read up to its last column rounded up to a chunk, the last one of the operand no further
+    tail = (int)((OP == OP_Q8 ? ld : (long)((extent + 7) & ~7)) - origin) * EB;
+    const int r = threadIdx.x / CPR, c = threadIdx.x % CPR;
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+      voff[i] = (int)((r + RPI * i) * ld * EB) + 16 * c;
+      lds[i] = OP == OP_ROW ? lg_row_off(r + RPI * i, c) : lg_col_off<TS>(r + RPI * i, 16 / EB * c);
+      if constexpr (OP == OP_Q8) soff[i] = (int)((r + RPI * i) * (ld >> 6)) + ((origin + 16 * c) >> 6);
+    }
   }
   __device__ __forceinline__ void load(Reg& r, int kt, bool live) const {
     const int k0 = kt * 64;
     if constexpr (OP == OP_ROW) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, live ? (int)(rows * ld * 2) : 0, 0x00020000);
-      const int ch = tid & 7, kp = (K + 7) & ~7;
-      const unsigned off = (unsigned)((long)(tid >> 3) * ld * 2) + (unsigned)(k0 + 8 * ch) * 2;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, live ? bytes : 0, 0x00020000);
+      if (k0 + 64 <= kp) {
 #pragma unroll
-      for (int i = 0; i < NC; i++) {
-        const unsigned o = off + (unsigned)(32 * i * ld * 2);
-        r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, k0 + 8 * ch < kp ? (int)o : (int)0x80000000u, 0, 0);
-      }
-    } else {
-      constexpr int EB = OP == OP_Q8 ? 1 : 2, CPR = TS * EB / 16, RPI = 256 / CPR;      // chunks per row, rows per round
-      const int kr = live ? min(64, K - k0) : 0;
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(base + (long)k0 * ld * EB), 0, kr > 0 ? (int)(((kr - 1) * ld + cols - r0) * EB) : 0, 0x00020000);
-      const int k = tid / CPR, c = tid % CPR;
-#pragma unroll
-      for (int i = 0; i < NC; i++)
-        r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)((k + RPI * i) * ld * EB + 16 * c), 0, 0);
-      if constexpr (OP == OP_Q8) {
-        const long lds_ = ld >> 6;
-        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(steps + k0 * lds_), 0, kr > 0 ? (int)(kr * lds_) : 0, 0x00020000);
+        for (int i = 0; i < NC; i++) r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff[i], 2 * k0, 0);
+      } else {         // the step that K ends in: chunks behind it would run into the next row
+        const bool in = k0 + 8 * (int)(threadIdx.x % CPR) < kp;
 #pragma unroll
         for (int i = 0; i < NC; i++)
-          r.step[i] = __builtin_amdgcn_raw_buffer_load_b8(rq, (int)((k + RPI * i) * lds_ + ((r0 + 16 * c) >> 6)), 0, 0);
+          r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, in ? voff[i] + 2 * k0 : (int)0x80000000u, 0, 0);
+      }
+    } else {
+      const int kr = live ? min(64, K - k0) : 0;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(base + (long)k0 * ld * EB), 0, kr > 0 ? (int)((kr - 1) * ld * EB) + tail : 0, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < NC; i++) r.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff[i], 0, 0);
+      if constexpr (OP == OP_Q8) {
+        const long ls = ld >> 6;
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(steps + k0 * ls), 0, kr > 0 ? (int)(kr * ls) : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NC; i++) r.step[i] = __builtin_amdgcn_raw_buffer_load_b8(rq, soff[i], 0, 0);
       }
     }
   }
   __device__ __forceinline__ void store(const Reg& r, unsigned char* img) const {
-    if constexpr (OP == OP_ROW) {
 #pragma unroll
-      for (int i = 0; i < NC; i++) *(u32x4*)(img + lg_row_off((tid >> 3) + 32 * i, tid & 7)) = r.v[i];
-    } else if constexpr (OP == OP_COL) {
-      constexpr int CPR = TS / 8, RPI = 256 / CPR;
-#pragma unroll
-      for (int i = 0; i < NC; i++) *(u32x4*)(img + lg_col_off<TS>(tid / CPR + RPI * i, 8 * (tid % CPR))) = r.v[i];
-    } else {
-      constexpr int CPR = TS / 16, RPI = 256 / CPR;
-#pragma unroll
-      for (int i = 0; i < NC; i++) {
+    for (int i = 0; i < NC; i++) {
+      if constexpr (OP != OP_Q8) {
+        *(u32x4*)(img + lds[i]) = r.v[i];
+      } else {
         const float step = q8_step(r.step[i]), off = -128.f * step;
         bf16x8 v[2];
 #pragma unroll
@@ -235,17 +251,15 @@ struct Tile {
 #pragma unroll
           for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = (__bf16)fmaf((float)((u >> (8 * b)) & 0xffu), step, off);
         }
-        unsigned char* p = img + lg_col_off<TS>(tid / CPR + RPI * i, 16 * (tid % CPR));
-        const int odd = tid & 1;      // neighbours write different halves of their 32 bytes at a time: no bank conflict
-        *(bf16x8*)(p + 16 * odd) = odd ? v[1] : v[0];
-        *(bf16x8*)(p + 16 - 16 * odd) = odd ? v[0] : v[1];
+        *(bf16x8*)(img + lds[i]) = v[0];
+        *(bf16x8*)(img + lds[i] + 16) = v[1];
       }
     }
   }
 };
 
 template <int TS, int OPA, int OPB, typename CT>
-__global__ __launch_bounds__(256) void lgemm_kernel(LgArgs g) {
+__global__ __launch_bounds__(256, TS == 64 ? 4 : 2) void lgemm_kernel(LgArgs g) {
   constexpr int NI = TS / 64, WT = TS / 2, IMG = TS * 128, DEPTH = TS == 64 ? 4 : 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
@@ -253,7 +267,9 @@ __global__ __launch_bounds__(256) void lgemm_kernel(LgArgs g) {
   const int per_z = g.tiles_m * g.tiles_n, total = per_z * g.nsplit * g.planes, per_xcd = (total + 7) >> 3;
   const int lid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   if (lid >= total || (int)(blockIdx.x >> 3) >= per_xcd) return;
-  const int tm = lid % g.tiles_m, tn = (lid / g.tiles_m) % g.tiles_n, z = lid / per_z;
+  // and those in blocks of 8 tile rows, walked column by column: the tiles at work on an XCD share a few rows and columns
+  const int z = lid / per_z, t = lid - z * per_z, grp = t / (8 * g.tiles_n), in = t - grp * 8 * g.tiles_n;
+  const int gh = min(8, g.tiles_m - 8 * grp), tn = in / gh, tm = 8 * grp + in - tn * gh;
   const int m0 = tm * TS, n0 = tn * TS, plane = z / g.nsplit;
   const int kt0 = (z % g.nsplit) * g.per_split, kt1 = min((g.K + 63) / 64, kt0 + g.per_split);
 
@@ -361,32 +377,28 @@ struct Gemm {
   long ws;             // workspace bytes
 };
 
-// Tile and K-ranges of one product of `planes` column blocks.  Cost model in microseconds, rates measured on the kernels at
-// one workgroup per CU: a step of 64 k, the slabs written and read again, 4 us for the launch that adds them.
-Gemm pick(long M, int N, long K, int planes, bool wide_ok, long wide_ws) {
+// Tile and K-ranges of one product of `planes` column blocks: the cheapest by a model in microseconds.  A step of 64 k with
+// w workgroups per CU took, measured over products from 300^3 to 16384 x 4096^2: 0.25 + 0.2 w at 64 x 64, 1.15 (w = 1) or
+// 0.70 w at 128 x 128, 2.3 w at 256 x 256; slabs are written and read at 7.5 TB/s, and a launch costs 3.5 us.
+Gemm pick(long M, int N, long K, int planes, bool wide_ok, int wide_ns, long wide_ws) {
   Gemm best = {256, 1, 0, wide_ws};
   const long nk = (K + 63) / 64;
+  const double mn = (double)M * N;
   double best_us = 1e30;
   if (wide_ok) {
-    const double tiles = (double)((M + 255) / 256) * ((N + 255) / 256) * planes;
-    double ns = 256.0 / tiles;
-    ns = ns < 1 ? 1 : ns > nk / 8.0 ? (nk < 8 ? 1 : nk / 8.0) : ns > 16 ? 16 : ns;
-    const double rounds = tiles * ns / 256;
-    best_us = (rounds < 1 ? 1 : rounds) * nk / ns * 2.1 + 4;
-    if (ns > 1.01 || planes > 1) best_us += (ns * planes + 1) * M * N * 8 / 4e6 + 4;
+    const long tiles = ((M + 255) / 256) * ((N + 255) / 256) * wide_ns;
+    best_us = planes * ((tiles + 255) / 256 * 2.3 * ((nk + wide_ns - 1) / wide_ns) + 3.5);
+    if (wide_ns > 1) best_us += planes * (mn * 4 * (2 * wide_ns + 1) / 7.5e6 + 3.5);
+    if (planes > 1) best_us += mn * 4 * (2 * planes + 1) / 7.5e6 + 3.5;
   }
   for (int ts = 64; ts <= 128; ts += 64) {
     const long tiles = ((M + ts - 1) / ts) * ((N + ts - 1) / ts) * planes;
-    if (tiles >= 1L << 26) continue;
-    const int per_cu = ts == 64 ? 4 : 2;               // resident workgroups
-    for (int ns = 1; ns <= 16; ns *= 2) {
+    if (tiles >= 1L << 24) continue;
+    for (int ns = 1; ns <= 64; ns *= 2) {
       if (ns > 1 && nk / ns < 4) break;
-      const double wgs = (double)tiles * ns, rounds = wgs <= 256 ? 1 : wgs / 256;
-      const double step = ts == 64 ? 0.30 : 0.75, floor_step = ts == 64 ? 0.11 : 0.42;
-      // few workgroups: a step is its latency; many: several share a CU and a step is its work
-      double us = wgs <= 256 * per_cu ? nk / ns * (step > floor_step * rounds ? step : floor_step * rounds) : nk / ns * floor_step * rounds;
-      us += 4;
-      if (ns * planes > 1) us += (ns * planes + 1.0) * M * N * 4 / 4e6 + 4;
+      const double w = (double)((tiles * ns + 255) / 256);
+      double us = 3.5 + (nk + ns - 1) / ns * (ts == 64 ? 0.25 + 0.2 * w : w == 1 ? 1.15 : 0.7 * w);
+      if (ns * planes > 1) us += mn * 4 * (2 * ns * planes + 1) / 7.5e6 + 3.5;
       if (us < best_us) {
         best_us = us;
         best.ts = ts;
@@ -417,7 +429,7 @@ struct Plan {
 };
 
 int colsum_parts(long rows, int cols) {
-  const long groups = (rows + 3) / 4, cols_wg = (cols + 511) / 512, cap = cols_wg < 16 ? 512 / cols_wg : 32;
+  const long groups = (rows + 3) / 4, cols_wg = (cols + 511) / 512, cap = cols_wg < 32 ? 1024 / cols_wg : 32;
   return (int)(groups < cap ? groups : cap);
 }
 
@@ -427,6 +439,8 @@ void common_plan(const ScpLinear8& a, Plan& p) {
   p.Np = up8(a.N);
   p.w_direct = a.w_bf16 && a.K % 8 == 0 && ((uintptr_t)a.W & 15) == 0;
 }
+
+int wide_splits(long M, int N, long K) { return scp_gemm_bf16_nsplit((int)M, N, (int)K); }
 
 long wide_ws_rows(const Plan& p, long M, int N, long K, long lda) {
   const long piece = WIDE_BYTES / (2 * lda);
@@ -446,7 +460,7 @@ Plan plan_fwd(const ScpLinear8& a) {
   p.b_off = o;
   if (!p.w_direct) o += align256((long)a.N * KK * 2);
   const bool ok = ((long)a.N + 192) * KK * 2 < WIDE_BYTES;
-  p.y = pick(a.M, a.N, KK, 1, ok, ok ? wide_ws_rows(p, a.M, a.N, KK, p.x_direct ? a.ldx : KK) : 0);
+  p.y = pick(a.M, a.N, KK, 1, ok, wide_splits(a.M, a.N, KK), ok ? wide_ws_rows(p, a.M, a.N, KK, p.x_direct ? a.ldx : KK) : 0);
   p.g_off = o;
   p.total = o + align256(p.y.ws);
   return p;
@@ -471,15 +485,15 @@ Plan plan_bwd(const ScpLinear8& a) {
   if (a.dx) {
     const long K2 = p.np == 1 ? a.N : NN;
     const bool ok = (K2 + 192) * p.Kp * 2 < WIDE_BYTES;
-    p.dx = pick(a.M, a.K, K2, 1, ok, ok ? wide_ws_rows(p, a.M, a.K, K2, p.dy_direct ? a.N : NN) : 0);
+    p.dx = pick(a.M, a.K, K2, 1, ok, wide_splits(a.M, a.K, K2), ok ? wide_ws_rows(p, a.M, a.K, K2, p.dy_direct ? a.N : NN) : 0);
     g = p.dx.ws;
   }
   if (a.dW) {
     const int planes = p.np == 6 ? 3 : 1;
     const long ld8 = (a.K + 63) / 64 * 64L, lda = p.dy_direct ? a.N : NN;
     // the wide form runs once per plane, each into a slab of its own
-    const long ws = a.M < (1L << 31) ? scp_gemm_q8_ws_floats(a.N, a.K, (int)a.M, lda > ld8 ? lda : ld8, a.K) * 4 : 0;
-    p.dw = pick(a.N, a.K, a.M, planes, a.M < (1L << 31), align256(ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
+    const long ws = scp_gemm_q8_ws_floats(a.N, a.K, (int)a.M, lda > ld8 ? lda : ld8, a.K) * 4;
+    p.dw = pick(a.N, a.K, a.M, planes, true, wide_splits(a.N, a.K, a.M), align256(ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
     if (p.dw.ws > g) g = p.dw.ws;
   }
   p.total = p.g_off + align256(g);
@@ -554,8 +568,7 @@ int rows_product(const Gemm& q, int b_col, long M, int N, long K, const __bf16* 
     void* c = c_bf16 ? (void*)((__bf16*)C + r * N) : (void*)((float*)C + r * N);
     int rc;
     if (q.ts == 256) {
-      rc = c_bf16 ? scp_gemm_bf16_c16(0, b_col, m, N, (int)K, A + r * lda, lda, B, ldb, c, N, bias, ws, st)
-                  : scp_gemm_bf16(0, b_col, m, N, (int)K, A + r * lda, lda, B, ldb, (float*)c, N, bias, nullptr, 0, ws, st);
+      rc = scp_gemm_rows(b_col, m, N, (int)K, A + r * lda, lda, B, ldb, c, c_bf16, N, bias, ws, st);
     } else {
       LgArgs g = {};
       g.A = A + r * lda; g.B = B; g.C = c;
@@ -567,6 +580,52 @@ int rows_product(const Gemm& q, int b_col, long M, int N, long K, const __bf16* 
     if (rc) return rc;
   }
   return SCP_OK;
+}
+
+// dy's blocks (write) and, if asked for, its column sums
+int dy_pass(const ScpLinear8& a, const Plan& p, bool write, hipStream_t st) {
+  char* ws = (char*)a.ws;
+  __bf16* dst = write ? (__bf16*)(ws + p.a_off) : nullptr;
+  float* part = a.db ? (float*)(ws + p.part_off) : nullptr;
+  const dim3 grid((a.N + 511) / 512, p.parts);
+#define DY(T, LAY, DST) \
+  hipLaunchKernelGGL((lin_dy_kernel<T, LAY, DST>), grid, dim3(256), 0, st, (const T*)a.dy, a.lddy, a.M, a.N, dst, p.Np, part)
+  if (a.x_bf16 && !write) DY(__bf16, LAY_ONE, false);
+  else if (a.x_bf16) DY(__bf16, LAY_ONE, true);
+  else if (!write) DY(float, LAY_ONE, false);
+  else if (p.np == 1) DY(float, LAY_ONE, true);
+  else DY(float, LAY_COLS_A, true);
+#undef DY
+  SCP_LAUNCH_CHECK();
+  if (a.db) {
+    hipLaunchKernelGGL(lin_db_kernel, dim3((a.N + 15) / 16), dim3(256), 0, st, part, p.parts, a.N, a.db);
+    SCP_LAUNCH_CHECK();
+  }
+  return SCP_OK;
+}
+
+// dW = dy^T v; A: dy's blocks
+int weight_product(const ScpLinear8& a, const Plan& p, const __bf16* A, long lda, float* ws, hipStream_t st) {
+  const int planes = p.np == 6 ? 3 : 1;
+  const int off[3] = {0, 2 * p.Np, 5 * p.Np};
+  if (p.dw.ts == 256) {
+    if (planes == 1) return scp_gemm_q8(a.N, a.K, (int)a.M, A, lda, a.codes, a.steps, a.dW, a.w_bf16, a.K, ws, st);
+    const long NK = (long)a.N * a.K;
+    float* slabs = ws + (p.dw.ws - 3 * NK * 4) / 4;
+    for (int i = 0; i < 3; i++)
+      if (int rc = scp_gemm_q8(a.N, a.K, (int)a.M, A + off[i], lda, a.codes, a.steps, slabs + i * NK, 0, a.K, ws, st)) return rc;
+    hipLaunchKernelGGL((lin_sum_kernel<float>), dim3((unsigned)((NK + 1023) / 1024)), dim3(256), 0, st, slabs, 3, NK, a.K, nullptr,
+                       (float*)a.dW);
+    SCP_LAUNCH_CHECK();
+    return SCP_OK;
+  }
+  LgArgs g = {};
+  g.A = A; g.B = a.codes; g.steps = a.steps; g.C = a.dW;
+  g.lda = lda; g.ldb = (a.K + 63) / 64 * 64;
+  g.M = a.N; g.N = a.K; g.K = (int)a.M;
+  g.planes = planes;
+  for (int i = 0; i < 3; i++) g.plane_off[i] = off[i];
+  return small_gemm<OP_COL, OP_Q8>(p.dw, g, a.w_bf16, nullptr, ws, st);
 }
 
 int check_args(const ScpLinear8* a, const char* who) {
@@ -642,22 +701,9 @@ extern "C" int scp_linear8_bwd(const ScpLinear8* a_, void* stream) {
     A = (const __bf16*)(ws + p.a_off);
     lda = NN;
   }
-  if (write_dy || a.db) {
-    __bf16* dst = write_dy ? (__bf16*)(ws + p.a_off) : nullptr;
-    float* part = a.db ? (float*)(ws + p.part_off) : nullptr;
-    const dim3 grid((a.N + 511) / 512, p.parts);
-    if (a.x_bf16)
-      hipLaunchKernelGGL((lin_dy_kernel<__bf16, LAY_ONE>), grid, dim3(256), 0, st, (const __bf16*)a.dy, a.lddy, a.M, a.N, dst, p.Np, part);
-    else if (p.np == 1)
-      hipLaunchKernelGGL((lin_dy_kernel<float, LAY_ONE>), grid, dim3(256), 0, st, (const float*)a.dy, a.lddy, a.M, a.N, dst, p.Np, part);
-    else
-      hipLaunchKernelGGL((lin_dy_kernel<float, LAY_COLS_A>), grid, dim3(256), 0, st, (const float*)a.dy, a.lddy, a.M, a.N, dst, p.Np, part);
-    SCP_LAUNCH_CHECK();
-  }
-  if (a.db) {
-    hipLaunchKernelGGL(lin_db_kernel, dim3((a.N + 15) / 16), dim3(256), 0, st, (const float*)(ws + p.part_off), p.parts, a.N, a.db);
-    SCP_LAUNCH_CHECK();
-  }
+  // The column sums come out of the pass that writes the operand's blocks; where none is needed, they come last, when the
+  // products have left dy in the last-level cache (16384 x 4096 bf16: 43 us before them, 20 us after).
+  if (write_dy && (rc = dy_pass(a, p, true, st))) return rc;
   if (a.dx) {
     const __bf16* B = (const __bf16*)a.W;
     if (!p.w_direct) {
@@ -667,27 +713,6 @@ extern "C" int scp_linear8_bwd(const ScpLinear8* a_, void* stream) {
     if ((rc = rows_product(p.dx, 1, a.M, a.K, p.np == 1 ? a.N : NN, A, lda, B, p.w_direct ? a.K : p.Kp, a.dx, a.x_bf16, nullptr, gws, st)))
       return rc;
   }
-  if (a.dW) {
-    const int planes = p.np == 6 ? 3 : 1;
-    const int off[3] = {0, 2 * p.Np, 5 * p.Np};
-    if (p.dw.ts == 256) {
-      if (planes == 1) return scp_gemm_q8(a.N, a.K, (int)a.M, A, lda, a.codes, a.steps, a.dW, a.w_bf16, a.K, gws, stream);
-      const long NK = (long)a.N * a.K;
-      float* slabs = gws + (p.dw.ws - 3 * NK * 4) / 4;
-      for (int i = 0; i < 3; i++)
-        if ((rc = scp_gemm_q8(a.N, a.K, (int)a.M, A + off[i], lda, a.codes, a.steps, slabs + i * NK, 0, a.K, gws, stream))) return rc;
-      hipLaunchKernelGGL((lin_sum_kernel<float>), dim3((unsigned)((NK + 1023) / 1024)), dim3(256), 0, st, slabs, 3, NK, a.K, nullptr,
-                         (float*)a.dW);
-      SCP_LAUNCH_CHECK();
-      return SCP_OK;
-    }
-    LgArgs g = {};
-    g.A = A; g.B = a.codes; g.steps = a.steps; g.C = a.dW;
-    g.lda = lda; g.ldb = (a.K + 63) / 64 * 64;
-    g.M = a.N; g.N = a.K; g.K = (int)a.M;
-    g.planes = planes;
-    for (int i = 0; i < 3; i++) g.plane_off[i] = off[i];
-    return small_gemm<OP_COL, OP_Q8>(p.dw, g, a.w_bf16, nullptr, gws, st);
-  }
-  return SCP_OK;
+  if (a.dW && (rc = weight_product(a, p, A, lda, gws, st))) return rc;
+  return a.db && !write_dy ? dy_pass(a, p, false, st) : SCP_OK;
 }

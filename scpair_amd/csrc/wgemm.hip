@@ -38,6 +38,7 @@ struct WgArgs {
   long lda, ldb, ldc, ldm;
   int M, N, K;
   int tiles_m, tiles_n, nsplit, ksteps_per_split;
+  int group;           // order of the tiles: 0 along m, else in blocks of that many tile rows
   unsigned a_bytes, b_bytes;
   unsigned c_bytes, m_bytes;   // extent of C (one slab) and of the mask when both are below 2 GiB, else 0 (guarded global stores)
   // weight gradient with the AdamW step applied in the epilogue (EPI_ADAMW): C = fp32 master weights, updated in place
@@ -103,9 +104,14 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   const int per_xcd = (total + 7) >> 3;
   const int lid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   if (lid >= total) return;
-  const int tm = lid % g.tiles_m;
-  const int tn = (lid / g.tiles_m) % g.tiles_n;
-  const int z = lid / (g.tiles_m * g.tiles_n);
+  const int per_z = g.tiles_m * g.tiles_n, z = lid / per_z;
+  int tm = lid % g.tiles_m, tn = (lid / g.tiles_m) % g.tiles_n;
+  if (g.group) {                        // blocks of `group` tile rows, walked column by column
+    const int t = lid - z * per_z, b = t / (g.group * g.tiles_n), r = t - b * g.group * g.tiles_n;
+    const int h = min(g.group, g.tiles_m - g.group * b);
+    tn = r / h;
+    tm = g.group * b + r - tn * h;
+  }
   const int m0 = tm * TM, n0 = tn * TN;
   const int nk_all = (g.K + TK - 1) / TK;
   const int kt0 = z * g.ksteps_per_split;
@@ -190,11 +196,9 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
 #pragma unroll
           for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = (__bf16)fmaf((float)((u >> (8 * b)) & 0xffu), step, off);
         }
-        // odd lanes write their second half first: the 16 lanes of a row then cover all banks in each of the two stores
         unsigned char* p = ib + col_off(rQ + 32 * i, 16 * cQ);
-        const int odd = cQ & 1;
-        *(bf16x8*)(p + 16 * odd) = odd ? v[1] : v[0];
-        *(bf16x8*)(p + 16 - 16 * odd) = odd ? v[0] : v[1];
+        *(bf16x8*)p = v[0];
+        *(bf16x8*)(p + 16) = v[1];
       }
       return;
     }
@@ -571,6 +575,10 @@ int reduce_slabs(const WgArgs& g, const float* ws, const float* bias, CT* C, hip
   return SCP_OK;
 }
 
+// Order of the tiles for the products of linear8: with long K-ranges, blocks of 8 tile rows, so that the 32 tiles at work on an
+// XCD share 8 + 4 operand tiles instead of 32 + 1 (16384 x 4096 x 4096: 575 -> 520 us)
+int tile_group(const WgArgs& g) { return g.ksteps_per_split >= 32 ? 8 : 0; }
+
 // K-ranges of a product with an 8-bit operand: at least as many as keep a range's bytes below 1 GiB
 int q8_nsplit(int M, int N, int K, long lda) {
   const int nk = (K + TK - 1) / TK;
@@ -708,19 +716,19 @@ extern "C" int scp_gemm_bf16(int a_col, int b_col, int M, int N, int K, const vo
   return SCP_OK;
 }
 
-extern "C" int scp_gemm_bf16_c16(int a_col, int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb,
-                                 void* C, long ldc, const float* bias, float* ws, void* stream_) {
-  SCP_CHECK(M > 0 && N > 0 && K > 0, SCP_ERR_ARG, "scp_gemm_bf16_c16: M, N, K must be positive (%d, %d, %d)", M, N, K);
-  SCP_CHECK(A && B && C, SCP_ERR_ARG, "scp_gemm_bf16_c16: null pointer");
-  SCP_CHECK(a_col == 0 && (b_col == 0 || b_col == 1), SCP_ERR_ARG, "scp_gemm_bf16_c16: a_col must be 0, b_col 0 or 1");
+extern "C" int scp_gemm_rows(int b_col, int M, int N, int K, const void* A, long lda, const void* B, long ldb, void* C,
+                             int c_bf16, long ldc, const float* bias, float* ws, void* stream_) {
+  SCP_CHECK(M > 0 && N > 0 && K > 0, SCP_ERR_ARG, "scp_gemm_rows: M, N, K must be positive (%d, %d, %d)", M, N, K);
+  SCP_CHECK(A && B && C, SCP_ERR_ARG, "scp_gemm_rows: null pointer");
+  SCP_CHECK(b_col == 0 || b_col == 1, SCP_ERR_ARG, "scp_gemm_rows: b_col must be 0 or 1");
   const long b_rows = b_col ? K : N, b_cols = b_col ? N : K;
   SCP_CHECK(lda >= ((K + 7) & ~7L) && ldb >= ((b_cols + 7) & ~7L) && ldc >= N, SCP_ERR_ARG,
-            "scp_gemm_bf16_c16: leading dimension too small (operands are padded to a multiple of 8 columns)");
+            "scp_gemm_rows: leading dimension too small (operands are padded to a multiple of 8 columns)");
   SCP_CHECK(lda % 8 == 0 && ldb % 8 == 0 && ((uintptr_t)A & 15) == 0 && ((uintptr_t)B & 15) == 0, SCP_ERR_ARG,
-            "scp_gemm_bf16_c16: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
+            "scp_gemm_rows: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
   // the slack of scp_gemm_bf16: offset + dead-load mark must not carry out of 32 bits
   SCP_CHECK((long)M * lda * 2 + 4096 < (1L << 31) && (b_rows + (b_col ? 3 * TK : 0)) * ldb * 2 + 4096 < (1L << 31), SCP_ERR_SHAPE,
-            "scp_gemm_bf16_c16: an operand within 3 K-steps of 2 GiB (or larger) is not supported");
+            "scp_gemm_rows: an operand within 3 K-steps of 2 GiB (or larger) is not supported");
   WgArgs g = {};
   g.A = (const __bf16*)A; g.B = (const __bf16*)B;
   g.lda = lda; g.ldb = ldb; g.ldc = ldc;
@@ -730,18 +738,24 @@ extern "C" int scp_gemm_bf16_c16(int a_col, int b_col, int M, int N, int K, cons
   g.ksteps_per_split = ((K + TK - 1) / TK + g.nsplit - 1) / g.nsplit;
   g.a_bytes = (unsigned)((long)M * lda * 2);
   g.b_bytes = (unsigned)(b_rows * ldb * 2);
-  SCP_CHECK((long)g.tiles_m * g.tiles_n * g.nsplit < (1L << 30), SCP_ERR_SHAPE, "scp_gemm_bf16_c16: too many tiles");
+  SCP_CHECK((long)g.tiles_m * g.tiles_n * g.nsplit < (1L << 30), SCP_ERR_SHAPE, "scp_gemm_rows: too many tiles");
+  g.group = tile_group(g);
+  const long cb = (long)M * ldc * 4;
+  g.c_bytes = cb < (1L << 31) ? (unsigned)cb : 0u;
+  g.m_bytes = 2;
   hipStream_t st = (hipStream_t)stream_;
   if (g.nsplit == 1) {
     g.C = (float*)C;
     g.bias = bias;
+    if (!c_bf16) return b_col ? launch<false, true>(g, st) : launch<false, false>(g, st);
     return b_col ? launch8<false, true, EPI_DIRECT, false, __bf16>(g, st) : launch8<false, false, EPI_DIRECT, false, __bf16>(g, st);
   }
-  SCP_CHECK(ws, SCP_ERR_ARG, "scp_gemm_bf16_c16: this shape runs as %d K-ranges and needs the workspace of scp_gemm_bf16_ws_floats",
+  SCP_CHECK(ws, SCP_ERR_ARG, "scp_gemm_rows: this shape runs as %d K-ranges and needs the workspace of scp_gemm_bf16_ws_floats",
             g.nsplit);
   g.C = ws;
   const int rc = b_col ? launch8<false, true, EPI_SLAB, false, float>(g, st) : launch8<false, false, EPI_SLAB, false, float>(g, st);
-  return rc ? rc : reduce_slabs(g, ws, bias, (__bf16*)C, st);
+  if (rc) return rc;
+  return c_bf16 ? reduce_slabs(g, ws, bias, (__bf16*)C, st) : reduce_slabs(g, ws, bias, (float*)C, st);
 }
 
 extern "C" long scp_gemm_q8_ws_floats(int M, int N, int K, long lda, long ldc) {
@@ -770,6 +784,7 @@ extern "C" int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const i
   SCP_CHECK(range * lda * 2 + 4096 < (1L << 31) && range * ldb + 4096 < (1L << 31), SCP_ERR_SHAPE,
             "scp_gemm_q8: a K-range of %ld rows of %ld columns passes 2 GiB", range, lda > ldb ? lda : ldb);
   SCP_CHECK((long)g.tiles_m * g.tiles_n * g.nsplit < (1L << 30), SCP_ERR_SHAPE, "scp_gemm_q8: too many tiles");
+  g.group = tile_group(g);
   hipStream_t st = (hipStream_t)stream_;
   if (g.nsplit == 1) {
     g.C = (float*)C;

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct as _struct
 
 import torch
 
@@ -2036,12 +2037,15 @@ _GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
-def _same_device(what, *tensors):
+def _same_device(what, first, *others):
     """Refuses CPU tensors and tensors of several GPUs in one call (None entries are skipped)."""
-    _lib.require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devices))}")
+    index = first.get_device()
+    if index < 0:
+        _lib.require_cuda(first)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _lib.require_cuda(t)
+            raise ValueError(f"{what}: tensors on different devices: {first.device}, {t.device}")
 
 
 def _call(index, fn, *args):
@@ -2089,74 +2093,47 @@ def _residual_norm_bwd(ctx, dr, dy):
     dx = x.new_empty((rows, cols)) if need[0] else None
     dh = h.new_empty((rows, cols)) if need[1] else None
     dgate = torch.empty_like(gate, memory_format=torch.contiguous_format) if need[2] else None
-    dscale = torch.empty_like(scale) if need[3] else None
-    # the norms' parameter gradients: rows of one small tensor
-    n = need[4] + need[5] + need[6] + need[7]
+    # the columns' gradients: rows of one small tensor
+    scale_col = need[3] and cfg["scale_mode"] == 2
+    n = need[4] + need[5] + need[6] + need[7] + scale_col
     small = iter(x.new_empty((n, cols), dtype=torch.float32).unbind(0)) if n else None
-    dw1, db1, dw2, db2 = (next(small) if need[i] else None for i in (4, 5, 6, 7))
+    dscale = next(small) if scale_col else torch.empty_like(scale) if need[3] else None
+    dw1 = next(small) if need[4] else None
+    db1 = next(small) if need[5] else None
+    dw2 = next(small) if need[6] else None
+    db2 = next(small) if need[7] else None
     grads = dx, dh, dgate, dscale, dw1, db1, dw2, db2, None
     if rows == 0:                        # no cell: nothing to launch, the parameters' sums are empty
         return tuple(None if t is None else t.zero_() for t in grads)
     L = _lib.lib()
-    a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
-    a.stats = stats.data_ptr()
     if dr is not None:
         dr = _rows_of(dr, cols)
-        a.dr, a.lddr = dr.data_ptr(), dr.stride(0)
     if dy is not None:
         dy = _rows_of(dy, cols)
-        a.dy, a.lddy = dy.data_ptr(), dy.stride(0)
-    if dx is not None:
-        a.dx = dx.data_ptr()
-    if dh is not None:
-        a.dh = dh.data_ptr()
-    if dgate is not None:
-        a.dgate = dgate.data_ptr()
-    if dscale is not None:
-        a.dscale = dscale.data_ptr()
-    if dw1 is not None:
-        a.dw1 = dw1.data_ptr()
-    if db1 is not None:
-        a.db1 = db1.data_ptr()
-    if dw2 is not None:
-        a.dw2 = dw2.data_ptr()
-    if db2 is not None:
-        a.db2 = db2.data_ptr()
     ws = None
     if n or dscale is not None or (dgate is not None and cfg["gate_mode"] == 3):
         ws = x.new_empty((L.scp_residual_norm_bwd_ws_floats(rows, cols),), dtype=torch.float32)
-        a.ws = ws.data_ptr()
-    _call(x.get_device(), L.scp_residual_norm_bwd, C.byref(a))
+    _call(x.get_device(), L.scp_residual_norm_bwd,
+          _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg, (None, None, stats, dr, dy) + grads[:8] + (ws,)))
     return grads
 
 
 _residual_norm_bwd_once = torch.autograd.function.once_differentiable(_residual_norm_bwd)      # a second derivative is refused
 
 
-def _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg):
+_RNORM_BLOCK = _struct.Struct("22P6l8i2f2i")      # ScpResidualNorm, packed in one go: a call is dominated by its host time
+
+
+def _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg, rest):
+    """The argument block; rest: r, y, stats, dr, dy, dx, dh, dgate, dscale, dw1, db1, dw2, db2, ws (tensors or None)."""
     rows, cols = x.shape
-    a = _lib.ResidualNorm()
-    a.x, a.ldx, a.rows, a.cols = x.data_ptr(), x.stride(0), rows, cols
-    a.x_bf16, a.h_bf16 = x.dtype == torch.bfloat16, cfg["y_type"] == torch.bfloat16
-    a.post, a.pre, a.eps, a.scale_value = cfg["post"], cfg["pre"], cfg["eps"], cfg["scale_value"]
-    a.gate_mode, a.gate_act, a.scale_mode = cfg["gate_mode"], cfg["gate_act"], cfg["scale_mode"]
-    if h is not None:
-        a.h, a.ldh = h.data_ptr(), h.stride(0)
-    if gate is not None:
-        a.gate = gate.data_ptr()
-        if cfg["gate_mode"] == 1:
-            a.ldg = gate.stride(0)
-    if scale is not None:
-        a.scale = scale.data_ptr()
-    if w1 is not None:
-        a.w1 = w1.data_ptr()
-    if b1 is not None:
-        a.b1 = b1.data_ptr()
-    if w2 is not None:
-        a.w2 = w2.data_ptr()
-    if b2 is not None:
-        a.b2 = b2.data_ptr()
-    return a
+    dr, dy = rest[3], rest[4]
+    return _RNORM_BLOCK.pack(
+        *[0 if t is None else t.data_ptr() for t in (x, h, gate, scale, w1, b1, w2, b2) + rest],
+        x.stride(0), 0 if h is None else h.stride(0), gate.stride(0) if cfg["gate_mode"] == 1 else 0,
+        0 if dr is None else dr.stride(0), 0 if dy is None else dy.stride(0), rows,
+        cols, x.dtype == torch.bfloat16, cfg["y_type"] == torch.bfloat16, cfg["post"], cfg["pre"], cfg["gate_mode"],
+        cfg["gate_act"], cfg["scale_mode"], cfg["scale_value"], cfg["eps"], 0, 0)
 
 
 def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, want_stats):
@@ -2165,14 +2142,17 @@ def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, want_stats):
     y = x.new_empty((rows, cols), dtype=cfg["y_type"])
     stats = x.new_empty((rows, 4), dtype=torch.float32) if want_stats else None
     if rows:
-        a = _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg)
-        a.y = y.data_ptr()
-        if r is not None:
-            a.r = r.data_ptr()
-        if stats is not None:
-            a.stats = stats.data_ptr()
-        _call(x.get_device(), _lib.lib().scp_residual_norm_fwd, C.byref(a))
+        _call(x.get_device(), _lib.lib().scp_residual_norm_fwd,
+              _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg, (r, y, stats) + (None,) * 11))
     return r, y, stats
+
+
+def _param(name, t, shape):
+    if t.dtype is torch.float32 and t.shape == shape and t.is_contiguous():
+        return t
+    if t.shape != shape or not t.is_floating_point():
+        raise ValueError(f"gated_residual_norm: {name} must be a floating-point tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    return _f32c(t)
 
 
 def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight=None, post_bias=None, pre="layer",
@@ -2223,31 +2203,26 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
     if post is None and (post_weight is not None or post_bias is not None):
         raise ValueError("gated_residual_norm: post_weight / post_bias without a post norm")
 
-    def column(name, t, norm):
-        if t is None:
-            return None
-        if norm == "rms" and name.endswith("bias"):
-            raise ValueError(f"gated_residual_norm: {name} with an rms norm, which has none")
-        if t.shape != (cols,) or not t.is_floating_point():
-            raise ValueError(f"gated_residual_norm: {name} must be a floating-point tensor of shape ({cols},), got "
-                             f"{t.dtype} {tuple(t.shape)}")
-        return _f32c(t)
-
-    w1, b1 = column("post_weight", post_weight, post), column("post_bias", post_bias, post)
-    w2, b2 = column("pre_weight", pre_weight, pre), column("pre_bias", pre_bias, pre)
+    column = (cols,)
+    w1 = None if post_weight is None else _param("post_weight", post_weight, column)
+    b1 = None if post_bias is None else _param("post_bias", post_bias, column)
+    w2 = None if pre_weight is None else _param("pre_weight", pre_weight, column)
+    b2 = None if pre_bias is None else _param("pre_bias", pre_bias, column)
+    if (b1 is not None and post == "rms") or (b2 is not None and pre == "rms"):
+        raise ValueError("gated_residual_norm: a bias with an rms norm, which has none")
     if scale is not None:
         if not isinstance(scale, torch.Tensor):
             cfg["scale_value"], scale = float(scale), None
         elif scale.numel() == 1 and scale.is_floating_point():
             cfg["scale_mode"], scale = 1, _f32c(scale)
         else:
-            cfg["scale_mode"], scale = 2, column("scale", scale, None)
+            cfg["scale_mode"], scale = 2, _param("scale", scale, column)
     if gate is not None:
         if gate.shape == shape and gate.dtype == h.dtype:
             cfg["gate_mode"], gate = 1, _rows_of(gate, cols)
         elif gate.shape == (*shape[:-1], 1) and gate.is_floating_point() and len(shape) > 1:
             cfg["gate_mode"], gate = 2, _f32c(gate)
-        elif gate.shape == (cols,) and gate.is_floating_point():
+        elif gate.shape == column and gate.is_floating_point():
             cfg["gate_mode"], gate = 3, _f32c(gate)
         else:
             raise ValueError(f"gated_residual_norm: a gate is {tuple(shape)} of {y_type}, {(*shape[:-1], 1)} or ({cols},), got "
@@ -2381,37 +2356,31 @@ def act8(z, kind="gelu", slope=0.01):
     return out if z.ndim == 2 else out.reshape(z.shape)
 
 
-def _linear8_args(x, W, split):
-    a = _lib.Linear8()
-    a.M, a.K, a.N = x.shape[0], x.shape[1], W.shape[0]
-    a.W, a.x_bf16, a.w_bf16, a.ns = W.data_ptr(), x.dtype == torch.bfloat16, W.dtype == torch.bfloat16, 3 if split else 1
-    return a
+_LINEAR8_BLOCK = _struct.Struct("11P3l5i4x")      # ScpLinear8
 
 
-def _linear8_run(what, a, index, ref):
-    """One of the two C entries with its workspace (none where the shape needs none)."""
+def _linear8_run(what, tensors, M, N, K, ldx, lddy, x16, w16, split, ref):
+    """One of the two C entries with its workspace (none where the shape needs none); tensors: the block's ten pointers."""
     L = _lib.lib()
-    nws = getattr(L, what + "_ws")(C.byref(a))
+    ptrs = [0 if t is None else t.data_ptr() for t in tensors]
+    shape = (M, ldx, lddy, N, K, x16, w16, 3 if split else 1)
+    fwd = what == "fwd"
+    nws = (L.scp_linear8_fwd_ws if fwd else L.scp_linear8_bwd_ws)(_LINEAR8_BLOCK.pack(*ptrs, 0, *shape))
     if nws < 0:
-        _lib.check(-1, what)
+        _lib.check(-1, "scp_linear8_" + what)
     ws = ref.new_empty((nws,), dtype=torch.uint8) if nws else None
-    if nws:
-        a.ws = ws.data_ptr()
-    _call(index, getattr(L, what), C.byref(a))
+    _call(ref.get_device(), L.scp_linear8_fwd if fwd else L.scp_linear8_bwd,
+          _LINEAR8_BLOCK.pack(*ptrs, ws.data_ptr() if nws else 0, *shape))
 
 
 def _linear8_fwd(x, W, b, split, keep):
     M, K = x.shape
-    y = x.new_empty((M, W.shape[0]))
+    N = W.shape[0]
+    y = x.new_empty((M, N))
     codes, steps = _empty_packed(M, K, x) if keep else (None, None)
-    a = _linear8_args(x, W, split)
     if M:
-        a.x, a.ldx, a.y = x.data_ptr(), x.stride(0), y.data_ptr()
-        if b is not None:
-            a.b = b.data_ptr()
-        if keep:
-            a.codes, a.steps = codes.data_ptr(), steps.data_ptr()
-        _linear8_run("scp_linear8_fwd", a, x.get_device(), x)
+        _linear8_run("fwd", (x, W, b, y, codes, steps, None, None, None, None), M, N, K, x.stride(0), 0,
+                     x.dtype == torch.bfloat16, W.dtype == torch.bfloat16, split, x)
     return y, codes, steps
 
 
@@ -2440,17 +2409,8 @@ def _linear8_bwd(ctx, dy):
     db = dy.new_empty((W.shape[0],), dtype=torch.float32) if need_b else None
     if M == 0:
         return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_(), None
-    a = _lib.Linear8()
-    a.M, a.K, a.N = M, K, W.shape[0]
-    a.W, a.x_bf16, a.w_bf16, a.ns = W.data_ptr(), dy.dtype == torch.bfloat16, W.dtype == torch.bfloat16, 3 if ctx.split else 1
-    a.dy, a.lddy = dy.data_ptr(), dy.stride(0)
-    if need_x:
-        a.dx = dx.data_ptr()
-    if need_w:
-        a.dW, a.codes, a.steps = dW.data_ptr(), codes.data_ptr(), steps.data_ptr()
-    if need_b:
-        a.db = db.data_ptr()
-    _linear8_run("scp_linear8_bwd", a, dy.get_device(), dy)
+    _linear8_run("bwd", (None, W, None, None, codes, steps, dy, dx, dW, db), M, W.shape[0], K, 0, dy.stride(0),
+                 dy.dtype == torch.bfloat16, W.dtype == torch.bfloat16, ctx.split, dy)
     return dx, dW, db, None
 
 

@@ -113,10 +113,10 @@ def test_checkpoint_c_entries_refuse():
     assert L.scp_unpack8(a, None, 2, 8, a, 0, None) == -1 and L.scp_unpack8(a, a, 2, 8, None, 0, None) == -1
     assert L.scp_act8_fwd(a, 0, 8, 2, 8, 3, 0.0, a, a, a, None) == -1 and L.scp_act8_fwd(a, 0, 8, 2, 8, 0, 0.0, a, a, None, None) == -1
     assert L.scp_act8_bwd(a, a, 2, 8, -1, 0.0, a, 0, 8, a, None) == -1 and L.scp_act8_bwd(a, a, 2, 8, 0, 0.0, None, 0, 8, a, None) == -1
-    assert L.scp_gemm_bf16_c16(1, 0, 8, 8, 8, a, 8, a, 8, a, 8, None, None, None) == -1
-    assert L.scp_gemm_bf16_c16(0, 0, 8, 8, 9, a, 8, a, 16, a, 8, None, None, None) == -1
-    assert L.scp_gemm_bf16_c16(0, 0, 8, 8, 8, a + 2, 8, a, 8, a, 8, None, None, None) == -1
-    assert L.scp_gemm_bf16_c16(0, 0, 1 << 20, 8, 1024, a, 1024, a, 1024, a, 8, None, None, None) == -2
+    assert L.scp_gemm_rows(2, 8, 8, 8, a, 8, a, 8, a, 1, 8, None, None, None) == -1
+    assert L.scp_gemm_rows(0, 8, 8, 9, a, 8, a, 16, a, 1, 8, None, None, None) == -1
+    assert L.scp_gemm_rows(0, 8, 8, 8, a + 2, 8, a, 8, a, 0, 8, None, None, None) == -1
+    assert L.scp_gemm_rows(0, 1 << 20, 8, 1024, a, 1024, a, 1024, a, 1, 8, None, None, None) == -2
     assert L.scp_gemm_q8(8, 8, 8, a, 8, a, None, a, 0, 8, None, None) == -1
     assert L.scp_gemm_q8(9, 8, 8, a, 8, a, a, a, 0, 8, None, None) == -1
     assert L.scp_gemm_q8(8, 8, 8, a, 12, a, a, a, 0, 8, None, None) == -1
