@@ -164,6 +164,23 @@ def lib():
     return _lib
 
 
+_trunk = None
+
+
+def trunk():
+    """The autograd nodes of the residual-trunk operators (csrc/trunk_binding.cpp), which launch through the library above."""
+    global _trunk
+    if _trunk is None:
+        lib()
+        try:
+            from . import _trunk as module
+        except ImportError as e:
+            raise RuntimeError(f"scpair_amd/_trunk.so cannot be loaded ({e}): build it with scpair_amd/csrc/build.sh "
+                               "(there is no fallback)") from e
+        _trunk = module
+    return _trunk
+
+
 class ScpError(RuntimeError):
     pass
 

@@ -20,6 +20,15 @@ for p in "${pids[@]}"; do wait $p; done
 rm -f "$OBJ/libgemm.o"
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o "$OUT" "$OBJ"/*.o
 echo "built $OUT"
+# autograd nodes of the residual-trunk operators: host code against torch's headers, launches through the library above
+EXT="$HERE/../_trunk.so"
+if [ "$HERE/trunk_binding.cpp" -nt "$EXT" ] || [ "$HERE/build.sh" -nt "$EXT" ] || [ "$ROOT/include/scpair_hip.h" -nt "$EXT" ]; then
+  read -r TORCH PYINC <<< "$(python3 -c 'import os, sysconfig, torch; print(os.path.dirname(torch.__file__), sysconfig.get_paths()["include"])')"
+  g++ -O2 -std=c++17 -fPIC -shared -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -I"$ROOT/include" -isystem "$TORCH/include" \
+    -isystem "$TORCH/include/torch/csrc/api/include" -isystem /opt/rocm/include -isystem "$PYINC" "$HERE/trunk_binding.cpp" -o "$EXT" \
+    -L"$HERE/.." -l:libscpair_hip.so -L"$TORCH/lib" -ltorch_python -ltorch -ltorch_cpu -lc10 -lc10_hip -Wl,-rpath,'$ORIGIN'
+  echo "built $EXT"
+fi
 # benchmark-only comparison library (rocBLAS bf16 GEMM beside the hand-written wide GEMM): not part of the product
 CMP="$ROOT/benchmarks/rocblas_cmp"
 if [ "$CMP/rocblas_cmp.hip" -nt "$CMP/librocblas_cmp.so" ]; then

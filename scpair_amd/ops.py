@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-import struct as _struct
 
 import torch
 
@@ -2048,103 +2047,10 @@ def _same_device(what, first, *others):
             raise ValueError(f"{what}: tensors on different devices: {first.device}, {t.device}")
 
 
-def _call(index, fn, *args):
-    """fn(*args, stream) on GPU `index`, which becomes the current device for the launch if it is not; checks the result."""
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc, fn.__name__)
-
-
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
 def _rows_of(t, cols):
     """2-D view [rows, cols] with contiguous columns of a [..., cols] tensor (a copy only if its strides allow no such view)."""
     t = t.reshape(-1, cols) if t.ndim != 2 else t
     return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
-
-
-class GatedResidualNormFn(torch.autograd.Function):
-    """scp_residual_norm_fwd / _bwd (csrc/residual_norm.hip); arguments as gated_residual_norm checked and laid them out."""
-
-    @staticmethod
-    def forward(ctx, x, h, gate, scale, w1, b1, w2, b2, cfg):
-        r, y, stats = _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, True)
-        ctx.save_for_backward(x, h, gate, scale, w1, b1, w2, b2, stats)
-        ctx.cfg = cfg
-        ctx.set_materialize_grads(False)
-        return r, y
-
-    @staticmethod
-    def backward(ctx, dr, dy):
-        return _residual_norm_bwd_once(ctx, dr, dy) if torch.is_grad_enabled() else _residual_norm_bwd(ctx, dr, dy)
-
-
-def _residual_norm_bwd(ctx, dr, dy):
-    x, h, gate, scale, w1, b1, w2, b2, stats = ctx.saved_tensors
-    if dr is None and dy is None:
-        return (None,) * 9
-    cfg, need = ctx.cfg, ctx.needs_input_grad
-    rows, cols = x.shape
-    dx = x.new_empty((rows, cols)) if need[0] else None
-    dh = h.new_empty((rows, cols)) if need[1] else None
-    dgate = torch.empty_like(gate, memory_format=torch.contiguous_format) if need[2] else None
-    # the columns' gradients: rows of one small tensor
-    scale_col = need[3] and cfg["scale_mode"] == 2
-    n = need[4] + need[5] + need[6] + need[7] + scale_col
-    small = iter(x.new_empty((n, cols), dtype=torch.float32).unbind(0)) if n else None
-    dscale = next(small) if scale_col else torch.empty_like(scale) if need[3] else None
-    dw1 = next(small) if need[4] else None
-    db1 = next(small) if need[5] else None
-    dw2 = next(small) if need[6] else None
-    db2 = next(small) if need[7] else None
-    grads = dx, dh, dgate, dscale, dw1, db1, dw2, db2, None
-    if rows == 0:                        # no cell: nothing to launch, the parameters' sums are empty
-        return tuple(None if t is None else t.zero_() for t in grads)
-    L = _lib.lib()
-    if dr is not None:
-        dr = _rows_of(dr, cols)
-    if dy is not None:
-        dy = _rows_of(dy, cols)
-    ws = None
-    if n or dscale is not None or (dgate is not None and cfg["gate_mode"] == 3):
-        ws = x.new_empty((L.scp_residual_norm_bwd_ws_floats(rows, cols),), dtype=torch.float32)
-    _call(x.get_device(), L.scp_residual_norm_bwd,
-          _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg, (None, None, stats, dr, dy) + grads[:8] + (ws,)))
-    return grads
-
-
-_residual_norm_bwd_once = torch.autograd.function.once_differentiable(_residual_norm_bwd)      # a second derivative is refused
-
-
-_RNORM_BLOCK = _struct.Struct("22P6l8i2f2i")      # ScpResidualNorm, packed in one go: a call is dominated by its host time
-
-
-def _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg, rest):
-    """The argument block; rest: r, y, stats, dr, dy, dx, dh, dgate, dscale, dw1, db1, dw2, db2, ws (tensors or None)."""
-    rows, cols = x.shape
-    dr, dy = rest[3], rest[4]
-    return _RNORM_BLOCK.pack(
-        *[0 if t is None else t.data_ptr() for t in (x, h, gate, scale, w1, b1, w2, b2) + rest],
-        x.stride(0), 0 if h is None else h.stride(0), gate.stride(0) if cfg["gate_mode"] == 1 else 0,
-        0 if dr is None else dr.stride(0), 0 if dy is None else dy.stride(0), rows,
-        cols, x.dtype == torch.bfloat16, cfg["y_type"] == torch.bfloat16, cfg["post"], cfg["pre"], cfg["gate_mode"],
-        cfg["gate_act"], cfg["scale_mode"], cfg["scale_value"], cfg["eps"], 0, 0)
-
-
-def _residual_norm_fwd(x, h, gate, scale, w1, b1, w2, b2, cfg, want_stats):
-    rows, cols = x.shape
-    r = x.new_empty((rows, cols)) if h is not None else None
-    y = x.new_empty((rows, cols), dtype=cfg["y_type"])
-    stats = x.new_empty((rows, 4), dtype=torch.float32) if want_stats else None
-    if rows:
-        _call(x.get_device(), _lib.lib().scp_residual_norm_fwd,
-              _residual_norm_args(x, h, gate, scale, w1, b1, w2, b2, cfg, (r, y, stats) + (None,) * 11))
-    return r, y, stats
 
 
 def _param(name, t, shape):
@@ -2173,7 +2079,6 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
     if not isinstance(x, torch.Tensor) or x.ndim == 0:
         raise ValueError("gated_residual_norm: x must be a tensor of at least one dimension")
     shape, cols = x.shape, x.shape[-1]
-    rows = x.numel() // cols if cols else 0
     if x.dtype not in _FLOATS:
         raise ValueError(f"gated_residual_norm: x must be float32 or bfloat16, got {x.dtype}")
     if post not in _NORMS or pre not in ("rms", "layer"):
@@ -2184,8 +2089,8 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
         raise ValueError(f"gated_residual_norm: eps must be positive, got {eps}")
     if not 1 <= cols <= 16384:
         raise ValueError(f"gated_residual_norm: 1 to 16384 columns, got {cols}")
-    cfg = {"post": _NORMS[post], "pre": _NORMS[pre], "gate_mode": 0, "gate_act": _GATE_ACTS[gate_act], "scale_mode": 0,
-           "scale_value": 1.0, "eps": float(eps)}
+    gate_mode = scale_mode = 0
+    scale_value = 1.0
     if h is None:
         if gate is not None or scale is not None or post is not None or post_weight is not None or post_bias is not None:
             raise ValueError("gated_residual_norm: gate, scale and post norm belong to a block's output h")
@@ -2199,7 +2104,6 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
     if y_type not in _FLOATS or (x.dtype == torch.bfloat16 and y_type != torch.bfloat16):
         raise ValueError(f"gated_residual_norm: x {x.dtype} with blocks of {y_type}: float32 or bfloat16 beside float32, "
                          "bfloat16 beside bfloat16")
-    cfg["y_type"] = y_type
     if post is None and (post_weight is not None or post_bias is not None):
         raise ValueError("gated_residual_norm: post_weight / post_bias without a post norm")
 
@@ -2212,30 +2116,25 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
         raise ValueError("gated_residual_norm: a bias with an rms norm, which has none")
     if scale is not None:
         if not isinstance(scale, torch.Tensor):
-            cfg["scale_value"], scale = float(scale), None
+            scale_value, scale = float(scale), None
         elif scale.numel() == 1 and scale.is_floating_point():
-            cfg["scale_mode"], scale = 1, _f32c(scale)
+            scale_mode, scale = 1, _f32c(scale)
         else:
-            cfg["scale_mode"], scale = 2, _param("scale", scale, column)
+            scale_mode, scale = 2, _param("scale", scale, column)
     if gate is not None:
         if gate.shape == shape and gate.dtype == h.dtype:
-            cfg["gate_mode"], gate = 1, _rows_of(gate, cols)
+            gate_mode, gate = 1, _rows_of(gate, cols)
         elif gate.shape == (*shape[:-1], 1) and gate.is_floating_point() and len(shape) > 1:
-            cfg["gate_mode"], gate = 2, _f32c(gate)
+            gate_mode, gate = 2, _f32c(gate)
         elif gate.shape == column and gate.is_floating_point():
-            cfg["gate_mode"], gate = 3, _f32c(gate)
+            gate_mode, gate = 3, _f32c(gate)
         else:
             raise ValueError(f"gated_residual_norm: a gate is {tuple(shape)} of {y_type}, {(*shape[:-1], 1)} or ({cols},), got "
                              f"{gate.dtype} {tuple(gate.shape)}")
     _same_device("gated_residual_norm", x, h, gate, scale, w1, b1, w2, b2)
-    x2 = _rows_of(x, cols)
-    h2 = None if h is None else _rows_of(h, cols)
-    tensors = (x2, h2, gate, scale, w1, b1, w2, b2)
-    track = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-    if track:
-        r, y = GatedResidualNormFn.apply(*tensors, cfg)
-    else:
-        r, y, _ = _residual_norm_fwd(*tensors, cfg, False)
+    r, y = _lib.trunk().residual_norm(_rows_of(x, cols), None if h is None else _rows_of(h, cols), gate, scale, w1, b1, w2, b2,
+                                      _NORMS[post], _NORMS[pre], gate_mode, _GATE_ACTS[gate_act], scale_mode, scale_value,
+                                      float(eps), y_type == torch.bfloat16)
     if x.ndim != 2:
         r, y = None if h is None else r.reshape(shape), y.reshape(shape)
     return x if h is None else r, y
@@ -2264,11 +2163,6 @@ def _check_floats(what, t):
                          f"{f'{t.dtype} {tuple(t.shape)}' if isinstance(t, torch.Tensor) else type(t).__name__}")
 
 
-def _empty_packed(rows, cols, ref):
-    groups = (cols + 63) // 64
-    return ref.new_empty((rows, 64 * groups), dtype=torch.int8), ref.new_empty((rows, groups), dtype=torch.uint8)
-
-
 def pack8(x):
     """The 8-bit checkpoint of a float32 or bfloat16 tensor [..., D] (a Packed8).  Every 64 columns of a row share a step
     2^k, the smallest power of two with max|x| <= 127 * 2^k (k >= -126; k <= 121, where codes saturate); a code is x / 2^k
@@ -2276,11 +2170,11 @@ def pack8(x):
     _check_floats("pack8", x)
     _same_device("pack8", x)
     cols = x.shape[-1]
-    codes, steps = _empty_packed(math.prod(x.shape[:-1]), cols, x)
     if x.numel():
-        t = _rows_of(x.detach(), cols)
-        _call(t.get_device(), _lib.lib().scp_pack8, t.data_ptr(), t.dtype == torch.bfloat16, t.stride(0), t.shape[0], cols,
-              codes.data_ptr(), steps.data_ptr())
+        codes, steps = _lib.trunk().pack8(_rows_of(x.detach(), cols))
+    else:
+        rows, groups = math.prod(x.shape[:-1]), (cols + 63) // 64
+        codes, steps = x.new_empty((rows, 64 * groups), dtype=torch.int8), x.new_empty((rows, groups), dtype=torch.uint8)
     return Packed8(codes, steps, x.shape, x.dtype)
 
 
@@ -2293,49 +2187,13 @@ def unpack8(p, dtype=None):
     if dtype not in _FLOATS:
         raise ValueError(f"unpack8: float32 or bfloat16, got {dtype}")
     _same_device("unpack8", p.codes, p.steps)
-    out = p.codes.new_empty(p.shape, dtype=dtype)
-    if out.numel():
-        _call(out.get_device(), _lib.lib().scp_unpack8, p.codes.data_ptr(), p.steps.data_ptr(), p.codes.shape[0], p.shape[-1],
-              out.data_ptr(), dtype == torch.bfloat16)
-    return out
+    if math.prod(p.shape) == 0:
+        return p.codes.new_empty(p.shape, dtype=dtype)
+    out = _lib.trunk().unpack8(p.codes, p.steps, p.shape[-1], dtype == torch.bfloat16)
+    return out if len(p.shape) == 2 else out.reshape(p.shape)
 
 
 _ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
-
-
-def _act8_fwd(z, kind, slope, keep):
-    rows, cols = z.shape
-    out = z.new_empty((rows, cols))
-    codes, steps = _empty_packed(rows, cols, z) if keep else (None, None)
-    _call(z.get_device(), _lib.lib().scp_act8_fwd, z.data_ptr(), z.dtype == torch.bfloat16, z.stride(0), rows, cols, kind, slope,
-          out.data_ptr(), _lib.ptr(codes), _lib.ptr(steps))
-    return out, codes, steps
-
-
-class Act8Fn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, kind, slope):
-        out, codes, steps = _act8_fwd(z, kind, slope, True)
-        ctx.save_for_backward(codes, steps)
-        ctx.cfg = kind, slope
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        return _act8_bwd_once(ctx, dout) if torch.is_grad_enabled() else _act8_bwd(ctx, dout)
-
-
-def _act8_bwd(ctx, dout):
-    codes, steps = ctx.saved_tensors
-    rows, cols = dout.shape
-    dout = _rows_of(dout, cols)
-    dz = dout.new_empty((rows, cols))
-    _call(dz.get_device(), _lib.lib().scp_act8_bwd, codes.data_ptr(), steps.data_ptr(), rows, cols, *ctx.cfg, dout.data_ptr(),
-          dout.dtype == torch.bfloat16, dout.stride(0), dz.data_ptr())
-    return dz, None, None
-
-
-_act8_bwd_once = torch.autograd.function.once_differentiable(_act8_bwd)      # a second derivative is refused
 
 
 def act8(z, kind="gelu", slope=0.01):
@@ -2348,73 +2206,8 @@ def act8(z, kind="gelu", slope=0.01):
     _same_device("act8", z)
     if z.numel() == 0:
         return z.clone()
-    t = _rows_of(z, z.shape[-1])
-    if torch.is_grad_enabled() and z.requires_grad:
-        out = Act8Fn.apply(t, _ACTS8[kind], float(slope))
-    else:
-        out = _act8_fwd(t, _ACTS8[kind], float(slope), False)[0]
+    out = _lib.trunk().act8(_rows_of(z, z.shape[-1]), _ACTS8[kind], float(slope))
     return out if z.ndim == 2 else out.reshape(z.shape)
-
-
-_LINEAR8_BLOCK = _struct.Struct("11P3l5i4x")      # ScpLinear8
-
-
-def _linear8_run(what, tensors, M, N, K, ldx, lddy, x16, w16, split, ref):
-    """One of the two C entries with its workspace (none where the shape needs none); tensors: the block's ten pointers."""
-    L = _lib.lib()
-    ptrs = [0 if t is None else t.data_ptr() for t in tensors]
-    shape = (M, ldx, lddy, N, K, x16, w16, 3 if split else 1)
-    fwd = what == "fwd"
-    nws = (L.scp_linear8_fwd_ws if fwd else L.scp_linear8_bwd_ws)(_LINEAR8_BLOCK.pack(*ptrs, 0, *shape))
-    if nws < 0:
-        _lib.check(-1, "scp_linear8_" + what)
-    ws = ref.new_empty((nws,), dtype=torch.uint8) if nws else None
-    _call(ref.get_device(), L.scp_linear8_fwd if fwd else L.scp_linear8_bwd,
-          _LINEAR8_BLOCK.pack(*ptrs, ws.data_ptr() if nws else 0, *shape))
-
-
-def _linear8_fwd(x, W, b, split, keep):
-    M, K = x.shape
-    N = W.shape[0]
-    y = x.new_empty((M, N))
-    codes, steps = _empty_packed(M, K, x) if keep else (None, None)
-    if M:
-        _linear8_run("fwd", (x, W, b, y, codes, steps, None, None, None, None), M, N, K, x.stride(0), 0,
-                     x.dtype == torch.bfloat16, W.dtype == torch.bfloat16, split, x)
-    return y, codes, steps
-
-
-class Linear8Fn(torch.autograd.Function):
-    """scp_linear8_fwd / _bwd (csrc/linear8.hip); keeps x as an 8-bit checkpoint, and W."""
-
-    @staticmethod
-    def forward(ctx, x, W, b, split):
-        y, codes, steps = _linear8_fwd(x, W, b, split, ctx.needs_input_grad[1])
-        ctx.save_for_backward(codes, steps, W)
-        ctx.split, ctx.dims = split, x.shape
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        return _linear8_bwd_once(ctx, dy) if torch.is_grad_enabled() else _linear8_bwd(ctx, dy)
-
-
-def _linear8_bwd(ctx, dy):
-    codes, steps, W = ctx.saved_tensors
-    need_x, need_w, need_b, _ = ctx.needs_input_grad
-    M, K = ctx.dims
-    dy = _rows_of(dy, W.shape[0])
-    dx = dy.new_empty((M, K)) if need_x else None
-    dW = torch.empty_like(W) if need_w else None
-    db = dy.new_empty((W.shape[0],), dtype=torch.float32) if need_b else None
-    if M == 0:
-        return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_(), None
-    _linear8_run("bwd", (None, W, None, None, codes, steps, dy, dx, dW, db), M, W.shape[0], K, 0, dy.stride(0),
-                 dy.dtype == torch.bfloat16, W.dtype == torch.bfloat16, ctx.split, dy)
-    return dx, dW, db, None
-
-
-_linear8_bwd_once = torch.autograd.function.once_differentiable(_linear8_bwd)
 
 
 def linear8(x, W, b=None):
@@ -2438,10 +2231,6 @@ def linear8(x, W, b=None):
     x2 = _rows_of(x, K)
     if x2.shape[0] >= 1 << 30:
         raise ValueError(f"linear8: at most 2^30 - 1 rows, got {x2.shape[0]}")
-    W, b = W if W.is_contiguous() else W.contiguous(), None if b is None else _f32c(b)
-    split = x.dtype == torch.float32 and _ns() == 3
-    if torch.is_grad_enabled() and (x.requires_grad or W.requires_grad or (b is not None and b.requires_grad)):
-        y = Linear8Fn.apply(x2, W, b, split)
-    else:
-        y = _linear8_fwd(x2, W, b, split, False)[0]
+    y = _lib.trunk().linear8(x2, W if W.is_contiguous() else W.contiguous(), None if b is None else _f32c(b),
+                             x.dtype == torch.float32 and _ns() == 3)
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], N)
