@@ -8,8 +8,9 @@
 // six column blocks of one long product -- first operand (h h m h m l), second (h m h l m h) -- so the matrix kernels know
 // nothing of them.  v is exact in one term: dW takes three pairs, read out of dy's blocks 0, 2 and 5.
 //
-// Two matrix kernels: the wide one (wgemm.hip, 256 x 256 tiles) where its tiles fill the chip, and the one below (64 x 64 or
-// 128 x 128 tiles, several K-ranges) for the minibatch sizes, where 256 x 256 leaves most CUs idle.
+// Three matrix kernels: the wide one (wgemm.hip, 256 x 256 tiles) where its tiles fill the chip; 128 x 128 tiles below that;
+// 64 x 64 tiles straight from the tensors, without prepared copies, for the minibatch sizes, where a launch counts as much as
+// the product.  A cost model with measured rates chooses (step_us).
 #include <stdlib.h>
 #include "ckpt8.h"
 #include "common.h"
@@ -258,18 +259,26 @@ struct Tile {
   }
 };
 
-template <int TS, int OPA, int OPB, typename CT>
-__global__ __launch_bounds__(256, TS == 64 ? 4 : 2) void lgemm_kernel(LgArgs g) {
-  constexpr int NI = TS / 64, WT = TS / 2, IMG = TS * 128, DEPTH = TS == 64 ? 4 : 2;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  // ids b, b + 8, b + 16 .. share an XCD: give them neighbouring tiles
+// The workgroup's tile and K-range.  Ids b, b + 8, b + 16 .. share an XCD: they get neighbouring tiles, and those in blocks of
+// 8 tile rows walked column by column, so that the tiles at work on an XCD share a few rows and columns.
+__device__ __forceinline__ bool lg_tile(const LgArgs& g, int& tm, int& tn, int& z) {
   const int per_z = g.tiles_m * g.tiles_n, total = per_z * g.nsplit * g.planes, per_xcd = (total + 7) >> 3;
   const int lid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if (lid >= total || (int)(blockIdx.x >> 3) >= per_xcd) return;
-  // and those in blocks of 8 tile rows, walked column by column: the tiles at work on an XCD share a few rows and columns
-  const int z = lid / per_z, t = lid - z * per_z, grp = t / (8 * g.tiles_n), in = t - grp * 8 * g.tiles_n;
-  const int gh = min(8, g.tiles_m - 8 * grp), tn = in / gh, tm = 8 * grp + in - tn * gh;
+  if (lid >= total || (int)(blockIdx.x >> 3) >= per_xcd) return false;
+  z = lid / per_z;
+  const int t = lid - z * per_z, grp = t / (8 * g.tiles_n), in = t - grp * 8 * g.tiles_n, gh = min(8, g.tiles_m - 8 * grp);
+  tn = in / gh;
+  tm = 8 * grp + in - tn * gh;
+  return true;
+}
+
+template <int OPA, int OPB, typename CT>
+__global__ __launch_bounds__(256, 2) void lgemm_kernel(LgArgs g) {
+  constexpr int TS = 128, NI = TS / 64, WT = TS / 2, IMG = TS * 128, DEPTH = 2;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  int tm, tn, z;
+  if (!lg_tile(g, tm, tn, z)) return;
   const int m0 = tm * TS, n0 = tn * TS, plane = z / g.nsplit;
   const int kt0 = (z % g.nsplit) * g.per_split, kt1 = min((g.K + 63) / 64, kt0 + g.per_split);
 
@@ -339,6 +348,188 @@ __global__ __launch_bounds__(256, TS == 64 ? 4 : 2) void lgemm_kernel(LgArgs g) 
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// 64 x 64 tiles straight from the tensors
+// ---------------------------------------------------------------------------------------------------------------------
+// The same product on 64 x 64 tiles for what one call of minibatch size is made of.  The operands are read as they are --
+// fp32 or bf16, any row stride, any alignment, any length -- and rounded (NP 1) or taken apart into three terms (NP 3) on the
+// way into LDS: no prepared copies, a third of the bytes of the six-block layout through the caches, and a fragment that is
+// in LDS serves every pair it belongs to.  Accesses are vectors of 8 elements without a test.  The step that K ends in is
+// made apart, after the others, where a K that is no multiple of 64 or the last columns of a col operand need care: a vector
+// that would pass the end goes element by element.  (In earlier steps a vector may run over the end of a k row, into the
+// next one: rows are 8 elements at least and no closer than their length, checked on the host.  Those columns are not stored.)
+template <typename T, int NP, bool COL>
+struct DTile {
+  typedef typename Vec8<T>::v V;
+  typedef typename Vec8<T>::vu VU;
+  struct Reg { V v[2]; };
+  const T* base;
+  long ld;
+  int K, n;                 // n: columns from the tile's origin on (col operands)
+  int start;                // first column or k of the lane's chunks
+  unsigned voff[2];
+  int lds[2];
+
+  __device__ __forceinline__ void init(const void* p, const uint8_t*, long ld_, int origin, int extent, int K_) {
+    ld = ld_;
+    K = K_;
+    n = extent - origin;
+    base = (const T*)p + (COL ? (long)origin : (long)origin * ld);
+    const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
+    start = COL && 8 * c >= n ? 0 : 8 * c;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int q = r + 32 * i;
+      voff[i] = (unsigned)((COL ? q : min(q, n - 1)) * ld) + start;      // rows behind the last: the last again
+      lds[i] = COL ? lg_col_off<64>(q, 8 * c) : lg_row_off(q, c);
+    }
+  }
+  __device__ __forceinline__ bool care() const { return (K & 63) || (COL && n < 64); }
+  __device__ __forceinline__ void load(Reg& r, int kt, bool live) const {
+    if (!live) return;        // uniform; what is in r then is stored, but never read
+    const T* p = base + (COL ? (long)kt * 64 * ld : (long)kt * 64);
+#pragma unroll
+    for (int i = 0; i < 2; i++) r.v[i] = *(const VU*)(p + voff[i]);
+  }
+  __device__ __forceinline__ void load_end(Reg& r, int kt) const {
+    const int k0 = kt * 64;
+    const T* p = base + (COL ? k0 * ld : (long)k0);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int have = COL ? (k0 + (int)(threadIdx.x >> 3) + 32 * i < K ? n - start : 0) : K - k0 - start;
+      V v;
+      if (have >= 8) {
+        v = *(const VU*)(p + voff[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = j < have ? p[voff[i] + j] : (T)0.f;
+      }
+      r.v[i] = v;
+    }
+  }
+  __device__ __forceinline__ void store(const Reg& r, unsigned char* img) const {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      if constexpr (sizeof(T) == 2) {
+        *(V*)(img + lds[i]) = r.v[i];
+      } else {
+        bf16x8 t[NP];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          __bf16 s[3];
+          bf16_split<NP>(r.v[i][j], s);
+#pragma unroll
+          for (int q = 0; q < NP; q++) t[q][j] = s[q];
+        }
+#pragma unroll
+        for (int q = 0; q < NP; q++) *(bf16x8*)(img + q * 8192 + lds[i]) = t[q];
+      }
+    }
+  }
+};
+
+// operand B: a DTile or an 8-bit checkpoint
+template <typename TB, int PB, int OPB> struct BTile { typedef DTile<TB, PB, OPB == OP_COL> t; };
+template <typename TB, int PB> struct BTile<TB, PB, OP_Q8> { typedef Tile<64, OP_Q8> t; };
+
+template <typename TA, int PA, bool ACOL, typename TB, int PB, int OPB, typename CT>
+__global__ __launch_bounds__(256, PA + PB > 2 ? 3 : 4) void dgemm_kernel(LgArgs g) {
+  typedef DTile<TA, PA, ACOL> TileA;
+  typedef typename BTile<TB, PB, OPB>::t TileB;
+  // one term each: two LDS stages, one barrier a step; three terms: one stage, so that three workgroups share a CU
+  constexpr int STAGES = PA + PB == 2 ? 2 : 1, STAGE = (PA + PB) * 8192;
+  constexpr int DEPTH = PA + PB > 2 ? 2 : sizeof(TA) + (OPB == OP_Q8 ? 1 : sizeof(TB)) <= 4 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[STAGES * STAGE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  int tm, tn, z;
+  if (!lg_tile(g, tm, tn, z)) return;
+  const int m0 = tm * 64, n0 = tn * 64;
+  const int nk = (g.K + 63) / 64, kt0 = z * g.per_split, kt1 = min(nk, kt0 + g.per_split);
+
+  TileA ta;
+  TileB tb;
+  ta.init(g.A, nullptr, g.lda, m0, g.M, g.K);
+  tb.init(g.B, g.steps, g.ldb, n0, g.N, g.K);
+  bool care = ta.care();
+  if constexpr (OPB != OP_Q8) care = care || tb.care();      // (a checkpoint's rows are padded: its loads check themselves)
+  const int ktv = kt1 - (care && kt1 == nk);                 // steps [kt0, ktv) in vectors
+  // the pairs below the leading one are summed apart: their sum keeps its low bits
+  f32x16 acc[PA == 3 ? 2 : 1];
+#pragma unroll
+  for (auto& q : acc)
+#pragma unroll
+    for (int e = 0; e < 16; e++) q[e] = 0.f;
+  auto multiply = [&](const unsigned char* ia) {
+    const unsigned char* ib = ia + PA * 8192;
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      bf16x8 fa[PA], fb[PB];
+#pragma unroll
+      for (int q = 0; q < PA; q++) fa[q] = lg_frag<64, ACOL>(ia + q * 8192, wm * 32, s, lane);
+#pragma unroll
+      for (int q = 0; q < PB; q++) fb[q] = lg_frag<64, OPB != OP_ROW>(ib + q * 8192, wn * 32, s, lane);
+      if constexpr (PA == 3) {
+#pragma unroll
+        for (int w = 2; w > 0; w--)          // pairs of weight 2^-16, then 2^-8
+#pragma unroll
+          for (int q = 0; q < PB; q++)
+            if (w - q >= 0 && w - q < PA) acc[1] = mfma32(fa[w - q], fb[q], acc[1]);
+      }
+      acc[0] = mfma32(fa[0], fb[0], acc[0]);
+    }
+  };
+
+  if (kt0 < ktv) {
+    typename TileA::Reg ra[DEPTH];
+    typename TileB::Reg rb[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) {
+      ta.load(ra[d], kt0 + d, kt0 + d < ktv);
+      tb.load(rb[d], kt0 + d, kt0 + d < ktv);
+    }
+    ta.store(ra[0], smem);
+    tb.store(rb[0], smem + PA * 8192);
+    __syncthreads();
+    for (int kt = kt0; kt < ktv; kt += DEPTH) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; d++) {
+        if (kt + d < ktv) {            // uniform
+          ta.load(ra[d], kt + d + DEPTH, kt + d + DEPTH < ktv);
+          tb.load(rb[d], kt + d + DEPTH, kt + d + DEPTH < ktv);
+          multiply(smem + (d % STAGES) * STAGE);
+          if constexpr (STAGES == 1) __syncthreads();
+          unsigned char* na = smem + ((d + 1) % STAGES) * STAGE;
+          ta.store(ra[(d + 1) % DEPTH], na);
+          tb.store(rb[(d + 1) % DEPTH], na + PA * 8192);
+          __syncthreads();
+        }
+      }
+    }
+  }
+  if (ktv < kt1) {
+    typename TileA::Reg ra;
+    typename TileB::Reg rb;
+    ta.load_end(ra, ktv);
+    if constexpr (OPB == OP_Q8) tb.load(rb, ktv, true);
+    else tb.load_end(rb, ktv);
+    ta.store(ra, smem);
+    tb.store(rb, smem + PA * 8192);
+    __syncthreads();
+    multiply(smem);
+  }
+
+  CT* C = (CT*)g.C + (long)z * g.M * g.ldc;
+  const int n = n0 + wn * 32 + (lane & 31);
+  if (n >= g.N) return;
+  const float bn = g.bias ? g.bias[n] : 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; e++) {
+    const int m = m0 + wm * 32 + acc_row(e, lane);
+    const float v = PA == 3 ? acc[0][e] + acc[PA == 3 ? 1 : 0][e] : acc[0][e];
+    if (m < g.M) C[(long)m * g.ldc + n] = (CT)(v + bn);
+  }
+}
+
 // C = sum of n slabs in slab order, + bias.  Slabs and C are [M][N], contiguous: 4 elements a thread.
 template <typename CT>
 __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ slabs, int n, long MN, int N,
@@ -372,57 +563,82 @@ long align256(long b) { return (b + 255) & ~255L; }
 int up8(int n) { return (n + 7) & ~7; }
 
 struct Gemm {
-  int ts;              // 64 or 128: lgemm tiles; 256: the wide kernel
+  int ts;              // 64: dgemm straight from the tensors; 128: lgemm, 256: the wide kernel, on prepared operands
   int nsplit, slabs;   // K-ranges; slabs of the result in the workspace (0: written directly)
   long ws;             // workspace bytes
+  double us;           // estimate
 };
 
-// Tile and K-ranges of one product of `planes` column blocks: the cheapest by a model in microseconds.  A step of 64 k with
-// w workgroups per CU took, measured over products from 300^3 to 16384 x 4096^2: 0.25 + 0.2 w at 64 x 64, 1.15 (w = 1) or
-// 0.70 w at 128 x 128, 2.3 w at 256 x 256; slabs are written and read at 7.5 TB/s, and a launch costs 3.5 us.
-Gemm pick(long M, int N, long K, int planes, bool wide_ok, int wide_ns, long wide_ws) {
-  Gemm best = {256, 1, 0, wide_ws};
-  const long nk = (K + 63) / 64;
+// Costs in microseconds of a step of 64 k with w workgroups per CU, measured over products from 300^3 to 16384 x 4096^2 (the
+// product's own time only; a launch 3.5, slabs written and read at 7.5 TB/s, prepared operands at 5).
+double step_us(int ts, int pairs, double w) {
+  if (ts == 64) return pairs == 1 ? 0.25 + 0.2 * w : pairs == 3 ? 0.5 + 0.48 * w : 0.6 + 0.85 * w;
+  if (ts == 128) return w == 1 ? 1.15 : 0.7 * w;
+  return 2.3 * w;
+}
+const double LAUNCH_US = 3.5;
+
+void consider(Gemm& best, int ts, int pairs, long M, int N, long K, int planes) {
+  const long nk = (K + 63) / 64, tiles = ((M + ts - 1) / ts) * ((N + ts - 1) / ts) * planes;
   const double mn = (double)M * N;
-  double best_us = 1e30;
-  if (wide_ok) {
-    const long tiles = ((M + 255) / 256) * ((N + 255) / 256) * wide_ns;
-    best_us = planes * ((tiles + 255) / 256 * 2.3 * ((nk + wide_ns - 1) / wide_ns) + 3.5);
-    if (wide_ns > 1) best_us += planes * (mn * 4 * (2 * wide_ns + 1) / 7.5e6 + 3.5);
-    if (planes > 1) best_us += mn * 4 * (2 * planes + 1) / 7.5e6 + 3.5;
-  }
-  for (int ts = 64; ts <= 128; ts += 64) {
-    const long tiles = ((M + ts - 1) / ts) * ((N + ts - 1) / ts) * planes;
-    if (tiles >= 1L << 24) continue;
-    for (int ns = 1; ns <= 64; ns *= 2) {
-      if (ns > 1 && nk / ns < 4) break;
-      const double w = (double)((tiles * ns + 255) / 256);
-      double us = 3.5 + (nk + ns - 1) / ns * (ts == 64 ? 0.25 + 0.2 * w : w == 1 ? 1.15 : 0.7 * w);
-      if (ns * planes > 1) us += mn * 4 * (2 * ns * planes + 1) / 7.5e6 + 3.5;
-      if (us < best_us) {
-        best_us = us;
-        best.ts = ts;
-        best.nsplit = ns;
-        best.slabs = ns * planes > 1 ? ns * planes : 0;
-        best.ws = (long)best.slabs * M * N * 4;
-      }
+  if (tiles >= 1L << 24) return;
+  for (int ns = 1; ns <= 64; ns *= 2) {
+    if (ns > 1 && nk / ns < 4) break;
+    double us = LAUNCH_US + (nk + ns - 1) / ns * step_us(ts, pairs, (double)((tiles * ns + 255) / 256));
+    if (ns * planes > 1) us += mn * 4 * (2 * ns * planes + 1) / 7.5e6 + LAUNCH_US;
+    if (us >= best.us) continue;
+    best.ts = ts;
+    best.nsplit = ns;
+    best.slabs = ns * planes > 1 ? ns * planes : 0;
+    best.ws = (long)best.slabs * M * N * 4;
+    best.us = us;
+#ifdef LIN8_TUNE
+    if (const char* e = getenv("LIN8_NS")) {
+      best.nsplit = atoi(e);
+      best.slabs = best.nsplit * planes > 1 ? best.nsplit * planes : 0;
+      best.ws = (long)best.slabs * M * N * 4;
+      return;
     }
+#endif
+  }
+}
+
+// straight from the tensors; pairs: term pairs per product
+Gemm pick_direct(long M, int N, long K, int pairs) {
+  Gemm best = {0, 1, 0, 0, 1e30};
+  consider(best, 64, pairs, M, N, K, 1);
+  return best;
+}
+
+// on prepared operands, of which `planes` column blocks are summed up apart
+Gemm pick_blocks(long M, int N, long K, int planes, bool wide_ok, long wide_ws) {
+  Gemm best = {0, 1, 0, 0, 1e30};
+  if (wide_ok) {
+    const long nk = (K + 63) / 64;
+    const int ns = scp_gemm_bf16_nsplit((int)M, N, (int)K);
+    const double mn = (double)M * N, w = (double)((((M + 255) / 256) * ((N + 255) / 256) * ns + 255) / 256);
+    double us = planes * (LAUNCH_US + step_us(256, 1, w) * ((nk + ns - 1) / ns));
+    if (ns > 1) us += planes * (mn * 4 * (2 * ns + 1) / 7.5e6 + LAUNCH_US);
+    if (planes > 1) us += mn * 4 * (2 * planes + 1) / 7.5e6 + LAUNCH_US;
+    best = {256, 1, 0, wide_ws, us};
   }
 #ifdef LIN8_TUNE
   if (const char* e = getenv("LIN8_TS")) {
-    best.ts = atoi(e);
-    best.nsplit = best.ts == 256 ? 1 : atoi(getenv("LIN8_NS"));
-    best.slabs = best.ts != 256 && best.nsplit * planes > 1 ? best.nsplit * planes : 0;
-    best.ws = best.ts == 256 ? wide_ws : (long)best.slabs * M * N * 4;
+    if (atoi(e) == 256) return best;
+    best.us = 1e30;
   }
 #endif
+  consider(best, 128, 1, M, N, K, planes);
   return best;
 }
+
+double prep_us(double elements, int in_bytes, int blocks) { return LAUNCH_US + elements * (in_bytes + 2 * blocks) / 5e6; }
 
 struct Plan {
   int np;                    // column blocks of an fp32 operand: 6 (ns 3), else 1
   int Kp, Np;
-  bool x_direct, w_direct, dy_direct;
+  bool x_direct, w_direct, dy_direct;          // usable as prepared operands as they are
+  bool prep_x, prep_w, prep_dy;                // copies to make
   long a_off, b_off, part_off, g_off, total;   // workspace: prepared operands, column sums, slabs
   int parts;
   Gemm y, dx, dw;
@@ -440,27 +656,44 @@ void common_plan(const ScpLinear8& a, Plan& p) {
   p.w_direct = a.w_bf16 && a.K % 8 == 0 && ((uintptr_t)a.W & 15) == 0;
 }
 
-int wide_splits(long M, int N, long K) { return scp_gemm_bf16_nsplit((int)M, N, (int)K); }
-
-long wide_ws_rows(const Plan& p, long M, int N, long K, long lda) {
+long wide_ws_rows(long M, int N, long K, long lda) {
   const long piece = WIDE_BYTES / (2 * lda);
   const long a = scp_gemm_bf16_ws_floats((int)(M < piece ? M : piece), N, (int)K, N);
   const long b = M > piece ? scp_gemm_bf16_ws_floats((int)(M % piece), N, (int)K, N) : 0;    // the last piece may split K
   return (a > b ? a : b) * 4;
 }
 
+bool tune_only(const Gemm& g) {
+#ifdef LIN8_TUNE
+  if (const char* e = getenv("LIN8_TS")) return g.ts != atoi(e);
+#endif
+  return g.ts == 0;
+}
+
+// dgemm forms the offsets inside a tile in 32 bits; its col operands (W for dx, dy for dW) also have rows of 8 elements at
+// least, no closer than their length
+bool direct_rows_ok(long ld) { return ld < 1L << 25; }
+
 Plan plan_fwd(const ScpLinear8& a) {
   Plan p = {};
   common_plan(a, p);
   p.x_direct = a.x_bf16 && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx >= a.K && ((uintptr_t)a.x & 15) == 0;
-  const long KK = (long)p.np * p.Kp;
+  const int xb = a.x_bf16 ? 2 : 4, wb = a.w_bf16 ? 2 : 4;
+  const long KK = p.np == 1 ? a.K : (long)p.np * p.Kp, ld = (long)p.np * p.Kp;
+  const bool ok = ((long)a.N + 192) * ld * 2 < WIDE_BYTES;
+  Gemm blocks = pick_blocks(a.M, a.N, KK, 1, ok, ok ? wide_ws_rows(a.M, a.N, KK, p.x_direct ? a.ldx : ld) : 0);
+  if (!p.x_direct) blocks.us += prep_us((double)a.M * a.K, xb, p.np) - LAUNCH_US;    // else packing is a launch of its own
+  if (!p.w_direct) blocks.us += prep_us((double)a.N * a.K, wb, p.np);
+  Gemm direct = pick_direct(a.M, a.N, a.K, p.np);
+  if (!direct_rows_ok(a.ldx)) direct.us = 1e30;
+  p.y = (direct.us < blocks.us || tune_only(blocks)) && !tune_only(direct) ? direct : blocks;
+  p.prep_x = p.y.ts != 64 && !p.x_direct;
+  p.prep_w = p.y.ts != 64 && !p.w_direct;
   long o = 0;
   p.a_off = o;
-  if (!p.x_direct) o += align256(a.M * KK * 2);
+  if (p.prep_x) o += align256(a.M * ld * 2);
   p.b_off = o;
-  if (!p.w_direct) o += align256((long)a.N * KK * 2);
-  const bool ok = ((long)a.N + 192) * KK * 2 < WIDE_BYTES;
-  p.y = pick(a.M, a.N, KK, 1, ok, wide_splits(a.M, a.N, KK), ok ? wide_ws_rows(p, a.M, a.N, KK, p.x_direct ? a.ldx : KK) : 0);
+  if (p.prep_w) o += align256((long)a.N * ld * 2);
   p.g_off = o;
   p.total = o + align256(p.y.ws);
   return p;
@@ -470,33 +703,43 @@ Plan plan_bwd(const ScpLinear8& a) {
   Plan p = {};
   common_plan(a, p);
   p.dy_direct = a.x_bf16 && a.N % 8 == 0 && a.lddy == a.N && ((uintptr_t)a.dy & 15) == 0;
-  const long NN = (long)p.np * p.Np;
-  const bool need_dy = a.dx || a.dW;
+  const int xb = a.x_bf16 ? 2 : 4, wb = a.w_bf16 ? 2 : 4, planes = p.np == 6 ? 3 : 1;
+  const long ld = (long)p.np * p.Np, K2 = p.np == 1 ? a.N : ld, lda = p.dy_direct ? a.N : ld;
+  const double dy_us = p.dy_direct ? 0 : prep_us((double)a.M * a.N, xb, p.np) - LAUNCH_US;   // else the column sums are a launch of their own
+  // Each product straight from the tensors or on prepared operands: the cheapest combination, dy being prepared once for both.
+  // Chosen as if all gradients were asked for, so that none depends on the others being wanted.
+  const bool ok = (K2 + 192) * p.Kp * 2 < WIDE_BYTES;
+  Gemm xb_ = pick_blocks(a.M, a.K, K2, 1, ok, ok ? wide_ws_rows(a.M, a.K, K2, lda) : 0);
+  if (!p.w_direct) xb_.us += prep_us((double)a.N * a.K, wb, p.np);
+  Gemm xd = pick_direct(a.M, a.K, a.N, p.np);
+  if (!direct_rows_ok(a.lddy) || a.K < 8) xd.us = 1e30;
+  // the wide form of dW runs once per plane, each into a slab of its own
+  const long ld8 = (a.K + 63) / 64 * 64L, wide_ws = scp_gemm_q8_ws_floats(a.N, a.K, (int)a.M, lda > ld8 ? lda : ld8, a.K) * 4;
+  const Gemm wb_ = pick_blocks(a.N, a.K, a.M, planes, true, align256(wide_ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
+  Gemm wd = pick_direct(a.N, a.K, a.M, planes);
+  if (!direct_rows_ok(a.lddy) || a.lddy < a.N || a.N < 8) wd.us = 1e30;
+  double best = 1e300;
+  for (int c = 0; c < 4; c++) {
+    const Gemm &x = c & 1 ? xb_ : xd, &w = c & 2 ? wb_ : wd;
+    const double us = x.us + w.us + (c ? dy_us : 0);
+    if (us >= best || tune_only(x) || tune_only(w)) continue;
+    best = us;
+    p.dx = x;
+    p.dw = w;
+  }
+  p.prep_w = a.dx && p.dx.ts != 64 && !p.w_direct;
+  p.prep_dy = ((a.dx && p.dx.ts != 64) || (a.dW && p.dw.ts != 64)) && !p.dy_direct;
   long o = 0;
   p.a_off = o;
-  if (need_dy && !p.dy_direct) o += align256(a.M * NN * 2);
+  if (p.prep_dy) o += align256(a.M * ld * 2);
   p.b_off = o;
-  if (a.dx && !p.w_direct) o += align256((p.np == 1 ? (long)a.N : NN) * p.Kp * 2);
+  if (p.prep_w) o += align256((p.np == 1 ? (long)a.N : ld) * p.Kp * 2);
   p.part_off = o;
   p.parts = colsum_parts(a.M, a.N);
   if (a.db) o += align256((long)p.parts * a.N * 4);
   p.g_off = o;
-  long g = 0;
-  if (a.dx) {
-    const long K2 = p.np == 1 ? a.N : NN;
-    const bool ok = (K2 + 192) * p.Kp * 2 < WIDE_BYTES;
-    p.dx = pick(a.M, a.K, K2, 1, ok, wide_splits(a.M, a.K, K2), ok ? wide_ws_rows(p, a.M, a.K, K2, p.dy_direct ? a.N : NN) : 0);
-    g = p.dx.ws;
-  }
-  if (a.dW) {
-    const int planes = p.np == 6 ? 3 : 1;
-    const long ld8 = (a.K + 63) / 64 * 64L, lda = p.dy_direct ? a.N : NN;
-    // the wide form runs once per plane, each into a slab of its own
-    const long ws = scp_gemm_q8_ws_floats(a.N, a.K, (int)a.M, lda > ld8 ? lda : ld8, a.K) * 4;
-    p.dw = pick(a.N, a.K, a.M, planes, true, wide_splits(a.N, a.K, a.M), align256(ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
-    if (p.dw.ws > g) g = p.dw.ws;
-  }
-  p.total = p.g_off + align256(g);
+  const long gx = a.dx ? p.dx.ws : 0, gw = a.dW ? p.dw.ws : 0;
+  p.total = o + align256(gx > gw ? gx : gw);
   return p;
 }
 
@@ -522,20 +765,9 @@ int prep_w(const ScpLinear8& a, const Plan& p, bool rows_below, __bf16* dst, hip
   return prep<float, LAY_COLS_B, false>(a.W, a.K, a.N, a.K, 0, dst, p.Kp, nullptr, nullptr, st);
 }
 
-template <int TS, int OPA, int OPB, typename CT>
-int launch_lg(const LgArgs& g, hipStream_t st) {
-  constexpr size_t smem = 4 * TS * 128;
-  static uint64_t done = 0;
-  if (int rc = scp_set_smem((const void*)lgemm_kernel<TS, OPA, OPB, CT>, smem, &done)) return rc;
-  const long total = (long)g.tiles_m * g.tiles_n * g.nsplit * g.planes;
-  hipLaunchKernelGGL((lgemm_kernel<TS, OPA, OPB, CT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), smem, st, g);
-  SCP_LAUNCH_CHECK();
-  return SCP_OK;
-}
-
-// a product on the smaller tiles, C contiguous [M][N]
-template <int OPA, int OPB>
-int small_gemm(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws, hipStream_t st) {
+// tiles, K-ranges and the sum of the slabs around one of the two kernels; C contiguous [M][N]
+template <typename Launch>
+int tiled(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws, hipStream_t st, Launch launch) {
   void* C = g.C;
   g.tiles_m = (g.M + q.ts - 1) / q.ts;
   g.tiles_n = (g.N + q.ts - 1) / q.ts;
@@ -546,38 +778,69 @@ int small_gemm(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws
   const int slabs = g.nsplit * g.planes;
   if (slabs > 1) g.C = ws;
   else g.bias = bias;
-  const bool b16 = slabs == 1 && c_bf16;
-  int rc = q.ts == 64 ? (b16 ? launch_lg<64, OPA, OPB, __bf16>(g, st) : launch_lg<64, OPA, OPB, float>(g, st))
-                      : (b16 ? launch_lg<128, OPA, OPB, __bf16>(g, st) : launch_lg<128, OPA, OPB, float>(g, st));
-  if (rc || slabs == 1) return rc;
+  const dim3 grid((unsigned)(((long)g.tiles_m * g.tiles_n * slabs + 7) / 8 * 8));
+  if (int rc = launch(g, grid, slabs == 1 && c_bf16)) return rc;
+  if (slabs == 1) return SCP_OK;
   const long MN = (long)g.M * g.N;
-  const dim3 grid((unsigned)((MN + 1023) / 1024));
-  if (c_bf16) hipLaunchKernelGGL((lin_sum_kernel<__bf16>), grid, dim3(256), 0, st, ws, slabs, MN, g.N, bias, (__bf16*)C);
-  else hipLaunchKernelGGL((lin_sum_kernel<float>), grid, dim3(256), 0, st, ws, slabs, MN, g.N, bias, (float*)C);
+  const dim3 sum((unsigned)((MN + 1023) / 1024));
+  if (c_bf16) hipLaunchKernelGGL((lin_sum_kernel<__bf16>), sum, dim3(256), 0, st, ws, slabs, MN, g.N, bias, (__bf16*)C);
+  else hipLaunchKernelGGL((lin_sum_kernel<float>), sum, dim3(256), 0, st, ws, slabs, MN, g.N, bias, (float*)C);
   SCP_LAUNCH_CHECK();
   return SCP_OK;
 }
 
-// out[M][N] = A B^T (b_col 0) or A B (b_col 1), + bias.  The wide kernel addresses its operands with 31 bits: a longer batch
-// runs in pieces.
+template <int OPA, int OPB, typename CT>
+int launch_lg(const LgArgs& g, dim3 grid, hipStream_t st) {
+  constexpr size_t smem = 4 * 128 * 128;
+  static uint64_t done = 0;
+  if (int rc = scp_set_smem((const void*)lgemm_kernel<OPA, OPB, CT>, smem, &done)) return rc;
+  hipLaunchKernelGGL((lgemm_kernel<OPA, OPB, CT>), grid, dim3(256), smem, st, g);
+  SCP_LAUNCH_CHECK();
+  return SCP_OK;
+}
+template <int OPA, int OPB>
+int block_gemm(const Gemm& q, const LgArgs& g, int c_bf16, const float* bias, float* ws, hipStream_t st) {
+  return tiled(q, g, c_bf16, bias, ws, st, [st](const LgArgs& a, dim3 grid, bool b16) {
+    return b16 ? launch_lg<OPA, OPB, __bf16>(a, grid, st) : launch_lg<OPA, OPB, float>(a, grid, st);
+  });
+}
+
+// terms of a product straight from the tensors: x (or dy) of TA, W of TB or x's checkpoint
+template <typename TA, int PA, bool ACOL, typename TB, int PB, int OPB>
+int direct_gemm(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws, hipStream_t st) {
+  g.planes = 1;
+  return tiled(q, g, c_bf16, bias, ws, st, [st](const LgArgs& a, dim3 grid, bool b16) -> int {
+    if (b16) hipLaunchKernelGGL((dgemm_kernel<TA, PA, ACOL, TB, PB, OPB, __bf16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((dgemm_kernel<TA, PA, ACOL, TB, PB, OPB, float>), grid, dim3(256), 0, st, a);
+    SCP_LAUNCH_CHECK();
+    return SCP_OK;
+  });
+}
+template <int OPB>
+int direct_rows(const ScpLinear8& a, const Plan& p, const Gemm& q, const LgArgs& g, const float* bias, float* ws, hipStream_t st) {
+  if (a.x_bf16 && a.w_bf16) return direct_gemm<__bf16, 1, false, __bf16, 1, OPB>(q, g, 1, bias, ws, st);
+  if (a.x_bf16) return direct_gemm<__bf16, 1, false, float, 1, OPB>(q, g, 1, bias, ws, st);
+  if (p.np == 1) return direct_gemm<float, 1, false, float, 1, OPB>(q, g, 0, bias, ws, st);
+  return direct_gemm<float, 3, false, float, 3, OPB>(q, g, 0, bias, ws, st);
+}
+
+// out[M][N] = A B^T (b_col 0) or A B (b_col 1), + bias, on prepared operands.  The wide kernel addresses its operands with 31
+// bits: a longer batch runs in pieces.
 int rows_product(const Gemm& q, int b_col, long M, int N, long K, const __bf16* A, long lda, const __bf16* B, long ldb, void* C,
                  int c_bf16, const float* bias, float* ws, hipStream_t st) {
-  const long piece = q.ts == 256 ? WIDE_BYTES / (2 * lda) : 1L << 30;
+  if (q.ts == 128) {
+    LgArgs g = {};
+    g.A = A; g.B = B; g.C = C;
+    g.lda = lda; g.ldb = ldb;
+    g.M = (int)M; g.N = N; g.K = (int)K;
+    g.planes = 1;
+    return b_col ? block_gemm<OP_ROW, OP_COL>(q, g, c_bf16, bias, ws, st) : block_gemm<OP_ROW, OP_ROW>(q, g, c_bf16, bias, ws, st);
+  }
+  const long piece = WIDE_BYTES / (2 * lda);
   for (long r = 0; r < M; r += piece) {
     const int m = (int)(M - r < piece ? M - r : piece);
     void* c = c_bf16 ? (void*)((__bf16*)C + r * N) : (void*)((float*)C + r * N);
-    int rc;
-    if (q.ts == 256) {
-      rc = scp_gemm_rows(b_col, m, N, (int)K, A + r * lda, lda, B, ldb, c, c_bf16, N, bias, ws, st);
-    } else {
-      LgArgs g = {};
-      g.A = A + r * lda; g.B = B; g.C = c;
-      g.lda = lda; g.ldb = ldb;
-      g.M = m; g.N = N; g.K = (int)K;
-      g.planes = 1;
-      rc = b_col ? small_gemm<OP_ROW, OP_COL>(q, g, c_bf16, bias, ws, st) : small_gemm<OP_ROW, OP_ROW>(q, g, c_bf16, bias, ws, st);
-    }
-    if (rc) return rc;
+    if (int rc = scp_gemm_rows(b_col, m, N, (int)K, A + r * lda, lda, B, ldb, c, c_bf16, N, bias, ws, st)) return rc;
   }
   return SCP_OK;
 }
@@ -604,28 +867,36 @@ int dy_pass(const ScpLinear8& a, const Plan& p, bool write, hipStream_t st) {
   return SCP_OK;
 }
 
-// dW = dy^T v; A: dy's blocks
+// dW = dy^T v; A: dy's blocks (unused straight from the tensors)
 int weight_product(const ScpLinear8& a, const Plan& p, const __bf16* A, long lda, float* ws, hipStream_t st) {
-  const int planes = p.np == 6 ? 3 : 1;
-  const int off[3] = {0, 2 * p.Np, 5 * p.Np};
-  if (p.dw.ts == 256) {
-    if (planes == 1) return scp_gemm_q8(a.N, a.K, (int)a.M, A, lda, a.codes, a.steps, a.dW, a.w_bf16, a.K, ws, st);
-    const long NK = (long)a.N * a.K;
-    float* slabs = ws + (p.dw.ws - 3 * NK * 4) / 4;
-    for (int i = 0; i < 3; i++)
-      if (int rc = scp_gemm_q8(a.N, a.K, (int)a.M, A + off[i], lda, a.codes, a.steps, slabs + i * NK, 0, a.K, ws, st)) return rc;
-    hipLaunchKernelGGL((lin_sum_kernel<float>), dim3((unsigned)((NK + 1023) / 1024)), dim3(256), 0, st, slabs, 3, NK, a.K, nullptr,
-                       (float*)a.dW);
-    SCP_LAUNCH_CHECK();
-    return SCP_OK;
-  }
   LgArgs g = {};
-  g.A = A; g.B = a.codes; g.steps = a.steps; g.C = a.dW;
-  g.lda = lda; g.ldb = (a.K + 63) / 64 * 64;
+  g.B = a.codes; g.steps = a.steps; g.C = a.dW;
+  g.ldb = (a.K + 63) / 64 * 64;
   g.M = a.N; g.N = a.K; g.K = (int)a.M;
-  g.planes = planes;
-  for (int i = 0; i < 3; i++) g.plane_off[i] = off[i];
-  return small_gemm<OP_COL, OP_Q8>(p.dw, g, a.w_bf16, nullptr, ws, st);
+  if (p.dw.ts == 64) {
+    g.A = (const __bf16*)a.dy;
+    g.lda = a.lddy;
+    if (a.x_bf16) return direct_gemm<__bf16, 1, true, __bf16, 1, OP_Q8>(p.dw, g, a.w_bf16, nullptr, ws, st);
+    if (p.np == 1) return direct_gemm<float, 1, true, __bf16, 1, OP_Q8>(p.dw, g, 0, nullptr, ws, st);
+    return direct_gemm<float, 3, true, __bf16, 1, OP_Q8>(p.dw, g, 0, nullptr, ws, st);
+  }
+  const int off[3] = {0, 2 * p.Np, 5 * p.Np};
+  g.planes = p.np == 6 ? 3 : 1;
+  if (p.dw.ts == 128) {
+    g.A = A;
+    g.lda = lda;
+    for (int i = 0; i < 3; i++) g.plane_off[i] = off[i];
+    return block_gemm<OP_COL, OP_Q8>(p.dw, g, a.w_bf16, nullptr, ws, st);
+  }
+  if (g.planes == 1) return scp_gemm_q8(a.N, a.K, (int)a.M, A, lda, a.codes, a.steps, a.dW, a.w_bf16, a.K, ws, st);
+  const long NK = (long)a.N * a.K;
+  float* slabs = ws + (p.dw.ws - 3 * NK * 4) / 4;
+  for (int i = 0; i < 3; i++)
+    if (int rc = scp_gemm_q8(a.N, a.K, (int)a.M, A + off[i], lda, a.codes, a.steps, slabs + i * NK, 0, a.K, ws, st)) return rc;
+  hipLaunchKernelGGL((lin_sum_kernel<float>), dim3((unsigned)((NK + 1023) / 1024)), dim3(256), 0, st, slabs, 3, NK, a.K, nullptr,
+                     (float*)a.dW);
+  SCP_LAUNCH_CHECK();
+  return SCP_OK;
 }
 
 int check_args(const ScpLinear8* a, const char* who) {
@@ -655,30 +926,35 @@ extern "C" int scp_linear8_fwd(const ScpLinear8* a_, void* stream) {
   SCP_CHECK(((uintptr_t)a.ws & 255) == 0, SCP_ERR_ARG, "scp_linear8_fwd: the workspace must be 256-byte aligned");
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)a.ws;
-  const long KK = (long)p.np * p.Kp;
-  int rc;
-  const __bf16* A = (const __bf16*)a.x;
-  long lda = a.ldx;
-  if (p.x_direct) {
-    rc = a.codes ? scp_pack8(a.x, 1, a.ldx, a.M, a.K, a.codes, a.steps, stream) : SCP_OK;
-  } else {
+  float* gws = (float*)(ws + p.g_off);
+  const long ld = (long)p.np * p.Kp;
+  int rc = SCP_OK;
+  const __bf16 *A = (const __bf16*)a.x, *B = (const __bf16*)a.W;
+  if (p.prep_x) {
     __bf16* dst = (__bf16*)(ws + p.a_off);
     A = dst;
-    lda = KK;
 #define PREP_X(T, LAY)                                                                                     \
   (a.codes ? prep<T, LAY, true>(a.x, a.ldx, a.M, a.K, 0, dst, p.Kp, a.codes, a.steps, st)                   \
            : prep<T, LAY, false>(a.x, a.ldx, a.M, a.K, 0, dst, p.Kp, nullptr, nullptr, st))
     rc = a.x_bf16 ? PREP_X(__bf16, LAY_ONE) : p.np == 1 ? PREP_X(float, LAY_ONE) : PREP_X(float, LAY_COLS_A);
 #undef PREP_X
+  } else if (a.codes) {
+    rc = scp_pack8(a.x, a.x_bf16, a.ldx, a.M, a.K, a.codes, a.steps, stream);
   }
   if (rc) return rc;
-  const __bf16* B = (const __bf16*)a.W;
-  if (!p.w_direct) {
+  if (p.y.ts == 64) {
+    LgArgs g = {};
+    g.A = A; g.B = B; g.C = a.y;
+    g.lda = a.ldx; g.ldb = a.K;
+    g.M = (int)a.M; g.N = a.N; g.K = a.K;
+    return direct_rows<OP_ROW>(a, p, p.y, g, a.b, gws, st);
+  }
+  if (p.prep_w) {
     B = (const __bf16*)(ws + p.b_off);
     if ((rc = prep_w(a, p, false, (__bf16*)(ws + p.b_off), st))) return rc;
   }
-  return rows_product(p.y, 0, a.M, a.N, p.np == 1 ? a.K : KK, A, lda, B, p.w_direct ? a.K : KK, a.y, a.x_bf16, a.b,
-                      (float*)(ws + p.g_off), st);
+  return rows_product(p.y, 0, a.M, a.N, p.np == 1 ? a.K : ld, A, p.prep_x ? ld : a.ldx, B, p.prep_w ? ld : a.K, a.y, a.x_bf16, a.b,
+                      gws, st);
 }
 
 extern "C" int scp_linear8_bwd(const ScpLinear8* a_, void* stream) {
@@ -692,27 +968,27 @@ extern "C" int scp_linear8_bwd(const ScpLinear8* a_, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)a.ws;
   float* gws = (float*)(ws + p.g_off);
-  const long NN = (long)p.np * p.Np;
-  const bool need_dy = a.dx || a.dW, write_dy = need_dy && !p.dy_direct;
+  const long ld = (long)p.np * p.Np, lda = p.prep_dy ? ld : a.N;
+  const __bf16* A = p.prep_dy ? (const __bf16*)(ws + p.a_off) : (const __bf16*)a.dy;
   int rc;
-  const __bf16* A = (const __bf16*)a.dy;
-  long lda = a.N;
-  if (write_dy) {
-    A = (const __bf16*)(ws + p.a_off);
-    lda = NN;
-  }
   // The column sums come out of the pass that writes the operand's blocks; where none is needed, they come last, when the
   // products have left dy in the last-level cache (16384 x 4096 bf16: 43 us before them, 20 us after).
-  if (write_dy && (rc = dy_pass(a, p, true, st))) return rc;
-  if (a.dx) {
+  if (p.prep_dy && (rc = dy_pass(a, p, true, st))) return rc;
+  if (a.dx && p.dx.ts == 64) {
+    LgArgs g = {};
+    g.A = (const __bf16*)a.dy; g.B = a.W; g.C = a.dx;
+    g.lda = a.lddy; g.ldb = a.K;
+    g.M = (int)a.M; g.N = a.K; g.K = a.N;
+    if ((rc = direct_rows<OP_COL>(a, p, p.dx, g, nullptr, gws, st))) return rc;
+  } else if (a.dx) {
     const __bf16* B = (const __bf16*)a.W;
-    if (!p.w_direct) {
+    if (p.prep_w) {
       B = (const __bf16*)(ws + p.b_off);
       if ((rc = prep_w(a, p, true, (__bf16*)(ws + p.b_off), st))) return rc;
     }
-    if ((rc = rows_product(p.dx, 1, a.M, a.K, p.np == 1 ? a.N : NN, A, lda, B, p.w_direct ? a.K : p.Kp, a.dx, a.x_bf16, nullptr, gws, st)))
+    if ((rc = rows_product(p.dx, 1, a.M, a.K, p.np == 1 ? a.N : ld, A, lda, B, p.prep_w ? p.Kp : a.K, a.dx, a.x_bf16, nullptr, gws, st)))
       return rc;
   }
   if (a.dW && (rc = weight_product(a, p, A, lda, gws, st))) return rc;
-  return a.db && !write_dy ? dy_pass(a, p, false, st) : SCP_OK;
+  return a.db && !p.prep_dy ? dy_pass(a, p, false, st) : SCP_OK;
 }

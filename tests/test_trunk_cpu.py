@@ -141,10 +141,13 @@ def test_linear8_c_entries_refuse():
         assert L.scp_linear8_fwd_ws(args(**bad)) == -1 and L.scp_linear8_bwd_ws(args(**bad)) == -1, bad
     for bad in (dict(M=1 << 30), dict(K=(1 << 20) + 1), dict(N=40000, K=40000)):
         assert L.scp_linear8_fwd(args(**bad), None) == -2 and L.scp_linear8_fwd_ws(args(**bad)) == -1, bad
-    for bad in (dict(x=None), dict(W=None), dict(y=None), dict(ldx=-1), dict(ws=None), dict(ws=4096 + 16)):
+    split = dict(M=64, N=4096, K=4096, ldx=4096, lddy=4096)          # few tiles, long sums: K-ranges, hence slabs
+    assert L.scp_linear8_fwd_ws(args(**split)) > 0 and L.scp_linear8_bwd_ws(args(**split, dx=4096)) > 0
+    for bad in (dict(x=None), dict(W=None), dict(y=None), dict(ldx=-1), dict(split, ws=None), dict(split, ws=4096 + 16)):
         assert L.scp_linear8_fwd(args(**bad), None) == -1, bad
-    for bad in (dict(dy=None), dict(lddy=-1), dict(dx=4096, W=None), dict(dW=4096), dict(dx=4096, ws=None), dict(db=4096, ws=None)):
+    for bad in (dict(dy=None), dict(lddy=-1), dict(dx=4096, W=None), dict(dW=4096), dict(split, dx=4096, ws=None),
+                dict(db=4096, ws=None)):
         assert L.scp_linear8_bwd(args(**bad), None) == -1, bad
-    # aligned bf16 operands need no copies: the workspace holds K-range slabs only, none for a large product
+    # aligned bf16 operands need no copies, and a large product no slabs
     big = dict(x_bf16=1, w_bf16=1, M=16384, N=4096, K=4096, ldx=4096, lddy=4096, dx=4096, dW=4096, codes=4096, steps=4096)
     assert L.scp_linear8_fwd_ws(args(**big)) == 0 and L.scp_linear8_bwd_ws(args(**big)) == 0
