@@ -259,12 +259,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
     if (want[0]) out[0] = fresh(x, {rows, cols}, x.scalar_type());
     if (want[1]) out[1] = fresh(x, {rows, cols}, t[1].scalar_type());
-    // the gradients of one number a column: rows of one small tensor
-    const Tensor small = columns ? fresh(x, {columns, cols}, at::kFloat) : Tensor();
+    // the gradients of one number a column: rows of one small tensor, each from a 256-byte boundary
+    const int64_t pitch = (cols + 63) / 64 * 64;
+    const Tensor small = columns ? fresh(x, {columns, pitch}, at::kFloat) : Tensor();
     int next = 0;
     for (int i = 2; i < 8; i++) {
       if (!want[i]) continue;
-      if (i > 3 || (i == 3 && f.scale_mode == 2) || (i == 2 && f.gate_mode == 3)) out[i] = small.select(0, next++);
+      if (i > 3 || (i == 3 && f.scale_mode == 2) || (i == 2 && f.gate_mode == 3)) out[i] = small.as_strided({cols}, {1}, pitch * next++);
       else out[i] = fresh(x, t[i].sizes(), t[i].scalar_type());
     }
     if (rows == 0) {           // no cell: nothing to launch, the parameters' sums are empty

@@ -177,6 +177,62 @@ class HipLinear(nn.Linear):
         return ops.linear(x, self.weight, self.bias, relu_input)
 
 
+class HipLinear8(HipLinear):
+    """HipLinear that keeps its input for the backward pass as an 8-bit checkpoint (ops.linear8): 1 + 1/64 byte per element
+    instead of 4 (or 2).  The weight gradient is taken from the checkpoint's values; output, input and bias gradient are not
+    affected."""
+
+    def forward(self, x):
+        return ops.linear8(x, self.weight, self.bias)
+
+
+class ResidualTrunk(nn.Module):
+    """A deep residual trunk over [..., width] for encoders beyond the reference's two hidden layers: `depth` blocks of
+    Linear -> activation -> Linear in a residual stream, with a norm in front of every block and behind it,
+
+        h_i = W2_i act(W1_i y_i + b1_i) + b2_i       r_i+1 = r_i + scale_i * act_g(gate_i) * Norm(h_i)       y_i+1 = Norm(r_i+1)
+
+    forward(x) returns the last y.  Everything between two blocks' products is one kernel each way
+    (ops.gated_residual_norm), and the blocks keep their activations in 8 bits (HipLinear8, ops.act8).
+    width, depth: >= 1 (width at most 16384); hidden: the blocks' inner width (4 * width by default); activation: 'gelu', 'silu'
+    or 'leaky_relu'; norm: 'layer' or 'rms'; gate: None, 'sigmoid' or 'tanh', a learned gate for every column; scale: initial
+    residual scale, learned per column; block_dtype: float32 or bfloat16, the type inside the blocks (the stream keeps x's)."""
+
+    def __init__(self, width, depth, hidden=None, activation="gelu", norm="layer", gate=None, scale=1.0, eps=1e-5,
+                 block_dtype=torch.float32):
+        super().__init__()
+        if width < 1 or width > 16384 or depth < 1:
+            raise ValueError(f"ResidualTrunk: width 1 to 16384 and depth >= 1, got {width}, {depth}")
+        if norm not in ("layer", "rms") or gate not in (None, "sigmoid", "tanh") or activation not in ops._ACTS8:
+            raise ValueError(f"ResidualTrunk: unknown norm {norm!r}, gate {gate!r} or activation {activation!r}")
+        if block_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"ResidualTrunk: block_dtype must be float32 or bfloat16, got {block_dtype}")
+        hidden = hidden or 4 * width
+        self.width, self.norm, self.gate_act, self.activation, self.eps, self.block_dtype = width, norm, gate, activation, eps, block_dtype
+        self.fc1 = nn.ModuleList(HipLinear8(width, hidden) for _ in range(depth))
+        self.fc2 = nn.ModuleList(HipLinear8(hidden, width) for _ in range(depth))
+        # pre[0] is the norm in front of the first block, pre[i + 1] the one behind block i's residual add
+        self.pre_weight = nn.ParameterList(nn.Parameter(torch.ones(width)) for _ in range(depth + 1))
+        self.post_weight = nn.ParameterList(nn.Parameter(torch.ones(width)) for _ in range(depth))
+        layer = norm == "layer"
+        self.pre_bias = nn.ParameterList(nn.Parameter(torch.zeros(width)) for _ in range(depth + 1)) if layer else None
+        self.post_bias = nn.ParameterList(nn.Parameter(torch.zeros(width)) for _ in range(depth)) if layer else None
+        self.scale = nn.ParameterList(nn.Parameter(torch.full((width,), float(scale))) for _ in range(depth))
+        self.gate = nn.ParameterList(nn.Parameter(torch.zeros(width)) for _ in range(depth)) if gate else None
+
+    def forward(self, x):
+        bias = (lambda p, i: None) if self.pre_bias is None else (lambda p, i: p[i])
+        r, y = ops.gated_residual_norm(x, pre=self.norm, pre_weight=self.pre_weight[0], pre_bias=bias(self.pre_bias, 0),
+                                       eps=self.eps, out_dtype=self.block_dtype)
+        for i, (fc1, fc2) in enumerate(zip(self.fc1, self.fc2)):
+            h = fc2(ops.act8(fc1(y), self.activation))
+            r, y = ops.gated_residual_norm(
+                r, h, gate=None if self.gate is None else self.gate[i], gate_act=self.gate_act or "none", scale=self.scale[i],
+                post=self.norm, post_weight=self.post_weight[i], post_bias=bias(self.post_bias, i), pre=self.norm,
+                pre_weight=self.pre_weight[i + 1], pre_bias=bias(self.pre_bias, i + 1), eps=self.eps)
+        return y
+
+
 def init_weights(nn_modules, method="xavier_normal"):
     """utils.py:68-78 (note the reference tests `type(m) == nn.Linear`; HipLinear must be initialised too)."""
     if isinstance(nn_modules, nn.Linear):

@@ -151,3 +151,20 @@ def test_linear8_c_entries_refuse():
     # aligned bf16 operands need no copies, and a large product no slabs
     big = dict(x_bf16=1, w_bf16=1, M=16384, N=4096, K=4096, ldx=4096, lddy=4096, dx=4096, dW=4096, codes=4096, steps=4096)
     assert L.scp_linear8_fwd_ws(args(**big)) == 0 and L.scp_linear8_bwd_ws(args(**big)) == 0
+
+
+@pytest.mark.parametrize("args,kw", [((0, 1), {}), ((16385, 1), {}), ((8, 0), {}), ((8, 1), {"norm": "batch"}),
+                                     ((8, 1), {"gate": "none"}), ((8, 1), {"activation": "relu6"}),
+                                     ((8, 1), {"block_dtype": torch.float16})])
+def test_residual_trunk_refuses(args, kw):
+    import scpair_amd as S
+    with pytest.raises(ValueError):
+        S.ResidualTrunk(*args, **kw)
+
+
+def test_residual_trunk_parameters():
+    import scpair_amd as S
+    names = {n for n, _ in S.ResidualTrunk(8, 2, gate="sigmoid").named_parameters()}
+    assert {"fc1.1.weight", "fc2.0.bias", "pre_weight.2", "pre_bias.2", "post_weight.1", "post_bias.1", "scale.1", "gate.1"} <= names
+    names = {n for n, _ in S.ResidualTrunk(8, 1, norm="rms").named_parameters()}
+    assert not any("norm" in n or "_bias" in n or "gate" in n for n in names)
