@@ -34,7 +34,7 @@ template <bool FAST> __device__ __forceinline__ float act_value(float x, int kin
     return 0.5f * x * (1.f + erff(x * 0.70710678f));
   }
   if (kind == ACT_SILU) return FAST ? x * __builtin_amdgcn_rcpf(1.f + __expf(-x)) : x / (1.f + expf(-x));
-  return x > 0.f ? x : slope * x;
+  return x > 0.f ? x : slope == 0.f && x < 0.f ? 0.f : slope * x;      // (relu of -infinity is 0)
 }
 template <bool FAST> __device__ __forceinline__ float act_slope(float x, int kind, float slope) {
   if (kind == ACT_GELU) {

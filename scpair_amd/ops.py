@@ -2186,6 +2186,11 @@ def unpack8(p, dtype=None):
     dtype = dtype or p.dtype
     if dtype not in _FLOATS:
         raise ValueError(f"unpack8: float32 or bfloat16, got {dtype}")
+    rows, groups = math.prod(p.shape[:-1]), (p.shape[-1] + 63) // 64
+    if (p.codes.dtype is not torch.int8 or p.steps.dtype is not torch.uint8 or p.codes.shape != (rows, 64 * groups)
+            or p.steps.shape != (rows, groups) or not p.codes.is_contiguous() or not p.steps.is_contiguous()):
+        raise ValueError(f"unpack8: codes {p.codes.dtype} {tuple(p.codes.shape)} and steps {p.steps.dtype} {tuple(p.steps.shape)} "
+                         f"are not the packed form of {tuple(p.shape)}")
     _same_device("unpack8", p.codes, p.steps)
     if math.prod(p.shape) == 0:
         return p.codes.new_empty(p.shape, dtype=dtype)

@@ -331,3 +331,85 @@ def test_captured_and_replayed():
         got = [o.clone() for o in outs]
         for a, b in zip(got, step(*leaves(*batch))):
             assert torch.equal(a, b)
+
+
+def test_relu_of_infinities():
+    from scpair_amd import ops
+    x = torch.tensor([[float("inf"), -float("inf"), float("nan"), -1.0, 0.0, 2.0]])
+    for dtype in (F32, B16):
+        a = ops.act8(x.to(dtype).cuda(), "leaky_relu", 0.0).cpu().float()
+        assert a[0, 0] == float("inf") and a[0, 1] == 0 and a[0, 2].isnan() and a[0, 3:].tolist() == [0.0, 0.0, 2.0]
+
+
+def _net(x, W, b):
+    from scpair_amd import ops
+    r, y = ops.gated_residual_norm(x, pre="rms")
+    h = ops.linear8(ops.act8(ops.linear8(y, W, b), "gelu"), W.t(), None)
+    return ops.gated_residual_norm(r, h, gate=y, scale=0.3, post="layer", pre="rms")[1]
+
+
+@pytest.mark.parametrize("dtype", [F32, B16])
+def test_backward_twice_offloaded_recomputed_and_elsewhere(dtype):
+    """The same gradients, bit for bit: from a second backward pass over a kept graph, with the saved tensors moved to host
+    memory in between, under activation recomputation, on another stream, and with the backward pass in the calling thread."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)
+    x, W, b, up = rn(70, 136).requires_grad_(), rn(264, 136).requires_grad_(), rn(264).requires_grad_(), rn(70, 136)
+    y = _net(x, W, b)
+    first = torch.autograd.grad(y, (x, W, b), up, retain_graph=True)
+    runs = [torch.autograd.grad(y, (x, W, b), up)]
+    with torch.autograd.graph.save_on_cpu():
+        y = _net(x, W, b)
+    runs.append(torch.autograd.grad(y, (x, W, b), up))
+    runs.append(torch.autograd.grad(checkpoint(_net, x, W, b, use_reentrant=False), (x, W, b), up))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, W, b)]
+        runs.append(torch.autograd.grad(_net(*leaves), leaves, up.clone()))
+        torch.cuda.current_stream().synchronize()
+    with torch.autograd.set_multithreading_enabled(False):
+        runs.append(torch.autograd.grad(_net(x, W, b), (x, W, b), up))
+    for run in runs:
+        for a, c in zip(first, run):
+            assert torch.equal(a, c)
+
+
+def test_second_derivatives_are_refused():
+    from scpair_amd import ops
+    x = torch.randn(8, 40, device="cuda", requires_grad=True)
+    W = torch.randn(16, 40, device="cuda", requires_grad=True)
+    for out in (ops.act8(x, "silu"), ops.linear8(x, W)):
+        d, = torch.autograd.grad(out.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            d.sum().backward()
+
+
+def test_weights_changed_between_forward_and_backward_are_refused():
+    from scpair_amd import ops
+    x, W = torch.randn(8, 40, device="cuda", requires_grad=True), torch.randn(16, 40, device="cuda", requires_grad=True)
+    y = ops.linear8(x, W)
+    with torch.no_grad():
+        W.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("N,K", [(1, 300), (7, 300), (300, 1), (300, 7), (9, 9)])
+@pytest.mark.parametrize("xt", [F32, B16])
+def test_linear8_narrow_sides_and_broadcast_rows(N, K, xt):
+    """Fewer than 8 inputs or outputs, and inputs and gradients whose rows are one row (stride 0)."""
+    from scpair_amd import ops
+    g = torch.Generator().manual_seed(N * 1000 + K)
+    x, W, up = torch.randn(1, K, generator=g).to(xt), torch.randn(N, K, generator=g).to(xt), torch.randn(1, N, generator=g).to(xt)
+    M = 200
+    xl, Wl = x.cuda().requires_grad_(), W.cuda().requires_grad_()
+    y = ops.linear8(xl.expand(M, K), Wl)
+    dxr, dW = torch.autograd.grad(y, (xl, Wl), up.cuda().expand(M, N))
+    xd, Wd, ud = x.double(), W.double(), up.double()
+    v = pack_ref(x)[2]
+    near = lambda got, want, err: ((got.detach().cpu().double() - want).abs() <= err + half_step(want, xt) * 1.01).all()
+    assert near(y, (xd @ Wd.t()).expand(M, N), bound(xd, Wd.t(), 6 * K) + 2.0 ** -20)
+    assert near(dW, M * (ud.t() @ v), M * (bound(ud.t(), v, 3 * M) + 2.0 ** -20))
+    # each row's dx is rounded to xt before autograd adds the rows
+    assert near(dxr, M * (ud @ Wd), M * (bound(ud, Wd, 6 * N) + 2.0 ** -20 + half_step(ud @ Wd, xt) + 16 * E * (ud @ Wd).abs()))

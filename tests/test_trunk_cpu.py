@@ -81,6 +81,12 @@ def test_residual_norm_c_entry_refuses():
     lambda: ops.unpack8(torch.zeros(3)),
     lambda: ops.unpack8(ops.Packed8(torch.zeros(1, 64, dtype=torch.int8), torch.zeros(1, 1, dtype=torch.uint8), (1, 64),
                                     torch.float32), torch.float64),
+    lambda: ops.unpack8(ops.Packed8(torch.zeros(1, 64, dtype=torch.int8), torch.zeros(1, 1, dtype=torch.uint8), (2, 64),
+                                    torch.float32)),
+    lambda: ops.unpack8(ops.Packed8(torch.zeros(1, 128, dtype=torch.int8)[:, ::2], torch.zeros(1, 1, dtype=torch.uint8), (1, 64),
+                                    torch.float32)),
+    lambda: ops.unpack8(ops.Packed8(torch.zeros(1, 64, dtype=torch.int8), torch.zeros(1, 2, dtype=torch.uint8), (1, 64),
+                                    torch.float32)),
     lambda: ops.act8(torch.zeros(3, 4, dtype=torch.float64)),
     lambda: ops.act8(torch.zeros(3, 4), "tanh"),
     lambda: ops.linear8(torch.zeros(3, 4), torch.zeros(5, 3)),
