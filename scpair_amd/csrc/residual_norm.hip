@@ -18,7 +18,7 @@
 //
 // Bound: HBM.  One pass over the data in each direction: a row lives in registers, 8 consecutive columns per lane and
 // chunk (16 bytes of bf16, 32 of fp32), and a workgroup walks rows with the column constants and column sums in registers
-// and the next row's values on their way.  Up to 1024 columns a row belongs to one wave (no barriers), above that to a workgroup.  Rows need no
+// and the next row's values on their way.  Narrow rows share a wave (8 to 64 lanes each, no barriers), wide ones have a workgroup.  Rows need no
 // alignment: the vector accesses are declared with the element's alignment, which the hardware takes as they are.
 // Column sums leave a workgroup as one partial row each; a second launch adds them in a fixed order (no atomics).
 #include "common.h"
@@ -90,14 +90,17 @@ __device__ __forceinline__ float gate_both(float g, int act, float& d) {
   return g;
 }
 
-// sum over the wave, in every lane
+// sum over the wave (or, G < 64, over groups of G neighbouring lanes), in every lane
+template <int G = 64>
 __device__ __forceinline__ float wsum(float v) {
   v += dppf<0xB1>(v);
   v += dppf<0x4E>(v);
+  if constexpr (G == 8) return v + dppf<0x141>(v);
   v += dppf<0x124>(v);
   v += dppf<0x128>(v);
-  v = xor16_sum(v);
-  return xor32_sum(v);
+  if constexpr (G >= 32) v = xor16_sum(v);
+  if constexpr (G == 64) v = xor32_sum(v);
+  return v;
 }
 // columns of wave w of a workgroup that holds a row in NCH rounds of blockDim.x chunks
 template <int NCH>
@@ -122,7 +125,7 @@ constexpr int RED = 4 * 16;
 template <int TPR, int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], float* red, int& turn) {
 #pragma unroll
-  for (int i = 0; i < NV; i++) v[i] = wsum(v[i]);
+  for (int i = 0; i < NV; i++) v[i] = wsum<(TPR < 64 ? TPR : 64)>(v[i]);
   if constexpr (TPR > 64) {
     float* s = red + (turn & 1) * RED;
     turn++;
@@ -149,7 +152,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const float 
     for (int c = 0; c < NCH; c++)
 #pragma unroll
       for (int i = 0; i < 8; i++) s += c == NCH - 1 ? v[c][i] * own[i] : v[c][i];
-    s = wsum(s);
+    s = wsum<(TPR < 64 ? TPR : 64)>(s);
     if constexpr (TPR > 64) {
       mean = s * __builtin_amdgcn_rcpf((float)max(wave_cols<NCH>(threadIdx.x >> 6, D), 1));
     } else {
@@ -184,8 +187,15 @@ __device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const float 
   rstd = 1.f / sqrtf(q[0] * inv_d + eps);
 }
 
-// Rows of one wave share a workgroup of four (independent in the forward; in the backward they add their column sums).
-template <int TPR> constexpr int threads() { return TPR == 64 ? 256 : TPR; }
+// Rows of TPR <= 64 lanes share a workgroup of four waves (independent in the forward; in the backward they add their column
+// sums); wider rows have a workgroup each, of at most TPR threads.
+template <int TPR> constexpr int threads() { return TPR <= 64 ? 256 : TPR; }
+template <int TPR> __device__ __forceinline__ long first_row() {
+  if constexpr (TPR > 64) return blockIdx.x;
+  // a wave's row is uniform: its address goes into scalar registers
+  const int in = TPR == 64 ? (int)__builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / TPR;
+  return (long)blockIdx.x * (256 / TPR) + in;
+}
 
 // column constants of one chunk: vector loads behind uniform tests
 template <bool SMALL>
@@ -234,17 +244,17 @@ __device__ __forceinline__ void fold(const ScpResidualNorm& a, int base, float* 
 // GF: a gate for every element
 template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL>
 __global__ __launch_bounds__(threads<TPR>()) void rnorm_fwd_kernel(ScpResidualNorm a) {
-  constexpr int RPW = threads<TPR>() / TPR;
+  constexpr int RPW = TPR <= 64 ? 256 / TPR : 1;
   __shared__ float red[TPR > 64 ? 2 * RED : 1];
-  const int t = RPW > 1 ? threadIdx.x & 63 : threadIdx.x, D = a.cols;
-  const int nt = RPW > 1 ? 64 : blockDim.x;      // threads of a row
+  const int t = RPW > 1 ? threadIdx.x & (TPR - 1) : threadIdx.x, D = a.cols;
+  const int nt = RPW > 1 ? TPR : blockDim.x;      // threads of a row
   const float inv_d = 1.f / (float)D;
   int turn = 0;
   if constexpr (TPR > 64) {
     for (int i = threadIdx.x; i < 2 * RED; i += blockDim.x) red[i] = 0.f;
     __syncthreads();
   }
-  long row = (long)blockIdx.x * RPW + (RPW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);   // wave-uniform
+  long row = first_row<TPR>();
   const long stride = (long)gridDim.x * RPW;
   int base[NCH];
 #pragma unroll
@@ -272,7 +282,9 @@ __global__ __launch_bounds__(threads<TPR>()) void rnorm_fwd_kernel(ScpResidualNo
     return v;
   };
   if (row >= a.rows) return;
-  Raw cur = load(row);
+  constexpr bool EARLY = !(TPR == 1024 && NCH == 2);      // (there the next row's values would spill)
+  Raw cur;
+  if (EARLY) cur = load(row);
 
   float A1[NCH][8], B1[NCH][8], W2[NCH][8], B2[NCH][8];
 #pragma unroll
@@ -288,8 +300,8 @@ __global__ __launch_bounds__(threads<TPR>()) void rnorm_fwd_kernel(ScpResidualNo
   }
 
   for (; row < a.rows; row += stride) {
-    const Raw v = cur;
-    if (row + stride < a.rows) cur = load(row + stride);
+    const Raw v = EARLY ? cur : load(row);
+    if (EARLY && row + stride < a.rows) cur = load(row + stride);
     float r[NCH][8];
     float m1 = 0.f, s1 = 1.f, m2, s2;
     if (a.h) {
@@ -336,20 +348,22 @@ constexpr int bwd_waves(int tpr) { return tpr == 1024 ? 4 : tpr == 768 ? 3 : 2; 
 
 // Partial column sums: ws[block][4][cols], order P, sum dy rhat, Q, sum dy; without BIAS (no post bias, no gradient of a pre
 // bias) the last two stay unwritten.
+// Rows above 8192 columns (WIDE) have no registers left for column sums: the row's two means are kept in rowc[rows][2] and
+// rnorm_colpass_kernel reads the tensors once more.
 template <typename XT, typename HT, int TPR, int NCH, bool GF, bool BIAS, bool SMALL>
-__global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kernel(ScpResidualNorm a) {
-  constexpr int RPW = threads<TPR>() / TPR, NA = BIAS ? 4 : 2;
+__global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kernel(ScpResidualNorm a, float* rowc) {
+  constexpr int RPW = TPR <= 64 ? 256 / TPR : 1, NA = BIAS ? 4 : 2;
   __shared__ float red[TPR > 64 ? 2 * RED : 1];
-  __shared__ float colbuf[RPW > 1 ? 2 * RPW * NCH * 512 : 1];
-  const int t = RPW > 1 ? threadIdx.x & 63 : threadIdx.x, D = a.cols;
-  const int nt = RPW > 1 ? 64 : blockDim.x;      // threads of a row
+  __shared__ float colbuf[RPW > 1 ? 2 * 256 * NCH * 8 : 1];
+  const int t = RPW > 1 ? threadIdx.x & (TPR - 1) : threadIdx.x, D = a.cols;
+  const int nt = RPW > 1 ? TPR : blockDim.x;      // threads of a row
   const float inv_d = 1.f / (float)D;
   int turn = 0;
   if constexpr (TPR > 64) {
     for (int i = threadIdx.x; i < 2 * RED; i += blockDim.x) red[i] = 0.f;
     __syncthreads();
   }
-  long row = (long)blockIdx.x * RPW + (RPW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);   // wave-uniform
+  long row = first_row<TPR>();
   const long stride = (long)gridDim.x * RPW;
   int base[NCH];
 #pragma unroll
@@ -389,7 +403,8 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
     return v;
   };
   float A1[NCH][8], B1[NCH][8], W2[NCH][8];
-  float acc[NA][NCH][8];
+  constexpr bool WIDE = TPR == 1024;
+  float acc[WIDE ? 1 : NA][WIDE ? 1 : NCH][8];
 #pragma unroll
   for (int c = 0; c < NCH; c++) {
     fold<SMALL>(a, base[c], A1[c], B1[c], W2[c]);
@@ -397,7 +412,7 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
 #pragma unroll
       for (int i = 0; i < 8; i++) B1[c][i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < NA; k++)
+    for (int k = 0; k < (WIDE ? 0 : NA); k++)
 #pragma unroll
       for (int i = 0; i < 8; i++) acc[k][c][i] = 0.f;
   }
@@ -431,12 +446,18 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
         const float ao = c == NCH - 1 ? av * own[i] : av;
         c12[0] += ao;
         c12[1] += ao * rh[c][i];
-        acc[1][c][i] += dy * rh[c][i];
-        if constexpr (BIAS) acc[3][c][i] += dy;
+        if constexpr (!WIDE) {
+          acc[1][c][i] += dy * rh[c][i];
+          if constexpr (BIAS) acc[3][c][i] += dy;
+        }
       }
     }
     if (a.dy) row_sum<TPR, 2>(c12, red, turn);
     const float c1 = s2 * c12[0] * lay2, c2 = s2 * c12[1] * inv_d;
+    if (WIDE && a.ws && t == 0) {
+      rowc[row * 2] = c1;
+      rowc[row * 2 + 1] = c2;
+    }
     float e[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
@@ -446,8 +467,10 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
         float g = grow;
         if constexpr (GF) g = G[c][i];
         const float dg = du[c][i] * g;
-        acc[0][c][i] += dg * hh[c][i];
-        if constexpr (BIAS) acc[2][c][i] += dg;
+        if constexpr (!WIDE) {
+          acc[0][c][i] += dg * hh[c][i];
+          if constexpr (BIAS) acc[2][c][i] += dg;
+        }
         const float bo = c == NCH - 1 ? dg * A1[c][i] * own[i] : dg * A1[c][i];
         e[0] += bo;
         e[1] += bo * hh[c][i];
@@ -483,11 +506,11 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
     }
   }
 
-  if (!a.ws) return;
+  if (WIDE || !a.ws) return;
   float* wsb = a.ws + (long)blockIdx.x * 4 * D;
   if constexpr (RPW > 1) {
-    // two sums at a time: every wave lays its own into LDS, then the workgroup adds the waves in wave order
-    const int w = threadIdx.x / 64;
+    // two sums at a time: every row's lanes lay their own into LDS, then the workgroup adds them in order
+    const int w = threadIdx.x / TPR;
 #pragma unroll
     for (int k0 = 0; k0 < NA; k0 += 2) {
       if (k0) __syncthreads();
@@ -496,24 +519,68 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
 #pragma unroll
         for (int c = 0; c < NCH; c++)
 #pragma unroll
-          for (int i = 0; i < 8; i++) colbuf[((k * RPW + w) * NCH * 8 + c * 8 + i) * 64 + t] = acc[k0 + k][c][i];
+          for (int i = 0; i < 8; i++) colbuf[((k * RPW + w) * NCH * 8 + c * 8 + i) * TPR + t] = acc[k0 + k][c][i];
       __syncthreads();
-      for (int j = threadIdx.x; j < 2 * D; j += 64 * RPW) {
-        const int k = j >= D, col = j - k * D, q = min(col >> 3, (D - 1) >> 3), ch = q >> 6;
+      for (int j = threadIdx.x; j < 2 * D; j += 256) {
+        const int k = j >= D, col = j - k * D, q = col >> 3, ch = q / TPR;
         const int i = col - chunk_base(q, D);
         float s = 0.f;
 #pragma unroll
-        for (int ww = 0; ww < RPW; ww++) s += colbuf[((k * RPW + ww) * NCH * 8 + ch * 8 + i) * 64 + (q & 63)];
+        for (int ww = 0; ww < RPW; ww++) s += colbuf[((k * RPW + ww) * NCH * 8 + ch * 8 + i) * TPR + (q & (TPR - 1))];
         wsb[(long)(k0 + k) * D + col] = s;
       }
     }
-  } else {
+  } else if constexpr (!WIDE) {
 #pragma unroll
     for (int k = 0; k < NA; k++)
 #pragma unroll
       for (int c = 0; c < NCH; c++)
         if (c < NCH - 1 || last) st8<SMALL, float>(wsb + (long)k * D, base[c], D, acc[k][c]);
   }
+}
+
+// The column sums of rows above 8192 columns: a thread takes 8 columns and every gridDim.y-th row, with the rows' statistics
+// and means at hand; ws as rnorm_bwd_kernel leaves it, one partial row per blockIdx.y.
+template <typename XT, typename HT, bool GF, bool BIAS>
+__global__ __launch_bounds__(256) void rnorm_colpass_kernel(ScpResidualNorm a, const float* __restrict__ rowc) {
+  const int D = a.cols, q = blockIdx.x * 256 + threadIdx.x, base = chunk_base(q, D);
+  if (8 * q >= D) return;
+  float A1[8], B1[8], W2[8], acc[BIAS ? 4 : 2][8];
+  fold<false>(a, base, A1, B1, W2);
+#pragma unroll
+  for (auto& k : acc)
+#pragma unroll
+    for (int i = 0; i < 8; i++) k[i] = 0.f;
+  for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const f32x4 st = *(const f32x4*)(a.stats + row * 4);
+    const float c1 = rowc[row * 2], c2 = rowc[row * 2 + 1];
+    const auto xv = ld8<false, XT>((const XT*)a.x + row * a.ldx, base, D);
+    typename Vec8<HT>::v hv, gv, yv;
+    typename Vec8<XT>::v rv;
+    if (a.h) hv = ld8<false, HT>((const HT*)a.h + row * a.ldh, base, D);
+    if constexpr (GF) gv = ld8<false, HT>((const HT*)a.gate + row * a.ldg, base, D);
+    if (a.dy) yv = ld8<false, HT>((const HT*)a.dy + row * a.lddy, base, D);
+    if (a.dr) rv = ld8<false, XT>((const XT*)a.dr + row * a.lddr, base, D);
+    const float grow = a.gate_mode == GATE_ROW ? gate_value(((const float*)a.gate)[row], a.gate_act) : 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float g = grow;
+      if constexpr (GF) g = gate_value((float)gv[i], a.gate_act);
+      const float hh = a.h ? ((float)hv[i] - st[0]) * st[1] : 0.f;
+      const float rh = ((float)xv[i] + (hh * A1[i] + B1[i]) * g - st[2]) * st[3];
+      const float dy = a.dy ? (float)yv[i] : 0.f;
+      const float dg = ((a.dr ? (float)rv[i] : 0.f) + st[3] * dy * W2[i] - (c1 + rh * c2)) * g;
+      acc[0][i] += dg * hh;
+      acc[1][i] += dy * rh;
+      if constexpr (BIAS) {
+        acc[2][i] += dg;
+        acc[3][i] += dy;
+      }
+    }
+  }
+  float* p = a.ws + (long)blockIdx.y * 4 * D;
+#pragma unroll
+  for (int k = 0; k < (BIAS ? 4 : 2); k++) st8<false, float>(p + (long)k * D, base, D, acc[k]);
 }
 
 // The columns' sums of the partial rows (fixed order, fp64), and from them the parameters' gradients.  A workgroup takes 32
@@ -585,32 +652,45 @@ __global__ __launch_bounds__(256) void rnorm_scale_kernel(const float* each, int
 
 constexpr int MAX_COLS = 16384;
 
-// Rows up to 1024 columns: a wave each, four to a workgroup.  Wider rows: a workgroup each, of as many waves as 8 columns per
-// lane take (16 where that would not fit its register budget).
-unsigned wg_threads(int cols, int nch) { return cols <= 1024 ? 256u : 64u * ((cols + 512 * nch - 1) / (512 * nch)); }
+// Lanes of a row in a shared workgroup, 8 columns each; wider rows have a workgroup each, of as many waves as they need.
+int row_lanes(int cols) { return cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : 64; }
+unsigned wide_threads(int cols, int nch) { return 64u * ((cols + 512 * nch - 1) / (512 * nch)); }
 
-// Workgroups of the backward: about those that are resident at once, since each leaves a partial row per column sum
+// Workgroups of the backward: about those that are resident at once, since each leaves a partial row per column sum (above 8192
+// columns: the partial rows of the column pass)
 int bwd_grid(long rows, int cols) {
-  const int rpw = cols <= 1024 ? 4 : 1;
-  const long need = (rows + rpw - 1) / rpw, cap = cols <= 2048 ? 512 : 256;
+  const int rpw = cols <= 512 ? 256 / row_lanes(cols) : 1;
+  const long need = (rows + rpw - 1) / rpw;
+  // (513 .. 1024 columns: two waves to a workgroup; few rows leave fewer partial rows, whose sum then costs as much as they do)
+  const long cap = cols <= 512 ? 512 : cols <= 1024 ? (rows < 16384 ? 512 : 1024) : cols <= 2048 ? 512 : cols <= 8192 ? 256 : 128;
   return (int)(need < cap ? need : cap);
 }
 
 template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL = false>
 int go_fwd(const ScpResidualNorm& a, hipStream_t st) {
-  const unsigned T = wg_threads(a.cols, NCH);
-  const long rpw = TPR == 64 ? 4 : 1, need = (a.rows + rpw - 1) / rpw, cap = 256L * (2048 / T);
+  const unsigned T = TPR <= 64 ? 256 : wide_threads(a.cols, NCH);
+  const long rpw = TPR <= 64 ? 256 / TPR : 1, need = (a.rows + rpw - 1) / rpw, cap = 256L * (2048 / T);
   hipLaunchKernelGGL((rnorm_fwd_kernel<XT, HT, TPR, NCH, GF, SMALL>), dim3((unsigned)(need < cap ? need : cap)), dim3(T), 0, st, a);
   SCP_LAUNCH_CHECK();
   return SCP_OK;
 }
 template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL = false>
 int go_bwd(const ScpResidualNorm& a, bool bias, hipStream_t st) {
-  const dim3 grid((unsigned)bwd_grid(a.rows, a.cols)), T(wg_threads(a.cols, NCH));
-  if (bias)
-    hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, true, SMALL>), grid, T, 0, st, a);
-  else
-    hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, false, SMALL>), grid, T, 0, st, a);
+  const int nblk = bwd_grid(a.rows, a.cols);
+  const dim3 T(TPR <= 64 ? 256 : wide_threads(a.cols, NCH));
+  if constexpr (TPR == 1024) {
+    float* rowc = a.ws ? a.ws + (long)nblk * 4 * a.cols + a.cols : nullptr;
+    hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, true, SMALL>), dim3((unsigned)(a.rows < 512 ? a.rows : 512)), T, 0, st,
+                       a, rowc);
+    SCP_LAUNCH_CHECK();
+    if (!a.ws) return SCP_OK;
+    const dim3 grid((a.cols + 2047) / 2048, nblk);
+    if (bias) hipLaunchKernelGGL((rnorm_colpass_kernel<XT, HT, GF, true>), grid, dim3(256), 0, st, a, rowc);
+    else hipLaunchKernelGGL((rnorm_colpass_kernel<XT, HT, GF, false>), grid, dim3(256), 0, st, a, rowc);
+  } else {
+    if (bias) hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, true, SMALL>), dim3(nblk), T, 0, st, a, nullptr);
+    else hipLaunchKernelGGL((rnorm_bwd_kernel<XT, HT, TPR, NCH, GF, false, SMALL>), dim3(nblk), T, 0, st, a, nullptr);
+  }
   SCP_LAUNCH_CHECK();
   return SCP_OK;
 }
@@ -621,20 +701,27 @@ int by_width(const ScpResidualNorm& a, int bwd, hipStream_t st) {
   const int D = a.cols;
   if (bwd) {
     const bool bias = bwd == 2;
-    if (D < 8) return go_bwd<XT, HT, 64, 1, GF, true>(a, bias, st);
+    if (D < 8) return go_bwd<XT, HT, 8, 1, GF, true>(a, bias, st);
+    if (D <= 64) return go_bwd<XT, HT, 8, 1, GF>(a, bias, st);
+    if (D <= 128) return go_bwd<XT, HT, 16, 1, GF>(a, bias, st);
+    if (D <= 256) return go_bwd<XT, HT, 32, 1, GF>(a, bias, st);
     if (D <= 512) return go_bwd<XT, HT, 64, 1, GF>(a, bias, st);
-    if (D <= 1024) return go_bwd<XT, HT, 64, 2, GF>(a, bias, st);
+    if (D <= 1024) return go_bwd<XT, HT, 128, 1, GF>(a, bias, st);
     if (D <= 2048) return go_bwd<XT, HT, 256, 1, GF>(a, bias, st);
     if (D <= 4096) return go_bwd<XT, HT, 512, 1, GF>(a, bias, st);
     if (D <= 6144) return go_bwd<XT, HT, 768, 1, GF>(a, bias, st);
     if (D <= 8192) return go_bwd<XT, HT, 512, 2, GF>(a, bias, st);
     return go_bwd<XT, HT, 1024, 2, GF>(a, bias, st);
   }
-  if (D < 8) return go_fwd<XT, HT, 64, 1, GF, true>(a, st);
+  if (D < 8) return go_fwd<XT, HT, 8, 1, GF, true>(a, st);
+  if (D <= 64) return go_fwd<XT, HT, 8, 1, GF>(a, st);
+  if (D <= 128) return go_fwd<XT, HT, 16, 1, GF>(a, st);
+  if (D <= 256) return go_fwd<XT, HT, 32, 1, GF>(a, st);
   if (D <= 512) return go_fwd<XT, HT, 64, 1, GF>(a, st);
   if (D <= 1024) return go_fwd<XT, HT, 64, 2, GF>(a, st);
   if (D <= 4096) return go_fwd<XT, HT, 512, 1, GF>(a, st);
-  if (D <= 8192) return go_fwd<XT, HT, 1024, 1, GF>(a, st);
+  if (D <= 6144) return go_fwd<XT, HT, 1024, 1, GF>(a, st);
+  if (D <= 8192) return go_fwd<XT, HT, 512, 2, GF>(a, st);
   return go_fwd<XT, HT, 1024, 2, GF>(a, st);
 }
 
@@ -679,7 +766,7 @@ extern "C" int scp_residual_norm_fwd(const ScpResidualNorm* a, void* stream) {
 
 extern "C" long scp_residual_norm_bwd_ws_floats(long rows, int cols) {
   if (rows <= 0 || cols <= 0 || cols > MAX_COLS) return 0;
-  return (long)bwd_grid(rows, cols) * 4 * cols + cols;
+  return (long)bwd_grid(rows, cols) * 4 * cols + cols + (cols > 8192 ? 2 * rows : 0);
 }
 
 extern "C" int scp_residual_norm_bwd(const ScpResidualNorm* a_, void* stream) {

@@ -118,8 +118,9 @@ def check(t, post, pre, act, eps=1e-5, use_dr=True, use_dy=True, layout=lambda v
 
 
 TYPES = [(F32, F32), (F32, B16), (B16, B16)]
-# widths of every variant: below a chunk, odd, one wave with one and two chunks, workgroups of 256 / 512 / 1024 threads
-WIDTHS = [1, 7, 8, 30, 65, 511, 512, 513, 900, 1024, 1025, 2047, 2048, 2500, 4096, 4099, 8192, 8193, 16383, 16384]
+# widths of every variant: below a chunk, odd, 8 to 64 lanes to a row, workgroups of 2 to 16 waves with one and two chunks
+WIDTHS = [1, 7, 8, 30, 64, 65, 128, 129, 256, 257, 511, 512, 513, 900, 1024, 1025, 2047, 2048, 2500, 4096, 4099, 6145, 8192, 8193, 16383,
+          16384]
 
 
 @pytest.mark.parametrize("cols", WIDTHS)
@@ -146,6 +147,11 @@ def test_forms(post, pre, gate, scale):
 def test_row_counts(rows):
     check(inputs((rows, 72), F32, F32, "layer", "layer", "row", "one", seed=rows), "layer", "layer", "sigmoid")
     check(inputs((rows, 1100), B16, B16, "rms", "layer", "col", "col", seed=rows), "rms", "layer", "tanh")
+    check(inputs((rows, 30), B16, B16, "layer", "rms", "full", "col", seed=rows), "layer", "rms", "tanh")
+    check(inputs((rows, 200), F32, B16, "rms", "layer", "row", "col", seed=rows), "rms", "layer", "sigmoid")
+    check(inputs((rows, 700), F32, F32, "layer", "rms", "full", "one", seed=rows), "layer", "rms", "sigmoid")
+    if rows < 1000:
+        check(inputs((rows, 9001), F32, F32, "layer", "layer", "col", "one", seed=rows), "layer", "layer", "sigmoid")
 
 
 @pytest.mark.parametrize("use", [(True, False), (False, True)])
