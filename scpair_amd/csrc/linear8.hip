@@ -11,6 +11,7 @@
 // Three matrix kernels: the wide one (wgemm.hip, 256 x 256 tiles) where its tiles fill the chip; 128 x 128 tiles below that;
 // 64 x 64 tiles straight from the tensors, without prepared copies, for the minibatch sizes, where a launch counts as much as
 // the product.  A cost model with measured rates chooses (step_us).
+#include <limits.h>
 #include <stdlib.h>
 #include "ckpt8.h"
 #include "common.h"
@@ -149,6 +150,10 @@ struct LgArgs {
   int M, N, K;
   int tiles_m, tiles_n, nsplit, per_split;   // K-ranges of per_split steps
   int planes, plane_off[3];                  // A's column blocks that are summed up
+  // dgemm, beside the product: A's 8-bit checkpoint (row A), A's column sums [nsplit][M] (col A); null: not asked for
+  int8_t* pack_codes;
+  uint8_t* pack_steps;
+  float* colsum;
 };
 
 template <int TS> __device__ __forceinline__ int lg_col_off(int k, int m) {
@@ -386,7 +391,7 @@ struct DTile {
   }
   __device__ __forceinline__ bool care() const { return (K & 63) || (COL && n < 64); }
   __device__ __forceinline__ void load(Reg& r, int kt, bool live) const {
-    if (!live) return;        // uniform; what is in r then is stored, but never read
+    if (!live) return;        // uniform; r is not used then
     const T* p = base + (COL ? (long)kt * 64 * ld : (long)kt * 64);
 #pragma unroll
     for (int i = 0; i < 2; i++) r.v[i] = *(const VU*)(p + voff[i]);
@@ -432,8 +437,11 @@ struct DTile {
 template <typename TB, int PB, int OPB> struct BTile { typedef DTile<TB, PB, OPB == OP_COL> t; };
 template <typename TB, int PB> struct BTile<TB, PB, OP_Q8> { typedef Tile<64, OP_Q8> t; };
 
+// Two by-products come out of A's tiles while they are in registers, and save a launch and a pass each: a step of 64 k of a row
+// operand is 8 lanes a group of the checkpoint, packed by the tile column kt mod tiles_n, so that no workgroup does it all; and
+// the column sums of a col operand (db), by the first tile column.
 template <typename TA, int PA, bool ACOL, typename TB, int PB, int OPB, typename CT>
-__global__ __launch_bounds__(256, PA + PB > 2 ? 3 : 4) void dgemm_kernel(LgArgs g) {
+__global__ __launch_bounds__(256, PA + PB > 2 || OPB == OP_ROW ? 3 : 4) void dgemm_kernel(LgArgs g) {
   typedef DTile<TA, PA, ACOL> TileA;
   typedef typename BTile<TB, PB, OPB>::t TileB;
   // one term each: two LDS stages, one barrier a step; three terms: one stage, so that three workgroups share a CU
@@ -479,6 +487,38 @@ __global__ __launch_bounds__(256, PA + PB > 2 ? 3 : 4) void dgemm_kernel(LgArgs 
     }
   };
 
+  const bool sums = ACOL && g.colsum && tn == 0;
+  float cs[ACOL ? 8 : 1] = {};
+  int next_pack = !ACOL && g.pack_codes ? kt0 + (tn - kt0 % g.tiles_n + g.tiles_n) % g.tiles_n : INT_MAX;
+  // A's tile of step kt on its way into LDS
+  auto put_a = [&](const typename TileA::Reg& r, int kt, unsigned char* img) {
+    ta.store(r, img);
+    if constexpr (ACOL) {
+      if (sums) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) cs[j] += (float)r.v[i][j];
+      }
+    } else if (OPB == OP_ROW && kt == next_pack) {
+      next_pack += g.tiles_n;
+      const long ld8 = (long)nk * 64;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = (float)r.v[i][j];
+        unsigned step;
+        const uint2 c = quantise(f, step);
+        const long m = m0 + (int)(threadIdx.x >> 3) + 32 * i;
+        if (m < g.M) {
+          *(uint2*)(g.pack_codes + m * ld8 + kt * 64 + 8 * (threadIdx.x & 7)) = c;
+          if ((threadIdx.x & 7) == 0) g.pack_steps[m * nk + kt] = (uint8_t)step;
+        }
+      }
+    }
+  };
+
   if (kt0 < ktv) {
     typename TileA::Reg ra[DEPTH];
     typename TileB::Reg rb[DEPTH];
@@ -487,7 +527,7 @@ __global__ __launch_bounds__(256, PA + PB > 2 ? 3 : 4) void dgemm_kernel(LgArgs 
       ta.load(ra[d], kt0 + d, kt0 + d < ktv);
       tb.load(rb[d], kt0 + d, kt0 + d < ktv);
     }
-    ta.store(ra[0], smem);
+    put_a(ra[0], kt0, smem);
     tb.store(rb[0], smem + PA * 8192);
     __syncthreads();
     for (int kt = kt0; kt < ktv; kt += DEPTH) {
@@ -498,9 +538,11 @@ __global__ __launch_bounds__(256, PA + PB > 2 ? 3 : 4) void dgemm_kernel(LgArgs 
           tb.load(rb[d], kt + d + DEPTH, kt + d + DEPTH < ktv);
           multiply(smem + (d % STAGES) * STAGE);
           if constexpr (STAGES == 1) __syncthreads();
-          unsigned char* na = smem + ((d + 1) % STAGES) * STAGE;
-          ta.store(ra[(d + 1) % DEPTH], na);
-          tb.store(rb[(d + 1) % DEPTH], na + PA * 8192);
+          if (kt + d + 1 < ktv) {
+            unsigned char* na = smem + ((d + 1) % STAGES) * STAGE;
+            put_a(ra[(d + 1) % DEPTH], kt + d + 1, na);
+            tb.store(rb[(d + 1) % DEPTH], na + PA * 8192);
+          }
           __syncthreads();
         }
       }
@@ -512,10 +554,25 @@ __global__ __launch_bounds__(256, PA + PB > 2 ? 3 : 4) void dgemm_kernel(LgArgs 
     ta.load_end(ra, ktv);
     if constexpr (OPB == OP_Q8) tb.load(rb, ktv, true);
     else tb.load_end(rb, ktv);
-    ta.store(ra, smem);
+    put_a(ra, ktv, smem);
     tb.store(rb, smem + PA * 8192);
     __syncthreads();
     multiply(smem);
+  }
+  if constexpr (ACOL) {
+    if (sums) {                  // uniform
+      __syncthreads();
+      float* p = (float*)smem;   // [32 rows of the tile][64 columns]
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[(threadIdx.x >> 3) * 64 + 8 * (threadIdx.x & 7) + j] = cs[j];
+      __syncthreads();
+      if (threadIdx.x < 64 && m0 + (int)threadIdx.x < g.M) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 32; r++) t += p[r * 64 + threadIdx.x];
+        g.colsum[(long)z * g.M + m0 + threadIdx.x] = t;
+      }
+    }
   }
 
   CT* C = (CT*)g.C + (long)z * g.M * g.ldc;
@@ -699,6 +756,9 @@ Plan plan_fwd(const ScpLinear8& a) {
   return p;
 }
 
+int ranges(const Gemm& q, long K);
+bool fused_db(const ScpLinear8& a, const Plan& p);
+
 Plan plan_bwd(const ScpLinear8& a) {
   Plan p = {};
   common_plan(a, p);
@@ -735,8 +795,8 @@ Plan plan_bwd(const ScpLinear8& a) {
   p.b_off = o;
   if (p.prep_w) o += align256((p.np == 1 ? (long)a.N : ld) * p.Kp * 2);
   p.part_off = o;
-  p.parts = colsum_parts(a.M, a.N);
-  if (a.db) o += align256((long)p.parts * a.N * 4);
+  p.parts = fused_db(a, p) ? ranges(p.dw, a.M) : colsum_parts(a.M, a.N);
+  if (a.db && !(fused_db(a, p) && p.parts == 1)) o += align256((long)p.parts * a.N * 4);
   p.g_off = o;
   const long gx = a.dx ? p.dx.ws : 0, gw = a.dW ? p.dw.ws : 0;
   p.total = o + align256(gx > gw ? gx : gw);
@@ -765,6 +825,12 @@ int prep_w(const ScpLinear8& a, const Plan& p, bool rows_below, __bf16* dst, hip
   return prep<float, LAY_COLS_B, false>(a.W, a.K, a.N, a.K, 0, dst, p.Kp, nullptr, nullptr, st);
 }
 
+// K-ranges that are left when a range takes whole steps
+int ranges(const Gemm& q, long K) {
+  const int nk = (int)((K + 63) / 64), per = (nk + q.nsplit - 1) / q.nsplit;
+  return (nk + per - 1) / per;
+}
+
 // tiles, K-ranges and the sum of the slabs around one of the two kernels; C contiguous [M][N]
 template <typename Launch>
 int tiled(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws, hipStream_t st, Launch launch) {
@@ -773,7 +839,7 @@ int tiled(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws, hip
   g.tiles_n = (g.N + q.ts - 1) / q.ts;
   const int nk = (g.K + 63) / 64;
   g.per_split = (nk + q.nsplit - 1) / q.nsplit;
-  g.nsplit = (nk + g.per_split - 1) / g.per_split;
+  g.nsplit = ranges(q, g.K);
   g.ldc = g.N;
   const int slabs = g.nsplit * g.planes;
   if (slabs > 1) g.C = ws;
@@ -845,6 +911,16 @@ int rows_product(const Gemm& q, int b_col, long M, int N, long K, const __bf16* 
   return SCP_OK;
 }
 
+// db from n partial rows
+int finish_db(const ScpLinear8& a, const float* part, int n, hipStream_t st) {
+  hipLaunchKernelGGL(lin_db_kernel, dim3((a.N + 15) / 16), dim3(256), 0, st, part, n, a.N, a.db);
+  SCP_LAUNCH_CHECK();
+  return SCP_OK;
+}
+
+// db comes out of dW's product where that reads dy itself, unless the pass that prepares dy has it already
+bool fused_db(const ScpLinear8& a, const Plan& p) { return a.db && a.dW && p.dw.ts == 64 && !p.prep_dy; }
+
 // dy's blocks (write) and, if asked for, its column sums
 int dy_pass(const ScpLinear8& a, const Plan& p, bool write, hipStream_t st) {
   char* ws = (char*)a.ws;
@@ -860,11 +936,7 @@ int dy_pass(const ScpLinear8& a, const Plan& p, bool write, hipStream_t st) {
   else DY(float, LAY_COLS_A, true);
 #undef DY
   SCP_LAUNCH_CHECK();
-  if (a.db) {
-    hipLaunchKernelGGL(lin_db_kernel, dim3((a.N + 15) / 16), dim3(256), 0, st, part, p.parts, a.N, a.db);
-    SCP_LAUNCH_CHECK();
-  }
-  return SCP_OK;
+  return a.db ? finish_db(a, part, p.parts, st) : SCP_OK;
 }
 
 // dW = dy^T v; A: dy's blocks (unused straight from the tensors)
@@ -876,9 +948,13 @@ int weight_product(const ScpLinear8& a, const Plan& p, const __bf16* A, long lda
   if (p.dw.ts == 64) {
     g.A = (const __bf16*)a.dy;
     g.lda = a.lddy;
-    if (a.x_bf16) return direct_gemm<__bf16, 1, true, __bf16, 1, OP_Q8>(p.dw, g, a.w_bf16, nullptr, ws, st);
-    if (p.np == 1) return direct_gemm<float, 1, true, __bf16, 1, OP_Q8>(p.dw, g, 0, nullptr, ws, st);
-    return direct_gemm<float, 3, true, __bf16, 1, OP_Q8>(p.dw, g, 0, nullptr, ws, st);
+    const int n = ranges(p.dw, a.M);
+    float* part = (float*)((char*)a.ws + p.part_off);
+    if (fused_db(a, p)) g.colsum = n == 1 ? a.db : part;
+    const int rc = a.x_bf16 ? direct_gemm<__bf16, 1, true, __bf16, 1, OP_Q8>(p.dw, g, a.w_bf16, nullptr, ws, st)
+                   : p.np == 1 ? direct_gemm<float, 1, true, __bf16, 1, OP_Q8>(p.dw, g, 0, nullptr, ws, st)
+                               : direct_gemm<float, 3, true, __bf16, 1, OP_Q8>(p.dw, g, 0, nullptr, ws, st);
+    return rc || !g.colsum || n == 1 ? rc : finish_db(a, part, n, st);
   }
   const int off[3] = {0, 2 * p.Np, 5 * p.Np};
   g.planes = p.np == 6 ? 3 : 1;
@@ -938,7 +1014,7 @@ extern "C" int scp_linear8_fwd(const ScpLinear8* a_, void* stream) {
            : prep<T, LAY, false>(a.x, a.ldx, a.M, a.K, 0, dst, p.Kp, nullptr, nullptr, st))
     rc = a.x_bf16 ? PREP_X(__bf16, LAY_ONE) : p.np == 1 ? PREP_X(float, LAY_ONE) : PREP_X(float, LAY_COLS_A);
 #undef PREP_X
-  } else if (a.codes) {
+  } else if (a.codes && p.y.ts != 64) {
     rc = scp_pack8(a.x, a.x_bf16, a.ldx, a.M, a.K, a.codes, a.steps, stream);
   }
   if (rc) return rc;
@@ -947,6 +1023,7 @@ extern "C" int scp_linear8_fwd(const ScpLinear8* a_, void* stream) {
     g.A = A; g.B = B; g.C = a.y;
     g.lda = a.ldx; g.ldb = a.K;
     g.M = (int)a.M; g.N = a.N; g.K = a.K;
+    g.pack_codes = a.codes; g.pack_steps = a.steps;
     return direct_rows<OP_ROW>(a, p, p.y, g, a.b, gws, st);
   }
   if (p.prep_w) {
@@ -990,5 +1067,5 @@ extern "C" int scp_linear8_bwd(const ScpLinear8* a_, void* stream) {
       return rc;
   }
   if (a.dW && (rc = weight_product(a, p, A, lda, gws, st))) return rc;
-  return a.db && !p.prep_dy ? dy_pass(a, p, false, st) : SCP_OK;
+  return a.db && !p.prep_dy && !fused_db(a, p) ? dy_pass(a, p, false, st) : SCP_OK;
 }
