@@ -418,16 +418,21 @@ struct DTile {
       if constexpr (sizeof(T) == 2) {
         *(V*)(img + lds[i]) = r.v[i];
       } else {
-        bf16x8 t[NP];
+        // the terms of bf16_split, two values at a time: a conversion instruction rounds and packs a pair
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        union { bf16x2 p[4]; bf16x8 v; } t[NP];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          __bf16 s[3];
-          bf16_split<NP>(r.v[i][j], s);
+        for (int j = 0; j < 4; j++) {
+          f32x2 f = {r.v[i][2 * j], r.v[i][2 * j + 1]};
 #pragma unroll
-          for (int q = 0; q < NP; q++) t[q][j] = s[q];
+          for (int q = 0; q < NP; q++) {
+            t[q].p[j] = __builtin_convertvector(f, bf16x2);
+            if (q + 1 < NP) f -= __builtin_convertvector(t[q].p[j], f32x2);
+          }
         }
 #pragma unroll
-        for (int q = 0; q < NP; q++) *(bf16x8*)(img + q * 8192 + lds[i]) = t[q];
+        for (int q = 0; q < NP; q++) *(bf16x8*)(img + q * 8192 + lds[i]) = t[q].v;
       }
     }
   }
@@ -629,7 +634,7 @@ struct Gemm {
 // Costs in microseconds of a step of 64 k with w workgroups per CU, measured over products from 300^3 to 16384 x 4096^2 (the
 // product's own time only; a launch 3.5, slabs written and read at 7.5 TB/s, prepared operands at 5).
 double step_us(int ts, int pairs, double w) {
-  if (ts == 64) return pairs == 1 ? 0.25 + 0.2 * w : pairs == 3 ? 0.5 + 0.48 * w : 0.6 + 0.85 * w;
+  if (ts == 64) return pairs == 1 ? 0.25 + 0.2 * w : pairs == 3 ? 0.5 + 0.48 * w : 0.5 + 0.85 * w;
   if (ts == 128) return w == 1 ? 1.15 : 0.7 * w;
   return 2.3 * w;
 }
