@@ -12,7 +12,6 @@
 // 64 x 64 tiles straight from the tensors, without prepared copies, for the minibatch sizes, where a launch counts as much as
 // the product.  A cost model with measured rates chooses (step_us).
 #include <limits.h>
-#include <stdlib.h>
 #include "ckpt8.h"
 #include "common.h"
 #include "scpair_hip.h"
@@ -620,6 +619,9 @@ __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ 
 // plans: what a call launches and where its workspace lies, a function of the shape alone
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr long WIDE_BYTES = (1L << 31) - 65536;      // operand extent that the wide kernel addresses
+// Rows of a prepared operand are no further apart: 128 of them stay within the 32-bit offsets of lgemm's tiles, and a piece of
+// WIDE_BYTES holds hundreds.  Rows of x further apart are copied (to rows of K, at most 2^20 columns, six times that in fp32).
+constexpr long MAX_LD = 1L << 20;
 
 long align256(long b) { return (b + 255) & ~255L; }
 int up8(int n) { return (n + 7) & ~7; }
@@ -654,14 +656,6 @@ void consider(Gemm& best, int ts, int pairs, long M, int N, long K, int planes) 
     best.slabs = ns * planes > 1 ? ns * planes : 0;
     best.ws = (long)best.slabs * M * N * 4;
     best.us = us;
-#ifdef LIN8_TUNE
-    if (const char* e = getenv("LIN8_NS")) {
-      best.nsplit = atoi(e);
-      best.slabs = best.nsplit * planes > 1 ? best.nsplit * planes : 0;
-      best.ws = (long)best.slabs * M * N * 4;
-      return;
-    }
-#endif
   }
 }
 
@@ -684,12 +678,6 @@ Gemm pick_blocks(long M, int N, long K, int planes, bool wide_ok, long wide_ws) 
     if (planes > 1) us += mn * 4 * (2 * planes + 1) / 7.5e6 + LAUNCH_US;
     best = {256, 1, 0, wide_ws, us};
   }
-#ifdef LIN8_TUNE
-  if (const char* e = getenv("LIN8_TS")) {
-    if (atoi(e) == 256) return best;
-    best.us = 1e30;
-  }
-#endif
   consider(best, 128, 1, M, N, K, planes);
   return best;
 }
@@ -725,13 +713,6 @@ long wide_ws_rows(long M, int N, long K, long lda) {
   return (a > b ? a : b) * 4;
 }
 
-bool tune_only(const Gemm& g) {
-#ifdef LIN8_TUNE
-  if (const char* e = getenv("LIN8_TS")) return g.ts != atoi(e);
-#endif
-  return g.ts == 0;
-}
-
 // dgemm forms the offsets inside a tile in 32 bits; its col operands (W for dx, dy for dW) also have rows of 8 elements at
 // least, no closer than their length
 bool direct_rows_ok(long ld) { return ld < 1L << 25; }
@@ -739,7 +720,7 @@ bool direct_rows_ok(long ld) { return ld < 1L << 25; }
 Plan plan_fwd(const ScpLinear8& a) {
   Plan p = {};
   common_plan(a, p);
-  p.x_direct = a.x_bf16 && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx >= a.K && ((uintptr_t)a.x & 15) == 0;
+  p.x_direct = a.x_bf16 && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx >= a.K && a.ldx <= MAX_LD && ((uintptr_t)a.x & 15) == 0;
   const int xb = a.x_bf16 ? 2 : 4, wb = a.w_bf16 ? 2 : 4;
   const long KK = p.np == 1 ? a.K : (long)p.np * p.Kp, ld = (long)p.np * p.Kp;
   const bool ok = ((long)a.N + 192) * ld * 2 < WIDE_BYTES;
@@ -748,7 +729,7 @@ Plan plan_fwd(const ScpLinear8& a) {
   if (!p.w_direct) blocks.us += prep_us((double)a.N * a.K, wb, p.np);
   Gemm direct = pick_direct(a.M, a.N, a.K, p.np);
   if (!direct_rows_ok(a.ldx)) direct.us = 1e30;
-  p.y = (direct.us < blocks.us || tune_only(blocks)) && !tune_only(direct) ? direct : blocks;
+  p.y = direct.us < blocks.us ? direct : blocks;
   p.prep_x = p.y.ts != 64 && !p.x_direct;
   p.prep_w = p.y.ts != 64 && !p.w_direct;
   long o = 0;
@@ -780,14 +761,14 @@ Plan plan_bwd(const ScpLinear8& a) {
   if (!direct_rows_ok(a.lddy) || a.K < 8) xd.us = 1e30;
   // the wide form of dW runs once per plane, each into a slab of its own
   const long ld8 = (a.K + 63) / 64 * 64L, wide_ws = scp_gemm_q8_ws_floats(a.N, a.K, (int)a.M, lda > ld8 ? lda : ld8, a.K) * 4;
-  const Gemm wb_ = pick_blocks(a.N, a.K, a.M, planes, true, align256(wide_ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
+  const Gemm wb_ = pick_blocks(a.N, a.K, a.M, planes, lda <= MAX_LD, align256(wide_ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
   Gemm wd = pick_direct(a.N, a.K, a.M, planes);
   if (!direct_rows_ok(a.lddy) || a.lddy < a.N || a.N < 8) wd.us = 1e30;
   double best = 1e300;
   for (int c = 0; c < 4; c++) {
     const Gemm &x = c & 1 ? xb_ : xd, &w = c & 2 ? wb_ : wd;
     const double us = x.us + w.us + (c ? dy_us : 0);
-    if (us >= best || tune_only(x) || tune_only(w)) continue;
+    if (us >= best) continue;
     best = us;
     p.dx = x;
     p.dw = w;
@@ -881,8 +862,14 @@ template <typename TA, int PA, bool ACOL, typename TB, int PB, int OPB>
 int direct_gemm(const Gemm& q, LgArgs g, int c_bf16, const float* bias, float* ws, hipStream_t st) {
   g.planes = 1;
   return tiled(q, g, c_bf16, bias, ws, st, [st](const LgArgs& a, dim3 grid, bool b16) -> int {
-    if (b16) hipLaunchKernelGGL((dgemm_kernel<TA, PA, ACOL, TB, PB, OPB, __bf16>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((dgemm_kernel<TA, PA, ACOL, TB, PB, OPB, float>), grid, dim3(256), 0, st, a);
+    if constexpr (sizeof(TA) == 2) {       // (fp32 tensors have fp32 products)
+      if (b16) {
+        hipLaunchKernelGGL((dgemm_kernel<TA, PA, ACOL, TB, PB, OPB, __bf16>), grid, dim3(256), 0, st, a);
+        SCP_LAUNCH_CHECK();
+        return SCP_OK;
+      }
+    }
+    hipLaunchKernelGGL((dgemm_kernel<TA, PA, ACOL, TB, PB, OPB, float>), grid, dim3(256), 0, st, a);
     SCP_LAUNCH_CHECK();
     return SCP_OK;
   });

@@ -413,3 +413,20 @@ def test_linear8_narrow_sides_and_broadcast_rows(N, K, xt):
     assert near(dW, M * (ud.t() @ v), M * (bound(ud.t(), v, 3 * M) + 2.0 ** -20))
     # each row's dx is rounded to xt before autograd adds the rows
     assert near(dxr, M * (ud @ Wd), M * (bound(ud, Wd, 6 * N) + 2.0 ** -20 + half_step(ud @ Wd, xt) + 16 * E * (ud @ Wd).abs()))
+
+
+@pytest.mark.parametrize("M,apart", [(130, 1 << 25), (3, 1 << 30)])
+def test_linear8_rows_far_apart(M, apart):
+    """Rows of x that no 32-bit offset reaches from one to the next give what the same rows side by side give."""
+    from scpair_amd import ops
+    g = torch.Generator().manual_seed(M)
+    W = torch.randn(72, 64, generator=g).to(B16).cuda()
+    rows = torch.randn(M, 64, generator=g).to(B16).cuda()
+    far = torch.empty((M - 1) * apart + 64, dtype=B16, device="cuda").as_strided((M, 64), (apart, 1))
+    far.copy_(rows)
+    xd, Wd = rows.cpu().double(), W.cpu().double()
+    want = xd @ Wd.t()
+    with torch.no_grad():
+        assert ((ops.linear8(far, W).cpu().double() - want).abs() <= bound(xd, Wd.t(), 64) + half_step(want, B16)).all()
+    p, q = ops.pack8(far), ops.pack8(rows)
+    assert torch.equal(p.codes, q.codes) and torch.equal(p.steps, q.steps)

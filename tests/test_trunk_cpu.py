@@ -158,6 +158,11 @@ def test_linear8_c_entries_refuse():
     big = dict(x_bf16=1, w_bf16=1, M=16384, N=4096, K=4096, ldx=4096, lddy=4096, dx=4096, dW=4096, codes=4096, steps=4096)
     assert L.scp_linear8_fwd_ws(args(**big)) == 0 and L.scp_linear8_bwd_ws(args(**big)) == 0
 
+    # rows too far apart for a tile's 32-bit offsets are copied, whatever the tile
+    for far in (1 << 25, 1 << 30, 1 << 33):
+        rows = dict(x_bf16=1, w_bf16=1, M=4096, N=4096, K=4096, lddy=4096)
+        assert L.scp_linear8_fwd_ws(args(**rows, ldx=far)) >= 4096 * 4096 * 2 > L.scp_linear8_fwd_ws(args(**rows, ldx=4104))
+
 
 @pytest.mark.parametrize("args,kw", [((0, 1), {}), ((16385, 1), {}), ((8, 0), {}), ((8, 1), {"norm": "batch"}),
                                      ((8, 1), {"gate": "none"}), ((8, 1), {"activation": "relu6"}),
