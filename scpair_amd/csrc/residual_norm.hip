@@ -642,10 +642,10 @@ __global__ __launch_bounds__(1024) void rnorm_cols_kernel(ScpResidualNorm a, int
 }
 
 // gradient of a single residual scale: the columns' shares added up by one workgroup
-__global__ __launch_bounds__(256) void rnorm_scale_kernel(const float* each, int D, float* out) {
+__global__ __launch_bounds__(1024) void rnorm_scale_kernel(const float* each, int D, float* out) {
   __shared__ double red[16];
   double s = 0.0;
-  for (int j = threadIdx.x; j < D; j += 256) s += (double)each[j];
+  for (int j = threadIdx.x; j < D; j += 1024) s += (double)each[j];
   s = block_sum_d(s, red);
   if (threadIdx.x == 0) out[0] = (float)s;
 }
@@ -669,7 +669,12 @@ int bwd_grid(long rows, int cols) {
 template <typename XT, typename HT, int TPR, int NCH, bool GF, bool SMALL = false>
 int go_fwd(const ScpResidualNorm& a, hipStream_t st) {
   const unsigned T = TPR <= 64 ? 256 : wide_threads(a.cols, NCH);
-  const long rpw = TPR <= 64 ? 256 / TPR : 1, need = (a.rows + rpw - 1) / rpw, cap = 256L * (2048 / T);
+  // About as many workgroups as are resident at once, each walking its rows with the next one on its way: beyond that a
+  // workgroup's column constants come again for every row (777 rows of 4999 bf16: 14 us against 17 us with three times as many,
+  // 777 x 8000 fp32 with a full gate 31 against 42 us, 4096 x 1024 fp32 with a full gate 20 against 24 us).  One-chunk rows
+  // have 16 waves a CU; rows of at most 512 columns have few constants, and a minibatch of them is spread as widely as it goes.
+  const long rpw = TPR <= 64 ? 256 / TPR : 1, need = (a.rows + rpw - 1) / rpw;
+  const long cap = 256L * (a.cols <= 512 ? 8 : a.cols <= 1024 ? 2 : NCH == 2 ? 1 : 1024 / T);
   hipLaunchKernelGGL((rnorm_fwd_kernel<XT, HT, TPR, NCH, GF, SMALL>), dim3((unsigned)(need < cap ? need : cap)), dim3(T), 0, st, a);
   SCP_LAUNCH_CHECK();
   return SCP_OK;
@@ -793,7 +798,7 @@ extern "C" int scp_residual_norm_bwd(const ScpResidualNorm* a_, void* stream) {
     hipLaunchKernelGGL((rnorm_cols_kernel<false>), dim3((a.cols + 31) / 32), dim3(1024), 0, st, a, nblk, each);
   SCP_LAUNCH_CHECK();
   if (each) {
-    hipLaunchKernelGGL(rnorm_scale_kernel, dim3(1), dim3(256), 0, st, each, a.cols, a.dscale);
+    hipLaunchKernelGGL(rnorm_scale_kernel, dim3(1), dim3(1024), 0, st, each, a.cols, a.dscale);
     SCP_LAUNCH_CHECK();
   }
   return SCP_OK;
