@@ -373,19 +373,48 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   }
   if constexpr (sizeof(CT) == 2) {
     static_assert(DIRECT, "slabs are fp32");
+    // A wave's 32-row strips go through a private LDS buffer (the operand stages are free after the loop's last barrier), so
+    // that 16 lanes write a 128-byte row segment: an accumulator's own layout makes 2-byte stores, 128 of them a lane.
+    static_assert(NW == 8, "strips of 64 columns");
+    constexpr int LD = 72;                      // lanes 32 .. 63 write four rows further down, to the other 32 banks
+    typedef CT ct4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
     CT* C16 = (CT*)(void*)g.C;
+    float* wt = (float*)smem + wave * (32 * LD);
+    const int c4 = (lane & 15) * 4, n = n0 + wn * WN + c4;
+    const bool whole = n + 4 <= g.N;
+    f32x4 bn = {0.f, 0.f, 0.f, 0.f};
+    if (g.bias) {
+      if (whole) bn = *(const f4u*)(g.bias + n);
+      else
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const int n = n0 + wn * WN + 32 * j + (lane & 31);
-      const float bn = (g.bias && n < g.N) ? g.bias[n] : 0.f;
+        for (int t = 0; t < 4; t++) bn[t] = n + t < g.N ? g.bias[n + t] : 0.f;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 4; i++) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int m = m0 + wm * 128 + 32 * i + acc_row(e, lane);
-          if (m < g.M && n < g.N) C16[(long)m * g.ldc + n] = (CT)(acc[i][j][e] + bn);
+      for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) wt[acc_row(e, lane) * LD + 32 * j + (lane & 31)] = acc[i][j][e];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int it = 0; it < 8; it++) {
+        const int row = 4 * it + (lane >> 4), m = m0 + wm * 128 + 32 * i + row;
+        const f32x4 v = *(const f32x4*)(wt + row * LD + c4) + bn;
+        if (m >= g.M) continue;
+        CT* p = C16 + (long)m * g.ldc + n;
+        if (whole) {
+          ct4 o;
+#pragma unroll
+          for (int t = 0; t < 4; t++) o[t] = (CT)v[t];
+          *(ct4*)p = o;
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4; t++)
+            if (n + t < g.N) p[t] = (CT)v[t];
         }
       }
+      __builtin_amdgcn_wave_barrier();
     }
     return;
   }
