@@ -8,9 +8,10 @@
 //   y  = x W^T   : A = x  row, B = W row        dx = dy W : A = dy row, B = W col        dW = dy^T x : A = dy col, B = x col
 //
 // Workgroup: tile 256 x 256 x 64 on 512 threads = 2 x 4 waves of 128 x 64 (4 x 2 accumulators of the 32x32x16 bf16
-// MFMA, two waves per SIMD) or on 256 threads = 2 x 2 waves of 128 x 128 (one wave per SIMD).  Operand tiles go
-// global -> registers (16-byte buffer loads, the range check supplies the zeros of ragged edges) -> LDS, two LDS
-// stages of 64 KB, one barrier per K-step: the next step's global loads are in flight while this step's 64 MFMAs run.
+// MFMA, two waves per SIMD) or on 256 threads = 2 x 2 waves of 128 x 128 (one wave per SIMD).  Operand tiles come with
+// 16-byte buffer loads, the range check supplying the zeros of ragged edges, straight into LDS (eight waves) or through
+// registers (four), two LDS stages of 64 KB, one barrier per K-step: the next step's global loads are in flight while this
+// step's 64 MFMAs run.
 //   row image  [256][64]  : 128-byte rows, 16-byte chunk c of row r at chunk c ^ ((r >> 1) & 7); read with ds_read_b128
 //   col image  [64][256]  : 512-byte rows, 64-byte segment s of row k at segment s ^ (k & 3); read with the
 //                           transposing ds_read_b64_tr_b16 (4 k-rows x 16 columns per 16 lanes), conflict-free
@@ -83,8 +84,10 @@ __device__ __forceinline__ bf16x8 read_frag(const unsigned char* img, int r0, in
 
 enum { EPI_SLAB = 0, EPI_DIRECT = 1, EPI_ADAMW = 2 };
 
-// NW = 8 (default for the plain products): two waves per SIMD, wave tile 128 x 64, one register set of prefetched tiles
-// (256 registers per lane): one wave's MFMA groups cover the other's waits.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
+// NW = 8 (default for the plain products): two waves per SIMD, wave tile 128 x 64; one wave's MFMA groups cover the other's
+// waits, and the next K-step's tiles go from memory to LDS without passing through registers (a lane's 16 bytes land at
+// LDS slot `lane` of its wave's KB, so the swizzle is applied to what the lane fetches; 16384 x 4096 x 4096 bf16: rows with
+// rows 437 us against 516 us through registers, 1258 TFLOP/s; rows with columns 499 against 512).  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
 // elsewhere): one wave per SIMD, wave tile 128 x 128, two register sets (loads two K-steps ahead).
 // BQ: the B operand (col) is an 8-bit activation checkpoint (ckpt8.hip): codes [K][ldb] int8 and one step byte per 64
 // columns.  A thread takes 16 codes with one 16-byte load, half the bytes of the bf16 operand, and takes them apart on the
@@ -94,8 +97,15 @@ enum { EPI_SLAB = 0, EPI_DIRECT = 1, EPI_ADAMW = 2 };
 template <bool A_COL, bool B_COL, int EPI, int NW = 4, bool BQ = false, typename CT = float>
 __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   constexpr bool DIRECT = EPI == EPI_DIRECT;
+  constexpr bool DMA = NW == 8;
   constexpr int NJ = NW == 4 ? 4 : 2, WN = 32 * NJ, CH = 32 / NW, LSTEP = 1024 * NW, NSET = NW == 4 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  // two objects: the compiler then sees that a stage's reads need not wait for the loads on their way into the other
+  __shared__ __attribute__((aligned(1024))) unsigned char stage0[DMA ? STAGE_BYTES : 1], stage1[DMA ? STAGE_BYTES : 1];
+  auto stage_of = [&](int stage) -> unsigned char* {
+    if constexpr (DMA) return stage ? stage1 : stage0;
+    return smem + stage * STAGE_BYTES;
+  };
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = NW == 4 ? wave >> 1 : wave >> 2, wn = NW == 4 ? wave & 1 : wave & 3;
 
@@ -132,8 +142,11 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   // chunk c = tid + 256 i.  row image: row (tid >> 3) + 32 i, chunk tid & 7; col image: k row (tid >> 5) + 8 i,
   // chunk tid & 31: the global offset and the LDS offset of chunk i are those of chunk 0 plus i times a constant
   const int Kp = (g.K + 7) & ~7;
-  const int rA = A_COL ? (tid >> 5) : (tid >> 3), cA = A_COL ? (tid & 31) : (tid & 7);
-  const int rB = B_COL ? (tid >> 5) : (tid >> 3), cB = B_COL ? (tid & 31) : (tid & 7);
+  // DMA: the chunk that belongs at LDS slot tid of the image, which the swizzle maps from the slot
+  const int rA = A_COL ? (tid >> 5) : (tid >> 3), rB = B_COL ? (tid >> 5) : (tid >> 3);
+  const int dR = (tid & 7) ^ ((tid >> 4) & 7), dC = (tid & 31) ^ (((tid >> 5) & 3) << 2);
+  const int cA = A_COL ? (DMA ? dC : tid & 31) : (DMA ? dR : tid & 7);
+  const int cB = B_COL ? (DMA ? dC : tid & 31) : (DMA ? dR : tid & 7);
   const unsigned baseA = A_COL ? (unsigned)(((long)rA * g.lda + m0 + 8 * cA) * 2) : (unsigned)(((long)(m0 + rA) * g.lda + 8 * cA) * 2);
   const unsigned baseB = B_COL ? (unsigned)(((long)rB * g.ldb + n0 + 8 * cB) * 2) : (unsigned)(((long)(n0 + rB) * g.ldb + 8 * cB) * 2);
   const unsigned stepA = (unsigned)((A_COL ? 8 : 32) * (NW / 4) * g.lda * 2), stepB = (unsigned)((B_COL ? 8 : 32) * (NW / 4) * g.ldb * 2);
@@ -155,17 +168,27 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   const unsigned baseQ = (unsigned)((long)rQ * g.ldb + n0 + 16 * cQ), baseS = (unsigned)((long)rQ * (g.ldb >> 6) + ((n0 + 16 * cQ) >> 6));
   unsigned qs[2];
 
-  // two register sets: the loads of K-step kt + 2 are issued during step kt and stored to LDS during step kt + 1,
+  // NW 4, two register sets: the loads of K-step kt + 2 are issued during step kt and stored to LDS during step kt + 1,
   // so a load has more than a whole K-step (64 MFMAs) to arrive
   u32x4 ra[NSET][CH], rb[NSET][CH];
-  auto load_tiles = [&](int kt, int set) {       // kt >= kt1: out of range, zeros
+  typedef __attribute__((address_space(3))) void lds_v;
+  const int wave_u = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto load_tiles = [&](int kt, int set, int stage) {       // kt >= kt1: out of range, zeros
     const int k0 = (BQ ? kt - kt0 : kt) * TK;
     const unsigned dead = (kt < kt1 ? 0u : OOR) | g.dbg_oor;
     const unsigned kA = (A_COL ? (unsigned)((long)k0 * g.lda * 2) : ((k0 + 8 * cA < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
     const unsigned kB = (B_COL ? (unsigned)((long)k0 * g.ldb * 2) : ((k0 + 8 * cB < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
-    if constexpr (BQ) {
+    if constexpr (DMA) {
+      unsigned char* ia = stage_of(stage) + wave_u * 1024;
+      unsigned char* ib = ia + TM * TK * 2;
 #pragma unroll
-      for (int i = 0; i < CH; i++) ra[set][i] = ld128(rsA, offA[i] + kA);
+      for (int i = 0; i < CH; i++) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_v*)(ia + LSTEP * i), 16, (int)(offA[i] + kA), 0, 0, 0);
+        if constexpr (!BQ) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_v*)(ib + LSTEP * i), 16, (int)(offB[i] + kB), 0, 0, 0);
+      }
+      if constexpr (!BQ) return;
+    }
+    if constexpr (BQ) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const unsigned kq = (unsigned)(k0 + 32 * i);
@@ -181,11 +204,10 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     }
   };
   auto store_tiles = [&](int stage, int set) {
-    unsigned char* ia = smem + stage * STAGE_BYTES;
+    if constexpr (DMA && !BQ) return;
+    unsigned char* ia = stage_of(stage);
     unsigned char* ib = ia + TM * TK * 2;
     if constexpr (BQ) {
-#pragma unroll
-      for (int i = 0; i < CH; i++) *(u32x4*)(ia + ldsA0 + LSTEP * i) = ra[set][i];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const float step = q8_step(qs[i]), off = -128.f * step;
@@ -219,7 +241,7 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
 
   bf16x8 fa[2][4], fb[2][NJ];
   auto read_frags = [&](int stage, int s, int set) {
-    const unsigned char* ia = smem + stage * STAGE_BYTES;
+    const unsigned char* ia = stage_of(stage);
     const unsigned char* ib = ia + TM * TK * 2;
 #pragma unroll
     for (int i = 0; i < 4; i++) fa[set][i] = read_frag<A_COL>(ia, wm * 128 + 32 * i, s, lane);
@@ -236,9 +258,11 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   constexpr int MFMA = 0x008, VMEM_RD = 0x020, DS_RD = 0x100, DS_WR = 0x200;
   constexpr int RD_A = A_COL ? 2 : 1, RD_B = B_COL ? 2 : 1;     // LDS reads per fragment
 
-  load_tiles(kt0, 0);
+  constexpr int VMCNT0 = 0x0f70;      // s_waitcnt vmcnt(0): this wave's part of the other stage has arrived
+  load_tiles(kt0, 0, 0);
   store_tiles(0, 0);
-  if (NSET == 2) load_tiles(kt0 + 1, 1);
+  if (NSET == 2) load_tiles(kt0 + 1, 1, 1);
+  if (DMA) __builtin_amdgcn_s_waitcnt(VMCNT0);
   __syncthreads();
   // One K-step = four MFMA groups of 4 x NJ products.  The fragments of group s + 1 are read while group s multiplies,
   // the global loads of a later step (kt + 2 with two register sets, kt + 1 with one) are spread over group 0 and the
@@ -259,7 +283,7 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   __builtin_amdgcn_sched_barrier(0);
   auto k_step = [&](int kt, int stage, int set_ld, int set_st) {
     read_frags(stage, 0, 0);
-    load_tiles(kt + NSET, set_ld);
+    load_tiles(kt + NSET, set_ld, stage ^ 1);
     read_frags(stage, 1, 1);
     products(0);
     WG_SCHED(true)
@@ -276,6 +300,7 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
       __builtin_amdgcn_sched_group_barrier(DS_WR, 1, 0);
       __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
     }
+    if (DMA) __builtin_amdgcn_s_waitcnt(VMCNT0);
     __syncthreads();
   };
 #undef WG_SCHED
@@ -380,7 +405,7 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     typedef CT ct4 __attribute__((ext_vector_type(4), aligned(2)));
     typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
     CT* C16 = (CT*)(void*)g.C;
-    float* wt = (float*)smem + wave * (32 * LD);
+    float* wt = (float*)stage_of(wave >> 2) + (wave & 3) * (32 * LD);
     const int c4 = (lane & 15) * 4, n = n0 + wn * WN + c4;
     const bool whole = n + 4 <= g.N;
     f32x4 bn = {0.f, 0.f, 0.f, 0.f};
@@ -556,7 +581,6 @@ int launch(const WgArgs& g, hipStream_t st) {
   static uint64_t done_d = 0, done_s = 0;
   const int total = g.tiles_m * g.tiles_n * g.nsplit;
   const unsigned grid = (unsigned)(((total + 7) / 8) * 8);
-  static uint64_t done_d8 = 0, done_s8 = 0;
   // eight waves by default (measured 2-10 % faster than four on every shape of the wide layers, same box, back to
   // back); SCPAIR_WGEMM_NW=4 selects the four-wave form for comparison
   const char* e8 = getenv("SCPAIR_WGEMM_NW");
@@ -570,13 +594,9 @@ int launch(const WgArgs& g, hipStream_t st) {
     if (rc) return rc;
     hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI_SLAB>), dim3(grid), dim3(256), 2 * STAGE_BYTES, st, g);
   } else if (g.nsplit == 1) {
-    int rc = scp_set_smem((const void*)wgemm_kernel<AC, BC, EPI_DIRECT, 8>, 2 * STAGE_BYTES, &done_d8);
-    if (rc) return rc;
-    hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI_DIRECT, 8>), dim3(grid), dim3(512), 2 * STAGE_BYTES, st, g);
+    hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI_DIRECT, 8>), dim3(grid), dim3(512), 0, st, g);
   } else {
-    int rc = scp_set_smem((const void*)wgemm_kernel<AC, BC, EPI_SLAB, 8>, 2 * STAGE_BYTES, &done_s8);
-    if (rc) return rc;
-    hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI_SLAB, 8>), dim3(grid), dim3(512), 2 * STAGE_BYTES, st, g);
+    hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI_SLAB, 8>), dim3(grid), dim3(512), 0, st, g);
   }
   SCP_LAUNCH_CHECK();
   return SCP_OK;
@@ -585,12 +605,8 @@ int launch(const WgArgs& g, hipStream_t st) {
 // eight-wave forms with a bf16 output and / or an 8-bit B operand
 template <bool AC, bool BC, int EPI, bool BQ, typename CT>
 int launch8(const WgArgs& g, hipStream_t st) {
-  static uint64_t done = 0;
-  const void* fn = (const void*)wgemm_kernel<AC, BC, EPI, 8, BQ, CT>;
-  if (int rc = scp_set_smem(fn, 2 * STAGE_BYTES, &done)) return rc;
   const int total = g.tiles_m * g.tiles_n * g.nsplit;
-  hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI, 8, BQ, CT>), dim3((unsigned)(((total + 7) / 8) * 8)), dim3(512), 2 * STAGE_BYTES,
-                     st, g);
+  hipLaunchKernelGGL((wgemm_kernel<AC, BC, EPI, 8, BQ, CT>), dim3((unsigned)(((total + 7) / 8) * 8)), dim3(512), 0, st, g);
   SCP_LAUNCH_CHECK();
   return SCP_OK;
 }
