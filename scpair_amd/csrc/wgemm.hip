@@ -57,6 +57,18 @@ __device__ __forceinline__ u32x4 ld128(__amdgpu_buffer_rsrc_t rsrc, unsigned vof
   return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)voff, 0, 0);
 }
 
+// 16 bytes per lane from memory into LDS, lane l's at lds + 16 l (lds: the same in all lanes).  In assembly because the compiler
+// lets no transposing LDS read pass such a load in flight (it waits for it, whichever buffer either one works on); whoever
+// issues it waits (vmcnt) and passes a barrier before the bytes are read.  The load has no output register.
+__device__ __forceinline__ void ld128_lds(u32x4 rsrc, unsigned lds, unsigned voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
+}
+__device__ __forceinline__ u32x4 rsrc_of(const void* p, unsigned bytes) {
+  const uint64_t a = (uint64_t)p;
+  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(a >> 32)),
+               (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+
 // LDS byte offsets inside an operand image
 // (rows r and r + 1 lie in the two halves of a 256-byte bank row, so the swizzle runs over r >> 1: the 16 lanes that
 // a ds_read_b128 serves together then touch 16 distinct 16-byte slots)
@@ -85,9 +97,9 @@ __device__ __forceinline__ bf16x8 read_frag(const unsigned char* img, int r0, in
 enum { EPI_SLAB = 0, EPI_DIRECT = 1, EPI_ADAMW = 2 };
 
 // NW = 8 (default for the plain products): two waves per SIMD, wave tile 128 x 64; one wave's MFMA groups cover the other's
-// waits, and the next K-step's tiles go from memory to LDS without passing through registers (a lane's 16 bytes land at
-// LDS slot `lane` of its wave's KB, so the swizzle is applied to what the lane fetches; 16384 x 4096 x 4096 bf16: rows with
-// rows 437 us against 516 us through registers, 1258 TFLOP/s; rows with columns 499 against 512).  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
+// waits, and the tiles go from memory to LDS without passing through registers (a lane's 16 bytes land at LDS slot `lane` of
+// its wave's KB, so the swizzle is applied to what the lane fetches).  16384 x 4096 x 4096 bf16: 426 us (1290 TFLOP/s) with
+// rows or columns for B; 516 and 512 us through registers, 437 and 499 us with the barrier at the step's end.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
 // elsewhere): one wave per SIMD, wave tile 128 x 128, two register sets (loads two K-steps ahead).
 // BQ: the B operand (col) is an 8-bit activation checkpoint (ckpt8.hip): codes [K][ldb] int8 and one step byte per 64
 // columns.  A thread takes 16 codes with one 16-byte load, half the bytes of the bf16 operand, and takes them apart on the
@@ -131,10 +143,12 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   // BQ: first row and rows of this K-range
   const long krow0 = BQ ? (long)kt0 * TK : 0;
   const long krows = min((long)g.K - krow0, (long)(kt1 - kt0) * TK);
-  const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(g.A + krow0 * g.lda), 0, BQ ? (int)(((krows - 1) * g.lda + ((g.M + 7) & ~7)) * 2) : (int)g.a_bytes, 0x00020000);
+  const void* pA = g.A + krow0 * g.lda;
+  const unsigned bytesA = BQ ? (unsigned)(((krows - 1) * g.lda + ((g.M + 7) & ~7)) * 2) : g.a_bytes;
+  const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc((void*)pA, 0, (int)bytesA, 0x00020000);
   const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc(
       BQ ? (void*)((const int8_t*)g.B + krow0 * g.ldb) : (void*)g.B, 0, BQ ? (int)(krows * g.ldb) : (int)g.b_bytes, 0x00020000);
+  const u32x4 dmaA = rsrc_of(pA, bytesA), dmaB = rsrc_of(g.B, g.b_bytes);
   const __amdgpu_buffer_rsrc_t rsS = __builtin_amdgcn_make_buffer_rsrc(
       BQ ? (void*)(g.steps + krow0 * (g.ldb >> 6)) : (void*)g.B, 0, BQ ? (int)(krows * (g.ldb >> 6)) : 0, 0x00020000);
   constexpr unsigned OOR = 0x80000000u;     // beyond any operand (host checks bytes < 2 GiB): the load returns zeros
@@ -171,23 +185,25 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   // NW 4, two register sets: the loads of K-step kt + 2 are issued during step kt and stored to LDS during step kt + 1,
   // so a load has more than a whole K-step (64 MFMAs) to arrive
   u32x4 ra[NSET][CH], rb[NSET][CH];
-  typedef __attribute__((address_space(3))) void lds_v;
-  const int wave_u = __builtin_amdgcn_readfirstlane(tid >> 6);
-  auto load_tiles = [&](int kt, int set, int stage) {       // kt >= kt1: out of range, zeros
+  const unsigned wave_kb = (unsigned)__builtin_amdgcn_readfirstlane(tid >> 6) * 1024u;
+  auto lds_of = [&](int stage) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)stage_of(stage) + wave_kb; };
+  auto k_off = [&](int kt, unsigned& kA, unsigned& kB) {       // kt >= kt1: out of range, zeros
     const int k0 = (BQ ? kt - kt0 : kt) * TK;
     const unsigned dead = (kt < kt1 ? 0u : OOR) | g.dbg_oor;
-    const unsigned kA = (A_COL ? (unsigned)((long)k0 * g.lda * 2) : ((k0 + 8 * cA < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
-    const unsigned kB = (B_COL ? (unsigned)((long)k0 * g.ldb * 2) : ((k0 + 8 * cB < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
-    if constexpr (DMA) {
-      unsigned char* ia = stage_of(stage) + wave_u * 1024;
-      unsigned char* ib = ia + TM * TK * 2;
-#pragma unroll
-      for (int i = 0; i < CH; i++) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_v*)(ia + LSTEP * i), 16, (int)(offA[i] + kA), 0, 0, 0);
-        if constexpr (!BQ) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_v*)(ib + LSTEP * i), 16, (int)(offB[i] + kB), 0, 0, 0);
-      }
-      if constexpr (!BQ) return;
-    }
+    kA = (A_COL ? (unsigned)((long)k0 * g.lda * 2) : ((k0 + 8 * cA < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
+    kB = (B_COL ? (unsigned)((long)k0 * g.ldb * 2) : ((k0 + 8 * cB < Kp) ? (unsigned)k0 * 2u : OOR)) | dead;
+  };
+  // chunk i of both operands into a stage
+  auto dma = [&](int stage, int i, unsigned kA, unsigned kB) {
+    const unsigned to = lds_of(stage) + LSTEP * i;
+    ld128_lds(dmaA, to, offA[i] + kA);
+    if constexpr (!BQ) ld128_lds(dmaB, to + TM * TK * 2, offB[i] + kB);
+  };
+  auto load_tiles = [&](int kt, int set) {       // into registers
+    const int k0 = (BQ ? kt - kt0 : kt) * TK;
+    const unsigned dead = (kt < kt1 ? 0u : OOR) | g.dbg_oor;
+    unsigned kA, kB;
+    k_off(kt, kA, kB);
     if constexpr (BQ) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
@@ -204,7 +220,6 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     }
   };
   auto store_tiles = [&](int stage, int set) {
-    if constexpr (DMA && !BQ) return;
     unsigned char* ia = stage_of(stage);
     unsigned char* ib = ia + TM * TK * 2;
     if constexpr (BQ) {
@@ -243,47 +258,115 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
   auto read_frags = [&](int stage, int s, int set) {
     const unsigned char* ia = stage_of(stage);
     const unsigned char* ib = ia + TM * TK * 2;
+    auto read_b = [&] {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) fb[set][j] = read_frag<B_COL>(ib, wn * WN + 32 * j, s, lane);
+    };
+    if (NW == 8) read_b();        // in the order of their use
 #pragma unroll
     for (int i = 0; i < 4; i++) fa[set][i] = read_frag<A_COL>(ia, wm * 128 + 32 * i, s, lane);
-#pragma unroll
-    for (int j = 0; j < NJ; j++) fb[set][j] = read_frag<B_COL>(ib, wn * WN + 32 * j, s, lane);
+    if (NW == 4) read_b();
   };
+  auto product = [&](int set, int q) { acc[q / NJ][q % NJ] = mfma32(fa[set][q / NJ], fb[set][q % NJ], acc[q / NJ][q % NJ]); };
   auto products = [&](int set) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int j = 0; j < NJ; j++) acc[i][j] = mfma32(fa[set][i], fb[set][j], acc[i][j]);
+    for (int q = 0; q < 4 * NJ; q++) product(set, q);
   };
   // instruction classes of __builtin_amdgcn_sched_group_barrier
   constexpr int MFMA = 0x008, VMEM_RD = 0x020, DS_RD = 0x100, DS_WR = 0x200;
   constexpr int RD_A = A_COL ? 2 : 1, RD_B = B_COL ? 2 : 1;     // LDS reads per fragment
 
   constexpr int VMCNT0 = 0x0f70;      // s_waitcnt vmcnt(0): this wave's part of the other stage has arrived
-  load_tiles(kt0, 0, 0);
-  store_tiles(0, 0);
-  if (NSET == 2) load_tiles(kt0 + 1, 1, 1);
-  if (DMA) __builtin_amdgcn_s_waitcnt(VMCNT0);
+  if constexpr (!DMA || BQ) {
+    load_tiles(kt0, 0);
+    store_tiles(0, 0);
+  }
+  if constexpr (DMA) {
+    unsigned kA, kB;
+    k_off(kt0, kA, kB);
+#pragma unroll
+    for (int i = 0; i < CH; i++) dma(0, i, kA, kB);
+    __builtin_amdgcn_s_waitcnt(VMCNT0);
+  } else {
+    load_tiles(kt0 + 1, 1);
+  }
   __syncthreads();
-  // One K-step = four MFMA groups of 4 x NJ products.  The fragments of group s + 1 are read while group s multiplies,
-  // the global loads of a later step (kt + 2 with two register sets, kt + 1 with one) are spread over group 0 and the
-  // LDS stores of step kt + 1's tiles over group 3 (the other stage: nobody reads it before the barrier), so the
-  // matrix pipe always has the next group's operands in registers.  Two steps per trip (static register sets); an
-  // odd range runs one step on zero tiles.
+  if constexpr (DMA) {
+    unsigned kA, kB;
+    k_off(kt0 + 1, kA, kB);
+#pragma unroll
+    for (int i = 0; i < CH; i++) dma(1, i, kA, kB);
+    if constexpr (BQ) load_tiles(kt0 + 1, 0);
+    read_frags(0, 0, 0);
+  }
+  // One K-step = four MFMA groups of 4 x NJ products, the fragments of the next group being read while a group multiplies.
+  // Two steps per trip; an odd range runs one step on zero tiles.
+  // NW 4: the global loads of step kt + 2 are spread over group 0 and the LDS stores of step kt + 1's tiles over group 3 (the
+  // other stage: nobody reads it before the barrier at the step's end).
+  // NW 8: the barrier stands before group 3, whose fragments are in registers by then: step kt + 1's tiles have arrived and
+  // nobody reads step kt's any more, so group 3 hides the first reads of the one and the loads of step kt + 2 into the other.
+  // A group's reads go out over its first three products: spread over all eight, the next group's first product waits for them.
 #define WG_SCHED(VM)                                                                 \
   _Pragma("unroll") for (int t = 0; t < 4; t++) {                                    \
     if (VM) __builtin_amdgcn_sched_group_barrier(VMEM_RD, 2, 0);                     \
     __builtin_amdgcn_sched_group_barrier(DS_RD, RD_A, 0);                            \
-    __builtin_amdgcn_sched_group_barrier(MFMA, NJ == 4 ? 2 : 1, 0);                  \
+    __builtin_amdgcn_sched_group_barrier(MFMA, 2, 0);                                \
   }                                                                                  \
   _Pragma("unroll") for (int t = 0; t < NJ; t++) {                                   \
-    if (VM && NJ == 4) __builtin_amdgcn_sched_group_barrier(VMEM_RD, 2, 0);          \
+    if (VM) __builtin_amdgcn_sched_group_barrier(VMEM_RD, 2, 0);                     \
     __builtin_amdgcn_sched_group_barrier(DS_RD, RD_B, 0);                            \
     __builtin_amdgcn_sched_group_barrier(MFMA, 2, 0);                                \
   }                                                                                  \
   __builtin_amdgcn_sched_barrier(0);
+  constexpr int RD = (4 * RD_A + NJ * RD_B + 2) / 3;
+#define WG_SCHED8                                                                    \
+  _Pragma("unroll") for (int t = 0; t < 3; t++) {                                    \
+    __builtin_amdgcn_sched_group_barrier(DS_RD, RD, 0);                              \
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);                                \
+  }                                                                                  \
+  _Pragma("unroll") for (int t = 0; t < 4; t++) {                                    \
+    if (BQ) __builtin_amdgcn_sched_group_barrier(DS_WR, 1, 0);                       \
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);                                \
+  }                                                                                  \
+  __builtin_amdgcn_sched_barrier(0);
   auto k_step = [&](int kt, int stage, int set_ld, int set_st) {
+    if constexpr (DMA) {
+      read_frags(stage, 1, 1);
+      products(0);
+      WG_SCHED8
+      read_frags(stage, 2, 0);
+      products(1);
+      WG_SCHED8
+      if constexpr (BQ) store_tiles(stage ^ 1, 0);
+      read_frags(stage, 3, 1);
+      products(0);
+      WG_SCHED8
+      __builtin_amdgcn_s_waitcnt(VMCNT0);
+      __syncthreads();
+      unsigned kA, kB;
+      k_off(kt + 2, kA, kB);
+      read_frags(stage ^ 1, 0, 0);
+      if constexpr (BQ) load_tiles(kt + 2, 0);
+#pragma unroll
+      for (int q = 0; q < 3; q++) product(1, q);
+#pragma unroll
+      for (int t = 0; t < 3; t++) {
+        __builtin_amdgcn_sched_group_barrier(DS_RD, RD, 0);
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        dma(stage, i, kA, kB);
+        product(1, 3 + i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      product(1, 7);
+      __builtin_amdgcn_sched_barrier(0);
+      return;
+    }
     read_frags(stage, 0, 0);
-    load_tiles(kt + NSET, set_ld, stage ^ 1);
+    load_tiles(kt + NSET, set_ld);
     read_frags(stage, 1, 1);
     products(0);
     WG_SCHED(true)
@@ -300,15 +383,19 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
       __builtin_amdgcn_sched_group_barrier(DS_WR, 1, 0);
       __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
     }
-    if (DMA) __builtin_amdgcn_s_waitcnt(VMCNT0);
     __syncthreads();
   };
 #undef WG_SCHED
+#undef WG_SCHED8
   for (int kt = kt0; kt < kt1; kt += 2) {
     k_step(kt, 0, 0, NSET - 1);
     k_step(kt + 1, 1, NSET - 1, 0);
   }
 
+  if (DMA) {       // the loads past the last step, before the stages get another use or another owner
+    __builtin_amdgcn_s_waitcnt(VMCNT0);
+    __syncthreads();
+  }
   // epilogue: accumulator element e of lane l is row acc_row(e, l), column l & 31 of its 32 x 32 tile
   if constexpr (EPI == EPI_ADAMW) {
     static_assert(NW == 4, "the AdamW epilogue is written for the four-wave tile");
