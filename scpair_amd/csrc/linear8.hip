@@ -637,9 +637,10 @@ struct Gemm {
 // product's own time only; a launch 3.5, slabs written and read at 7.5 TB/s, prepared operands at 5).
 double step_us(int ts, int pairs, double w) {
   if (ts == 64) return pairs == 1 ? 0.25 + 0.2 * w : pairs == 3 ? 0.5 + 0.48 * w : 0.5 + 0.85 * w;
-  if (ts == 128) return w == 1 ? 1.15 : 0.7 * w;
-  return 2.3 * w;
+  return w == 1 ? 1.15 : 0.7 * w;
 }
+// the wide kernel's: rows of both operands or columns of W; the weight gradient, which takes codes apart
+const double WIDE_ROWS_US = 1.7, WIDE_Q8_US = 1.9;
 const double LAUNCH_US = 3.5;
 
 void consider(Gemm& best, int ts, int pairs, long M, int N, long K, int planes) {
@@ -667,13 +668,13 @@ Gemm pick_direct(long M, int N, long K, int pairs) {
 }
 
 // on prepared operands, of which `planes` column blocks are summed up apart
-Gemm pick_blocks(long M, int N, long K, int planes, bool wide_ok, long wide_ws) {
+Gemm pick_blocks(long M, int N, long K, int planes, bool wide_ok, long wide_ws, double wide_us) {
   Gemm best = {0, 1, 0, 0, 1e30};
   if (wide_ok) {
     const long nk = (K + 63) / 64;
     const int ns = scp_gemm_bf16_nsplit((int)M, N, (int)K);
     const double mn = (double)M * N, w = (double)((((M + 255) / 256) * ((N + 255) / 256) * ns + 255) / 256);
-    double us = planes * (LAUNCH_US + step_us(256, 1, w) * ((nk + ns - 1) / ns));
+    double us = planes * (LAUNCH_US + wide_us * w * ((nk + ns - 1) / ns));
     if (ns > 1) us += planes * (mn * 4 * (2 * ns + 1) / 7.5e6 + LAUNCH_US);
     if (planes > 1) us += mn * 4 * (2 * planes + 1) / 7.5e6 + LAUNCH_US;
     best = {256, 1, 0, wide_ws, us};
@@ -724,7 +725,7 @@ Plan plan_fwd(const ScpLinear8& a) {
   const int xb = a.x_bf16 ? 2 : 4, wb = a.w_bf16 ? 2 : 4;
   const long KK = p.np == 1 ? a.K : (long)p.np * p.Kp, ld = (long)p.np * p.Kp;
   const bool ok = ((long)a.N + 192) * ld * 2 < WIDE_BYTES;
-  Gemm blocks = pick_blocks(a.M, a.N, KK, 1, ok, ok ? wide_ws_rows(a.M, a.N, KK, p.x_direct ? a.ldx : ld) : 0);
+  Gemm blocks = pick_blocks(a.M, a.N, KK, 1, ok, ok ? wide_ws_rows(a.M, a.N, KK, p.x_direct ? a.ldx : ld) : 0, WIDE_ROWS_US);
   if (!p.x_direct) blocks.us += prep_us((double)a.M * a.K, xb, p.np) - LAUNCH_US;    // else packing is a launch of its own
   if (!p.w_direct) blocks.us += prep_us((double)a.N * a.K, wb, p.np);
   Gemm direct = pick_direct(a.M, a.N, a.K, p.np);
@@ -755,13 +756,14 @@ Plan plan_bwd(const ScpLinear8& a) {
   // Each product straight from the tensors or on prepared operands: the cheapest combination, dy being prepared once for both.
   // Chosen as if all gradients were asked for, so that none depends on the others being wanted.
   const bool ok = (K2 + 192) * p.Kp * 2 < WIDE_BYTES;
-  Gemm xb_ = pick_blocks(a.M, a.K, K2, 1, ok, ok ? wide_ws_rows(a.M, a.K, K2, lda) : 0);
+  Gemm xb_ = pick_blocks(a.M, a.K, K2, 1, ok, ok ? wide_ws_rows(a.M, a.K, K2, lda) : 0, WIDE_ROWS_US);
   if (!p.w_direct) xb_.us += prep_us((double)a.N * a.K, wb, p.np);
   Gemm xd = pick_direct(a.M, a.K, a.N, p.np);
   if (!direct_rows_ok(a.lddy) || a.K < 8) xd.us = 1e30;
   // the wide form of dW runs once per plane, each into a slab of its own
   const long ld8 = (a.K + 63) / 64 * 64L, wide_ws = scp_gemm_q8_ws_floats(a.N, a.K, (int)a.M, lda > ld8 ? lda : ld8, a.K) * 4;
-  const Gemm wb_ = pick_blocks(a.N, a.K, a.M, planes, lda <= MAX_LD, align256(wide_ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0));
+  const Gemm wb_ = pick_blocks(a.N, a.K, a.M, planes, lda <= MAX_LD, align256(wide_ws) + (planes > 1 ? 3L * a.N * a.K * 4 : 0),
+                               WIDE_Q8_US);
   Gemm wd = pick_direct(a.N, a.K, a.M, planes);
   if (!direct_rows_ok(a.lddy) || a.lddy < a.N || a.N < 8) wd.us = 1e30;
   double best = 1e300;

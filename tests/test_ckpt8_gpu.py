@@ -430,3 +430,43 @@ def test_linear8_rows_far_apart(M, apart):
         assert ((ops.linear8(far, W).cpu().double() - want).abs() <= bound(xd, Wd.t(), 64) + half_step(want, B16)).all()
     p, q = ops.pack8(far), ops.pack8(rows)
     assert torch.equal(p.codes, q.codes) and torch.equal(p.steps, q.steps)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (7, 9, 200), (256, 256, 64), (300, 517, 65), (257, 255, 129), (513, 264, 4097),
+                                   (1000, 777, 1000)])
+def test_wide_products_at_any_size(M, N, K):
+    """The three forms of the wide kernel that linear8 uses for large batches, at sizes that end inside its tiles and K-steps."""
+    from scpair_amd import _lib, ops
+    L = _lib.lib()
+    up = lambda n: (n + 7) // 8 * 8
+    g = torch.Generator().manual_seed(M + N + K)
+    A, W = torch.zeros(M, up(K), dtype=B16), torch.zeros(N, up(K), dtype=B16)
+    A[:, :K], W[:, :K] = torch.randn(M, K, generator=g).to(B16), torch.randn(N, K, generator=g).to(B16)
+    Wc = torch.full((K, up(N)), 7.0, dtype=B16)                   # columns behind N are read, but never used
+    Wc[:, :N] = W[:, :K].t()
+    bias = torch.randn(N, generator=g)
+    x = torch.randn(K, N, generator=g).to(B16)
+    dy = torch.full((K, up(M)), 7.0, dtype=B16)
+    dy[:, :M] = A[:, :K].t()
+    a, w, wc, b, d = (t.cuda() for t in (A, W, Wc, bias, dy))
+    p = ops.pack8(x.cuda())
+    ad = A[:, :K].double()
+    for c16 in (1, 0):
+        ws = torch.empty(max(L.scp_gemm_bf16_ws_floats(M, N, K, N), L.scp_gemm_q8_ws_floats(M, N, K, max(up(M), p.codes.shape[1]), N), 1),
+                         device="cuda")
+        for col in (0, 1, 2):
+            out = torch.full((M + 1, N), 3.0, dtype=B16 if c16 else F32, device="cuda")
+            if col == 2:
+                rc = L.scp_gemm_q8(M, N, K, d.data_ptr(), up(M), p.codes.data_ptr(), p.steps.data_ptr(), out.data_ptr(), c16, N,
+                                   ws.data_ptr(), _lib.stream())
+                right, add = pack_ref(x)[2], 0.0
+            else:
+                o = wc if col else w
+                rc = L.scp_gemm_rows(col, M, N, K, a.data_ptr(), a.stride(0), o.data_ptr(), o.stride(0), out.data_ptr(), c16, N,
+                                     b.data_ptr(), ws.data_ptr(), _lib.stream())
+                right, add = W[:, :K].double().t(), bias.double()
+            assert rc == 0
+            want = ad @ right + add
+            err = bound(ad, right, K) + E * want.abs() * 2 + (half_step(want, B16) * 1.01 if c16 else 0)
+            assert ((out[:M].cpu().double() - want).abs() <= err).all(), (col, c16)
+            assert (out[M] == 3.0).all()
