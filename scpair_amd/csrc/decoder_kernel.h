@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
       // Bernoulli, interior tile with 0/1 labels only: no bounds / NaN / soft-label handling (same algebra)
       const bool ber_fast = IS_BER && (f0 + FT <= g.F) && (c0 + CB <= g.B) && (tflag == 0);
       if (ber_fast) {
-        // Straight line over pairs of elements (the compiler packs them into v_pk_* forms).  Deferred to the points where
+        // Straight line over pairs of elements (two independent chains of sums).  Deferred to the points where
         // the sums leave the workgroup: the 1 / n of the mean (inv_n) and the (1 - sr) of the per-cell gradient; the
         // likelihood is summed in log2 units (one v_log per element, no product) and scaled once per tile; bias and
         // the -log2(e) of the exponential share one fma.
