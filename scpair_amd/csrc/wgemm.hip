@@ -59,9 +59,10 @@ __device__ __forceinline__ u32x4 ld128(__amdgpu_buffer_rsrc_t rsrc, unsigned vof
 
 // 16 bytes per lane from memory into LDS, lane l's at lds + 16 l (lds: the same in all lanes).  In assembly because the compiler
 // lets no transposing LDS read pass such a load in flight (it waits for it, whichever buffer either one works on); whoever
-// issues it waits (vmcnt) and passes a barrier before the bytes are read.  The load has no output register.
+// issues it waits (vmcnt) and passes a barrier before the bytes are read.  The load has no output register.  The wait states in
+// front of it: one behind m0, five behind a vector instruction that wrote the descriptor (the compiler sees neither).
 __device__ __forceinline__ void ld128_lds(u32x4 rsrc, unsigned lds, unsigned voff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
 __device__ __forceinline__ u32x4 rsrc_of(const void* p, unsigned bytes) {
   const uint64_t a = (uint64_t)p;
