@@ -99,8 +99,8 @@ enum { EPI_SLAB = 0, EPI_DIRECT = 1, EPI_ADAMW = 2 };
 
 // NW = 8 (default for the plain products): two waves per SIMD, wave tile 128 x 64; one wave's MFMA groups cover the other's
 // waits, and the tiles go from memory to LDS without passing through registers (a lane's 16 bytes land at LDS slot `lane` of
-// its wave's KB, so the swizzle is applied to what the lane fetches).  16384 x 4096 x 4096 bf16: 426 us (1290 TFLOP/s) with
-// rows or columns for B; 516 and 512 us through registers, 437 and 499 us with the barrier at the step's end.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
+// its wave's KB, so the swizzle is applied to what the lane fetches).  16384 x 4096 x 4096 bf16: 425-445 us (1240-1290 TFLOP/s)
+// with rows or columns for B; 516 and 512 us through registers, 437 and 499 us with the barrier at the step's end.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
 // elsewhere): one wave per SIMD, wave tile 128 x 128, two register sets (loads two K-steps ahead).
 // BQ: the B operand (col) is an 8-bit activation checkpoint (ckpt8.hip): codes [K][ldb] int8 and one step byte per 64
 // columns.  A thread takes 16 codes with one 16-byte load, half the bytes of the bf16 operand, and takes them apart on the
@@ -484,53 +484,56 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     }
     return;
   }
-  if constexpr (sizeof(CT) == 2) {
-    static_assert(DIRECT, "slabs are fp32");
-    // A wave's 32-row strips go through a private LDS buffer (the operand stages are free after the loop's last barrier), so
-    // that 16 lanes write a 128-byte row segment: an accumulator's own layout makes 2-byte stores, 128 of them a lane.
-    static_assert(NW == 8, "strips of 64 columns");
-    constexpr int LD = 72;                      // lanes 32 .. 63 write four rows further down, to the other 32 banks
-    typedef CT ct4 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-    CT* C16 = (CT*)(void*)g.C;
-    float* wt = (float*)stage_of(wave >> 2) + (wave & 3) * (32 * LD);
-    const int c4 = (lane & 15) * 4, n = n0 + wn * WN + c4;
-    const bool whole = n + 4 <= g.N;
-    f32x4 bn = {0.f, 0.f, 0.f, 0.f};
-    if (g.bias) {
-      if (whole) bn = *(const f4u*)(g.bias + n);
-      else
+  if constexpr (NW == 8) {
+    // A wave's 32-row strips go through a private LDS buffer (the operand stages are free by now), so that 16 lanes write a row
+    // segment of 64 columns: an accumulator's own layout makes 2- or 4-byte stores, 128 of them a lane, and registers spill over
+    // their addresses (weight gradient 900 x 20 k over 1024 rows, fp32: 62 against 89 us).
+    if (sizeof(CT) == 2 || !(DIRECT && g.mask)) {
+      static_assert(sizeof(CT) == 4 || DIRECT, "slabs are fp32");
+      constexpr int LD = 72;                      // lanes 32 .. 63 write four rows further down, to the other 32 banks
+      typedef CT ct4 __attribute__((ext_vector_type(4), aligned(sizeof(CT))));
+      typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+      CT* Cs = (CT*)(void*)g.C + (DIRECT ? 0 : (long)z * g.M * g.ldc);
+      float* wt = (float*)stage_of(wave >> 2) + (wave & 3) * (32 * LD);
+      const int c4 = (lane & 15) * 4, n = n0 + wn * WN + c4;
+      const bool whole = n + 4 <= g.N;
+      f32x4 bn = {0.f, 0.f, 0.f, 0.f};
+      if (DIRECT && g.bias) {
+        if (whole) bn = *(const f4u*)(g.bias + n);
+        else
 #pragma unroll
-        for (int t = 0; t < 4; t++) bn[t] = n + t < g.N ? g.bias[n + t] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-#pragma unroll
-      for (int j = 0; j < NJ; j++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) wt[acc_row(e, lane) * LD + 32 * j + (lane & 31)] = acc[i][j][e];
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int it = 0; it < 8; it++) {
-        const int row = 4 * it + (lane >> 4), m = m0 + wm * 128 + 32 * i + row;
-        const f32x4 v = *(const f32x4*)(wt + row * LD + c4) + bn;
-        if (m >= g.M) continue;
-        CT* p = C16 + (long)m * g.ldc + n;
-        if (whole) {
-          ct4 o;
-#pragma unroll
-          for (int t = 0; t < 4; t++) o[t] = (CT)v[t];
-          *(ct4*)p = o;
-        } else {
-#pragma unroll
-          for (int t = 0; t < 4; t++)
-            if (n + t < g.N) p[t] = (CT)v[t];
-        }
+          for (int t = 0; t < 4; t++) bn[t] = n + t < g.N ? g.bias[n + t] : 0.f;
       }
-      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) wt[acc_row(e, lane) * LD + 32 * j + (lane & 31)] = acc[i][j][e];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int it = 0; it < 8; it++) {
+          const int row = 4 * it + (lane >> 4), m = m0 + wm * 128 + 32 * i + row;
+          const f32x4 v = *(const f32x4*)(wt + row * LD + c4) + bn;
+          if (m >= g.M) continue;
+          CT* p = Cs + (long)m * g.ldc + n;
+          if (whole) {
+            ct4 o;
+#pragma unroll
+            for (int t = 0; t < 4; t++) o[t] = (CT)v[t];
+            *(ct4*)p = o;
+          } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+              if (n + t < g.N) p[t] = (CT)v[t];
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      return;
     }
-    return;
   }
+  if constexpr (sizeof(CT) == 2) return;
   float* Cz = g.C + (DIRECT ? 0 : (long)z * g.M * g.ldc);
   if (m0 + TM <= g.M && n0 + TN <= g.N && !(DIRECT && g.mask)) {
     // interior tile: no tests; one store instruction writes two 128-byte row segments
