@@ -376,8 +376,8 @@ long scp_residual_norm_bwd_ws_floats(long rows, int cols);
 int scp_residual_norm_bwd(const ScpResidualNorm* args /* host */, void* stream);
 
 /* ---- 8-bit activation checkpoints (no counterpart in the reference, which keeps every activation in fp32): 64 columns of a
- *      row share a step 2^k, the smallest with max|x| <= 127 * 2^k, -126 <= k <= 121; codes int8 [rows][ld], ld = cols rounded up
- *      to 64 (zeros behind cols); steps uint8 [rows][ld / 64], k + 127 (255: the group held an infinity or a NaN and reads as
+ *      row share a step 2^k, the smallest with max|x| <= 127 * 2^k, -126 <= k <= 121; codes int8 [rows][ld], -127 to 127, ld = cols
+ *      rounded up to 64 (zeros behind cols); steps uint8 [rows][ld / 64], k + 127 (255: the group held an infinity or a NaN and reads as
  *      NaN).  x, out, dout, dx: fp32, or bf16 with `bf16`; inputs with a row stride, any alignment, outputs contiguous; codes
  *      16-byte aligned.  kind 0 gelu (erf), 1 silu, 2 leaky relu; act8_fwd without codes and
  *      steps (both null) writes only out; act8_bwd: dx = dout * act'(values of the codes). ---- */
@@ -417,6 +417,8 @@ typedef struct {
 } ScpLinear8;
 long scp_linear8_fwd_ws(const ScpLinear8* args /* host */);
 long scp_linear8_bwd_ws(const ScpLinear8* args /* host */);
+/* host only: the tile edge (64, 128 or 256) of each product at these sizes, types, strides and alignments: tiles[0] y, [1] dx, [2] dW */
+int scp_linear8_tiles(const ScpLinear8* args /* host */, int* tiles /* host */);
 int scp_linear8_fwd(const ScpLinear8* args /* host */, void* stream);
 int scp_linear8_bwd(const ScpLinear8* args /* host */, void* stream);
 

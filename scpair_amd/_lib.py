@@ -140,6 +140,7 @@ _SIGS = {
     "scp_gemm_q8": (I, [I, I, I, P, L, P, P, P, I, L, P, P]),
     "scp_linear8_fwd_ws": (L, [P]),
     "scp_linear8_bwd_ws": (L, [P]),
+    "scp_linear8_tiles": (I, [P, P]),
     "scp_linear8_fwd": (I, [P, P]),
     "scp_linear8_bwd": (I, [P, P]),
     "scp_step_state_set": (I, [P, U64, F, F, P]),

@@ -8,6 +8,15 @@
 // the step a step byte stands for: 2^(e - 127), NaN for a bad group
 __device__ __forceinline__ float q8_step(unsigned e) { return __uint_as_float(e == SCP_Q8_BAD ? 0x7fc00000u : e << 23); }
 
+// Four codes to bf16 values, for the products that read a checkpoint.  127 - code is the byte's bits but the top one inverted, an
+// unsigned byte that converts in one instruction; the fma's addend 127 * step is finite for every step up to 2^121 (128 * 2^121
+// is not), and its result is exact.
+__device__ __forceinline__ void q8_values(unsigned codes, float step, __bf16* out) {
+  const unsigned u = codes ^ 0x7f7f7f7fu;
+#pragma unroll
+  for (int b = 0; b < 4; b++) out[b] = (__bf16)fmaf((float)((u >> (8 * b)) & 0xffu), -step, 127.f * step);
+}
+
 namespace {
 
 typedef float vf8 __attribute__((ext_vector_type(8)));

@@ -253,13 +253,14 @@ struct Tile {
       if constexpr (OP != OP_Q8) {
         *(u32x4*)(img + lds[i]) = r.v[i];
       } else {
-        const float step = q8_step(r.step[i]), off = -128.f * step;
+        const float step = q8_step(r.step[i]);
         bf16x8 v[2];
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-          const unsigned u = r.v[i][w] ^ 0x80808080u;      // code + 128: unsigned bytes convert in one instruction
+          __bf16 f[4];
+          q8_values(r.v[i][w], step, f);
 #pragma unroll
-          for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = (__bf16)fmaf((float)((u >> (8 * b)) & 0xffu), step, off);
+          for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = f[b];
         }
         *(bf16x8*)(img + lds[i]) = v[0];
         *(bf16x8*)(img + lds[i] + 16) = v[1];
@@ -991,6 +992,16 @@ int check_args(const ScpLinear8* a, const char* who) {
 
 extern "C" long scp_linear8_fwd_ws(const ScpLinear8* a) { return check_args(a, "scp_linear8_fwd") ? -1 : plan_fwd(*a).total; }
 extern "C" long scp_linear8_bwd_ws(const ScpLinear8* a) { return check_args(a, "scp_linear8_bwd") ? -1 : plan_bwd(*a).total; }
+
+extern "C" int scp_linear8_tiles(const ScpLinear8* a, int* tiles) {
+  if (int rc = check_args(a, "scp_linear8_tiles")) return rc;
+  SCP_CHECK(tiles, SCP_ERR_ARG, "scp_linear8_tiles: null pointer");
+  const Plan b = plan_bwd(*a);
+  tiles[0] = plan_fwd(*a).y.ts;
+  tiles[1] = b.dx.ts;
+  tiles[2] = b.dw.ts;
+  return SCP_OK;
+}
 
 extern "C" int scp_linear8_fwd(const ScpLinear8* a_, void* stream) {
   if (int rc = check_args(a_, "scp_linear8_fwd")) return rc;

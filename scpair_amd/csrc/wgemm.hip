@@ -226,13 +226,14 @@ __global__ __launch_bounds__(64 * NW) void wgemm_kernel(WgArgs g) {
     if constexpr (BQ) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const float step = q8_step(qs[i]), off = -128.f * step;
+        const float step = q8_step(qs[i]);
         bf16x8 v[2];
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-          const unsigned u = rb[set][i][w] ^ 0x80808080u;      // code + 128: unsigned bytes convert in one instruction
+          __bf16 f[4];
+          q8_values(rb[set][i][w], step, f);
 #pragma unroll
-          for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = (__bf16)fmaf((float)((u >> (8 * b)) & 0xffu), step, off);
+          for (int b = 0; b < 4; b++) v[w >> 1][(w & 1) * 4 + b] = f[b];
         }
         unsigned char* p = ib + col_off(rQ + 32 * i, 16 * cQ);
         *(bf16x8*)p = v[0];
