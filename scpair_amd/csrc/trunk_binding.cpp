@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "scpair_hip.h"
@@ -52,6 +53,14 @@ variable_list once(variable_list grads, const char* who) {
   return grads;
 }
 
+// A call that needs no backward pass makes no node, and a launch is nothing that torch sees: a forward-mode tangent would get lost,
+// and a trace would keep the call's result as a constant.  Both are refused, whether a node is made or not.
+void visible(const char* who, std::initializer_list<const Tensor*> given) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), who, ": cannot be traced");
+  for (const Tensor* t : given)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), who, ": forward-mode derivatives are not implemented");
+}
+
 // Which forward arguments want a gradient: absent tensors have no edge, so edges are counted along.
 struct Needs {
   AutogradContext* ctx;
@@ -67,6 +76,7 @@ std::pair<Tensor, Tensor> empty_packed(const Tensor& like, int64_t rows, int64_t
 }
 
 std::pair<Tensor, Tensor> pack8(const Tensor& x) {
+  visible("pack8", {});
   c10::DeviceGuard guard(x.device());
   auto p = empty_packed(x, x.size(0), x.size(1));
   check(scp_pack8(ptr(x), is16(x), x.stride(0), x.size(0), (int)x.size(1), ptr<int8_t>(p.first), ptr<uint8_t>(p.second),
@@ -75,6 +85,7 @@ std::pair<Tensor, Tensor> pack8(const Tensor& x) {
 }
 
 Tensor unpack8(const Tensor& codes, const Tensor& steps, int64_t cols, bool bf16) {
+  visible("unpack8", {});
   c10::DeviceGuard guard(codes.device());
   Tensor out = fresh(codes, {codes.size(0), cols}, bf16 ? at::kBFloat16 : at::kFloat);
   check(scp_unpack8(ptr<int8_t>(codes), ptr<uint8_t>(steps), codes.size(0), (int)cols, ptr(out), bf16, stream_of(codes)),
@@ -113,6 +124,7 @@ struct Act8 : torch::autograd::Function<Act8> {
 };
 
 Tensor act8(const Tensor& z, int64_t kind, double slope) {
+  visible("act8", {&z});
   if (at::GradMode::is_enabled() && z.requires_grad()) return Act8::apply(z, kind, slope);
   return act8_forward(z, kind, slope, nullptr, nullptr);
 }
@@ -176,9 +188,11 @@ struct Linear8 : torch::autograd::Function<Linear8> {
 };
 
 Tensor linear8(const Tensor& x, const Tensor& W, const Opt& b, bool split) {
+  const Tensor bias = value(b);
+  visible("linear8", {&x, &W, &bias});
   if (at::GradMode::is_enabled() && (x.requires_grad() || W.requires_grad() || (b.has_value() && b->requires_grad())))
     return Linear8::apply(x, W, b, split, W.requires_grad());
-  return linear8_forward(x, W, value(b), split, nullptr, nullptr);
+  return linear8_forward(x, W, bias, split, nullptr, nullptr);
 }
 
 // ---- gated_residual_norm ----------------------------------------------------------------------------------------------
@@ -294,13 +308,13 @@ std::pair<Opt, Tensor> residual_norm(const Tensor& x, const Opt& h, const Opt& g
                                      const Opt& w2, const Opt& b2, int64_t post, int64_t pre, int64_t gate_mode, int64_t gate_act,
                                      int64_t scale_mode, double scale_value, double eps, bool y16) {
   const NormForm f = {post, pre, gate_mode, gate_act, scale_mode, scale_value, eps, y16};
+  const variable_list t = {x, value(h), value(gate), value(scale), value(w1), value(b1), value(w2), value(b2)};
+  visible("gated_residual_norm", {&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7]});
   bool track = false;
-  if (at::GradMode::is_enabled()) {
-    track = x.requires_grad();
-    for (const Opt* t : {&h, &gate, &scale, &w1, &b1, &w2, &b2}) track = track || (t->has_value() && (*t)->requires_grad());
-  }
+  if (at::GradMode::is_enabled())
+    for (const Tensor& v : t) track = track || (v.defined() && v.requires_grad());
   if (!track) {
-    auto ry = norm_forward({x, value(h), value(gate), value(scale), value(w1), value(b1), value(w2), value(b2)}, f, nullptr);
+    auto ry = norm_forward(t, f, nullptr);
     return {ry.first.defined() ? Opt(ry.first) : std::nullopt, ry.second};
   }
   const variable_list o = ResidualNorm::apply(x, h, gate, scale, w1, b1, w2, b2, f);

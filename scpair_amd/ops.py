@@ -2075,7 +2075,7 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
     under the root.  Weights default to ones, biases to zeros.  y has h's type (h None: out_dtype, x's by default).  At most
     16384 columns, which lie next to each other (other layouts are copied); rows may have any stride.
     Sums and statistics are fp32, every output is rounded once, y is the norm of r before r's rounding; results are bitwise
-    reproducible.  Gradients flow to every tensor given; a second derivative is refused."""
+    reproducible.  Gradients flow to every tensor given; a second derivative, a forward-mode derivative and tracing are refused."""
     if not isinstance(x, torch.Tensor) or x.ndim == 0:
         raise ValueError("gated_residual_norm: x must be a tensor of at least one dimension")
     shape, cols = x.shape, x.shape[-1]
@@ -2203,7 +2203,7 @@ _ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
 
 def act8(z, kind="gelu", slope=0.01):
     """act(z) for z [..., D] float32 or bfloat16, keeping z for the backward pass as an 8-bit checkpoint that the same launch
-    writes: dz = dout * act'(unpack8(pack8(z))).  kind: 'gelu' (the erf form), 'silu', or 'leaky_relu' (slope; 0 is relu; a
+    writes: dz = dout * act'(unpack8(pack8(z))); other derivatives and tracing are refused.  kind: 'gelu' (the erf form), 'silu', or 'leaky_relu' (slope; 0 is relu; a
     value whose code is 0 counts as not positive)."""
     _check_floats("act8", z)
     if kind not in _ACTS8:
@@ -2219,7 +2219,7 @@ def linear8(x, W, b=None):
     """y = x W^T + b for x [..., K], W [N, K], b [N], keeping x for the backward pass as an 8-bit checkpoint: dW = dy^T
     unpack8(pack8(x)), while y, dx and db are what linear gives.  x float32 with W float32: y float32, products in the
     precision of set_precision.  x bfloat16 with W bfloat16 or float32 (rounded once per call): y bfloat16, bf16 products
-    with fp32 sums; dW has W's type.  b may have any floating-point type.  W and its gradient stay below 2 GiB of bf16."""
+    with fp32 sums; dW has W's type.  Other derivatives and tracing are refused.  b may have any floating-point type.  W and its gradient stay below 2 GiB of bf16."""
     _check_floats("linear8", x)
     _check_floats("linear8", W)
     K = x.shape[-1]
