@@ -143,11 +143,12 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], float* red, int& turn) {
   }
 }
 
-// Mean and 1 / spread of a row held as v[NCH][8]; own: 1 for the columns of the last chunk that are this lane's, else 0.
+// Mean and 1 / spread of a row held as v[NCH][8]; own: the columns of the last chunk that are this lane's.  The others are left out
+// by a select: multiplied by 0, an infinity would become NaN.
 // The squares are taken about a mean, never about zero.  A workgroup's row needs one exchange for both: each wave takes its
 // squares about its own mean, and M2 = sum_w M2_w + (sum_w - n_w mean)^2 / n_w, n_w the columns of wave w.
 template <int TPR, int NCH>
-__device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const float (&own)[8], int kind, int D, float inv_d, float eps,
+__device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const bool (&own)[8], int kind, int D, float inv_d, float eps,
                                           float* red, int& turn, float& mean, float& rstd) {
   mean = 0.f;
   float s = 0.f;
@@ -155,7 +156,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const float 
 #pragma unroll
     for (int c = 0; c < NCH; c++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) s += c == NCH - 1 ? v[c][i] * own[i] : v[c][i];
+      for (int i = 0; i < 8; i++) s += c < NCH - 1 || own[i] ? v[c][i] : 0.f;
     s = wsum<(TPR < 64 ? TPR : 64)>(s);
     if constexpr (TPR > 64) {
       mean = s * __builtin_amdgcn_rcpf((float)max(wave_cols<NCH>(threadIdx.x >> 6, D), 1));
@@ -168,8 +169,8 @@ __device__ __forceinline__ void row_stats(const float (&v)[NCH][8], const float 
   for (int c = 0; c < NCH; c++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float e = v[c][i] - mean;
-      q[0] += (c == NCH - 1 ? e * own[i] : e) * e;
+      const float e = c < NCH - 1 || own[i] ? v[c][i] - mean : 0.f;
+      q[0] += e * e;
     }
   if (TPR > 64 && kind == NORM_LAYER) {
     q[0] = wsum(q[0]);
@@ -264,9 +265,9 @@ __global__ __launch_bounds__(threads<TPR>()) void rnorm_fwd_kernel(ScpResidualNo
 #pragma unroll
   for (int c = 0; c < NCH; c++) base[c] = chunk_base(t + nt * c, D);
   const bool last = 8 * (t + nt * (NCH - 1)) < D;     // this lane's last chunk exists; the others always do
-  float own[8];
+  bool own[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) own[i] = chunk_owns(t + nt * (NCH - 1), i, D) ? 1.f : 0.f;
+  for (int i = 0; i < 8; i++) own[i] = chunk_owns(t + nt * (NCH - 1), i, D);
 
   // the next row's values are fetched while this one's sums run
   struct Raw {
@@ -373,9 +374,9 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
 #pragma unroll
   for (int c = 0; c < NCH; c++) base[c] = chunk_base(t + nt * c, D);
   const bool last = 8 * (t + nt * (NCH - 1)) < D;
-  float own[8];
+  bool own[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) own[i] = chunk_owns(t + nt * (NCH - 1), i, D) ? 1.f : 0.f;
+  for (int i = 0; i < 8; i++) own[i] = chunk_owns(t + nt * (NCH - 1), i, D);
 
   struct Raw {
     typename Vec8<XT>::v x[NCH], dr[NCH];
@@ -420,8 +421,7 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
 #pragma unroll
       for (int i = 0; i < 8; i++) acc[k][c][i] = 0.f;
   }
-  const float lay1 = a.post == NORM_LAYER ? inv_d : 0.f, cor1 = a.post == NORM_NONE ? 0.f : inv_d;
-  const float lay2 = a.pre == NORM_LAYER ? inv_d : 0.f;
+  const bool layer1 = a.post == NORM_LAYER, norm1 = a.post != NORM_NONE, layer2 = a.pre == NORM_LAYER;
 
   // Fetching the next row early is worth half of the waves where the registers allow it (32768 x 4096 bf16: 305 us against
   // 396 us with four waves per SIMD and no early fetch); with 16 columns per lane it spills (1024 x 900 fp32: 21 against 17 us).
@@ -431,7 +431,8 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
   for (; row < a.rows; row += stride) {
     const Raw v = EARLY ? cur : load(row);
     if (EARLY && row + stride < a.rows) cur = load(row + stride);
-    const float m1 = v.st[0], s1 = v.st[1], m2 = v.st[2], s2 = v.st[3];
+    // y not used: its norm has no share in du, not even where the row has none (an infinity)
+    const float m1 = v.st[0], s1 = v.st[1], m2 = v.st[2], s2 = a.dy ? v.st[3] : 0.f;
     float hh[NCH][8], rh[NCH][8], du[NCH][8], G[GF ? NCH : 1][8], dG[GF ? NCH : 1][8];
     const float grow = a.gate_mode == GATE_ROW ? gate_value(v.grow, a.gate_act) : 1.f;
     float c12[2] = {0.f, 0.f};
@@ -444,12 +445,12 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
         hh[c][i] = ((float)v.h[c][i] - m1) * s1;
         // without a block A1 is the scale's default, but the statistics are 0 and 1 and h is zero: nothing is added
         const float r = (float)v.x[c][i] + (hh[c][i] * A1[c][i] + B1[c][i]) * g;
-        rh[c][i] = (r - m2) * s2;
+        rh[c][i] = a.dy ? (r - m2) * s2 : 0.f;
         const float dy = (float)v.dy[c][i], av = dy * W2[c][i];
         du[c][i] = (float)v.dr[c][i] + s2 * av;
-        const float ao = c == NCH - 1 ? av * own[i] : av;
-        c12[0] += ao;
-        c12[1] += ao * rh[c][i];
+        const bool in = c < NCH - 1 || own[i];
+        c12[0] += in ? av : 0.f;
+        c12[1] += in ? av * rh[c][i] : 0.f;
         if constexpr (!WIDE) {
           acc[1][c][i] += dy * rh[c][i];
           if constexpr (BIAS) acc[3][c][i] += dy;
@@ -457,7 +458,8 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
       }
     }
     if (a.dy) row_sum<TPR, 2>(c12, red, turn);
-    const float c1 = s2 * c12[0] * lay2, c2 = s2 * c12[1] * inv_d;
+    // means that the norm does not have stay 0, whatever their sums are
+    const float c1 = layer2 ? s2 * c12[0] * inv_d : 0.f, c2 = s2 * c12[1] * inv_d;
     if (WIDE && a.ws && t == 0) {
       rowc[row * 2] = c1;
       rowc[row * 2 + 1] = c2;
@@ -475,16 +477,17 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
           acc[0][c][i] += dg * hh[c][i];
           if constexpr (BIAS) acc[2][c][i] += dg;
         }
-        const float bo = c == NCH - 1 ? dg * A1[c][i] * own[i] : dg * A1[c][i];
-        e[0] += bo;
-        e[1] += bo * hh[c][i];
-        if constexpr (!GF) e[2] += (c == NCH - 1 ? du[c][i] * own[i] : du[c][i]) * (hh[c][i] * A1[c][i] + B1[c][i]);
+        const bool in = c < NCH - 1 || own[i];
+        const float b = dg * A1[c][i];
+        e[0] += in ? b : 0.f;
+        e[1] += in ? b * hh[c][i] : 0.f;
+        if constexpr (!GF) e[2] += in ? du[c][i] * (hh[c][i] * A1[c][i] + B1[c][i]) : 0.f;
       }
       if (a.dx && (c < NCH - 1 || last)) st8<SMALL, XT>((XT*)a.dx + row * D, base[c], D, du[c]);
     }
     if (!a.h) continue;
     row_sum<TPR, GF ? 2 : 3>((float(&)[GF ? 2 : 3])e, red, turn);
-    const float e1 = e[0] * lay1, e2 = e[1] * cor1;
+    const float e1 = layer1 ? e[0] * inv_d : 0.f, e2 = norm1 ? e[1] * inv_d : 0.f;
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
       if (c == NCH - 1 && !last) continue;
@@ -493,7 +496,7 @@ __global__ __launch_bounds__(threads<TPR>(), bwd_waves(TPR)) void rnorm_bwd_kern
       for (int i = 0; i < 8; i++) {
         float g = grow;
         if constexpr (GF) g = G[c][i];
-        dh[i] = s1 * (du[c][i] * g * A1[c][i] - e1 - hh[c][i] * e2);
+        dh[i] = s1 * (du[c][i] * g * A1[c][i] - e1 - (norm1 ? hh[c][i] * e2 : 0.f));
       }
       if (a.dh) st8<SMALL, HT>((HT*)a.dh + row * D, base[c], D, dh);
       if constexpr (GF) {
@@ -557,7 +560,7 @@ __global__ __launch_bounds__(256) void rnorm_colpass_kernel(ScpResidualNorm a, c
     for (int i = 0; i < 8; i++) k[i] = 0.f;
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const f32x4 st = *(const f32x4*)(a.stats + row * 4);
-    const float c1 = rowc[row * 2], c2 = rowc[row * 2 + 1];
+    const float c1 = rowc[row * 2], c2 = rowc[row * 2 + 1], s2 = a.dy ? st[3] : 0.f;
     const auto xv = ld8<false, XT>((const XT*)a.x + row * a.ldx, base, D);
     typename Vec8<HT>::v hv, gv, yv;
     typename Vec8<XT>::v rv;
@@ -571,9 +574,9 @@ __global__ __launch_bounds__(256) void rnorm_colpass_kernel(ScpResidualNorm a, c
       float g = grow;
       if constexpr (GF) g = gate_value((float)gv[i], a.gate_act);
       const float hh = a.h ? ((float)hv[i] - st[0]) * st[1] : 0.f;
-      const float rh = ((float)xv[i] + (hh * A1[i] + B1[i]) * g - st[2]) * st[3];
+      const float rh = a.dy ? ((float)xv[i] + (hh * A1[i] + B1[i]) * g - st[2]) * s2 : 0.f;
       const float dy = a.dy ? (float)yv[i] : 0.f;
-      const float dg = ((a.dr ? (float)rv[i] : 0.f) + st[3] * dy * W2[i] - (c1 + rh * c2)) * g;
+      const float dg = ((a.dr ? (float)rv[i] : 0.f) + s2 * dy * W2[i] - (c1 + rh * c2)) * g;
       acc[0][i] += dg * hh;
       acc[1][i] += dy * rh;
       if constexpr (BIAS) {
