@@ -182,8 +182,10 @@ class HipLinear8(HipLinear):
     instead of 4 (or 2).  The weight gradient is taken from the checkpoint's values; output, input and bias gradient are not
     affected."""
 
-    def forward(self, x):
-        return ops.linear8(x, self.weight, self.bias)
+    def forward(self, x, relu_input=False):
+        """relu_input: y = Linear(relu(x)), a relu of its own in front (exact, so it keeps its output as torch.relu does;
+        ops.act8 before the layer keeps 8 bits instead)."""
+        return ops.linear8(torch.relu(x) if relu_input else x, self.weight, self.bias)
 
 
 class ResidualTrunk(nn.Module):

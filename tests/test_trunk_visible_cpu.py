@@ -48,3 +48,11 @@ def test_plain_calls_still_run():
     for which in (0, 4, 6):
         out = calls(x, W, b)[which][2]()
         assert out.requires_grad if which == 0 else out[1].requires_grad
+
+
+def test_linear8_module_takes_the_arguments_of_its_base():
+    import scpair_amd as S
+    layer = S.HipLinear8(8, 3)
+    for args in ((), (False,), (True,)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            layer(torch.zeros(2, 8), *args)
