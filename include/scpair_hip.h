@@ -367,7 +367,7 @@ typedef struct {
   int gate_mode;       /* 0 none, 1 per element, 2 per row, 3 per column */
   int gate_act;        /* 0 none, 1 sigmoid, 2 tanh */
   int scale_mode;      /* 0 scale_value, 1 one learned number, 2 per column */
-  float scale_value, eps;
+  float scale_value, eps;           /* eps > 0 */
   int want1, want2;    /* set by the backward itself */
 } ScpResidualNorm;
 int scp_residual_norm_max_cols(void);

@@ -755,6 +755,7 @@ int check_args(const ScpResidualNorm* a, const char* who) {
   SCP_CHECK(a->cols <= MAX_COLS, SCP_ERR_SHAPE, "%s: at most %d columns (got %d)", who, MAX_COLS, a->cols);
   SCP_CHECK(!(a->x_bf16 && !a->h_bf16), SCP_ERR_ARG, "%s: a bf16 residual stream needs bf16 blocks", who);
   SCP_CHECK(a->x && a->ldx >= 0 && a->ldh >= 0 && a->ldg >= 0, SCP_ERR_ARG, "%s: null x or negative row stride", who);
+  SCP_CHECK(a->eps > 0.f && a->eps < __builtin_inff(), SCP_ERR_ARG, "%s: eps must be positive and finite", who);
   SCP_CHECK(a->pre == NORM_RMS || a->pre == NORM_LAYER, SCP_ERR_ARG, "%s: pre must be rms (1) or layer (2)", who);
   SCP_CHECK(a->post >= NORM_NONE && a->post <= NORM_LAYER, SCP_ERR_ARG, "%s: post must be 0, 1 or 2", who);
   SCP_CHECK(a->gate_mode >= GATE_NONE && a->gate_mode <= GATE_COL && a->gate_act >= ACT_NONE && a->gate_act <= ACT_TANH &&

@@ -2085,8 +2085,8 @@ def gated_residual_norm(x, h=None, gate=None, scale=None, post=None, post_weight
         raise ValueError(f"gated_residual_norm: post must be None, 'rms' or 'layer' and pre 'rms' or 'layer', got {post!r}, {pre!r}")
     if gate_act not in _GATE_ACTS:
         raise ValueError(f"gated_residual_norm: gate_act must be one of {sorted(_GATE_ACTS)}, got {gate_act!r}")
-    if not (eps > 0 and math.isfinite(eps)):
-        raise ValueError(f"gated_residual_norm: eps must be positive, got {eps}")
+    if not 2.0 ** -149 <= eps <= torch.finfo(torch.float32).max:
+        raise ValueError(f"gated_residual_norm: eps must be positive (and neither 0 nor infinite in float32), got {eps}")
     if not 1 <= cols <= 16384:
         raise ValueError(f"gated_residual_norm: 1 to 16384 columns, got {cols}")
     gate_mode = scale_mode = 0
