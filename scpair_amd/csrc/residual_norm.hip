@@ -762,7 +762,8 @@ int check_args(const ScpResidualNorm* a, const char* who) {
                 a->scale_mode >= SCALE_VALUE && a->scale_mode <= SCALE_COL, SCP_ERR_ARG, "%s: unknown gate or scale mode", who);
   SCP_CHECK((a->gate_mode == GATE_NONE || a->gate) && (a->scale_mode == SCALE_VALUE || a->scale), SCP_ERR_ARG,
             "%s: gate or scale mode without its values", who);
-  SCP_CHECK(a->h || (a->gate_mode == GATE_NONE && a->post == NORM_NONE), SCP_ERR_ARG, "%s: gate or post norm without a block", who);
+  SCP_CHECK(a->h || (a->gate_mode == GATE_NONE && a->post == NORM_NONE && a->scale_mode == SCALE_VALUE && !a->w1 && !a->b1),
+            SCP_ERR_ARG, "%s: gate, scale or post norm without a block", who);
   return SCP_OK;
 }
 
@@ -791,7 +792,7 @@ extern "C" int scp_residual_norm_bwd(const ScpResidualNorm* a_, void* stream) {
   a.want1 = a.h && (a.dw1 || a.db1 || a.dscale || (a.gate_mode == GATE_COL && a.dgate));
   a.want2 = a.dw2 || a.db2;
   SCP_CHECK(!(a.want1 || a.want2) || a.ws, SCP_ERR_ARG, "scp_residual_norm_bwd: parameter gradients need the workspace");
-  SCP_CHECK((!a.dw1 || a.w1) && (!a.db1 || a.b1) && (!a.dscale || a.scale_mode != SCALE_VALUE) &&
+  SCP_CHECK((!a.dh || a.h) && (!a.dw1 || a.w1) && (!a.db1 || a.b1) && (!a.dscale || a.scale_mode != SCALE_VALUE) &&
                 (!a.dgate || a.gate_mode != GATE_NONE), SCP_ERR_ARG, "scp_residual_norm_bwd: gradient of an absent parameter");
   if (!(a.want1 || a.want2)) a.ws = nullptr;
   hipStream_t st = (hipStream_t)stream;

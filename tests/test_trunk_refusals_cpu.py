@@ -23,3 +23,16 @@ def test_eps_that_fp32_cannot_hold(eps):
     f = C.c_float(eps).value
     assert L.scp_residual_norm_fwd(norm_args(eps=f), None) == -1 and b"eps" in L.scp_last_error()
     assert L.scp_residual_norm_bwd(norm_args(eps=f), None) == -1 and b"eps" in L.scp_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(b1=64), dict(w1=64), dict(scale_mode=1, scale=64), dict(scale_mode=2, scale=64)])
+def test_parts_of_a_block_without_one(bad):
+    """h null: the backward pass took b1 into its recomputed row, and gradients of the others stayed unwritten."""
+    L = _lib.lib()
+    for entry in (L.scp_residual_norm_fwd, L.scp_residual_norm_bwd):
+        assert entry(norm_args(h=None, **bad), None) == -1 and b"without a block" in L.scp_last_error()
+
+
+def test_gradients_of_an_absent_block():
+    L = _lib.lib()
+    assert L.scp_residual_norm_bwd(norm_args(h=None, dh=64, dx=64), None) == -1 and b"absent" in L.scp_last_error()
