@@ -926,14 +926,10 @@ extern "C" int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const i
   if (g.nsplit == 1) {
     g.C = (float*)C;
     if (c_bf16) return launch8<true, true, EPI_DIRECT, true, __bf16>(g, st);
-    const long cb = (long)M * ldc * 4;
-    g.c_bytes = cb < (1L << 31) ? (unsigned)cb : 0u;
     return launch8<true, true, EPI_DIRECT, true, float>(g, st);
   }
   SCP_CHECK(ws, SCP_ERR_ARG, "scp_gemm_q8: this shape runs as %d K-ranges and needs the workspace of scp_gemm_q8_ws_floats", g.nsplit);
   g.C = ws;
-  const long cb = (long)M * ldc * 4;
-  g.c_bytes = cb < (1L << 31) ? (unsigned)cb : 0u;
   const int rc = launch8<true, true, EPI_SLAB, true, float>(g, st);
   if (rc) return rc;
   return c_bf16 ? reduce_slabs(g, ws, nullptr, (__bf16*)C, st) : reduce_slabs(g, ws, nullptr, (float*)C, st);
