@@ -38,12 +38,18 @@ __device__ __forceinline__ float normal_cdf_fast(float x, float gauss) {      //
   const float tail = t * p * gauss;
   return x < 0.f ? tail : 1.f - tail;
 }
+// exp of a non-positive argument only, so that a Newton step on the reciprocal (1 .. 2) is safe.  The step makes silu of every bf16
+// down to -87 the nearest bf16 to its value (the hardware's reciprocal alone: not at 5.9375, 5.6e-7 below the middle of two).
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  const float e = __expf(-fabsf(x)), d = 1.f + e, r = __builtin_amdgcn_rcpf(d), q = fmaf(fmaf(-d, r, 1.f), r, r);
+  return x < 0.f ? e * q : q;
+}
 template <bool FAST> __device__ __forceinline__ float act_value(float x, int kind, float slope) {
   if (kind == ACT_GELU) {
     if (FAST) return x * normal_cdf_fast(x, __expf(-0.5f * x * x));
     return 0.5f * x * (1.f + erff(x * 0.70710678f));
   }
-  if (kind == ACT_SILU) return FAST ? x * __builtin_amdgcn_rcpf(1.f + __expf(-x)) : x / (1.f + expf(-x));
+  if (kind == ACT_SILU) return FAST ? x * sigmoid_fast(x) : x / (1.f + expf(-x));
   return x > 0.f ? x : slope == 0.f && x < 0.f ? 0.f : slope * x;      // (relu of -infinity is 0)
 }
 template <bool FAST> __device__ __forceinline__ float act_slope(float x, int kind, float slope) {

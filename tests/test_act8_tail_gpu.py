@@ -59,3 +59,12 @@ def test_gelu_everywhere_else(dtype):
     want = act_ref(x.double(), "gelu", 0.0)
     got = ops.act8(x.cuda(), "gelu").cpu().double()
     assert ((got - want).abs() <= x.double().abs() * 2.0 ** -21 + want.abs() * (2.0 ** -8 if dtype == B16 else E) + 2.0 ** -134).all()
+
+
+def test_silu_of_every_bf16_is_the_nearest_bf16():
+    """From -87 up (exp(x) below it is no normal fp32 number), magnitudes from 2^-120 up (values are normal bf16 numbers)."""
+    from scpair_amd import ops
+    x = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(B16)
+    x = x[torch.isfinite(x) & (x >= -87) & (x.abs() >= 2.0 ** -120)]
+    want = act_ref(x.double(), "silu", 0.0).to(B16)
+    assert x.numel() > 40000 and torch.equal(ops.act8(x.reshape(1, -1).cuda(), "silu").cpu()[0], want)
