@@ -399,7 +399,8 @@ int scp_gemm_q8(int M, int N, int K, const void* A, long lda, const int8_t* code
 /* The whole layer, everything it launches: y = x W^T + b with x's checkpoint written beside it, and its gradients.  x, y, dy, dx
  * fp32 or bf16 (x_bf16), W and dW fp32 or bf16 (w_bf16; an fp32 x needs an fp32 W), W contiguous [N][K], b and db fp32.
  * ns as everywhere (fp32 x only).  codes / steps: forward nullable (no weight gradient to come).  dx, dW, db: nullable.
- * ws: scp_linear8_fwd_ws / _bwd_ws(args) bytes (-1: bad arguments), 256-byte aligned. */
+ * ws: scp_linear8_fwd_ws / _bwd_ws bytes of the same argument block, its pointers included (alignment decides about copies, absent
+ * ones need nothing); -1: bad arguments; 256-byte aligned. */
 typedef struct {
   const void* x;
   const void* W;

@@ -11,8 +11,8 @@
 //
 // Bound of every kernel here: HBM.  A lane holds 8 consecutive columns, 8 lanes a group; the group's maximum is a maximum
 // of integers (the magnitudes' bit patterns, which also shows infinities and NaN) over three lane exchanges.  Measured,
-// 16384 x 8192 bf16: packing 70 us, unpacking 67 us (0.40 GB each, 5.8 and 6.0 TB/s), silu 116 us forward with the packing
-// (0.67 GB, 5.8 TB/s), 137 us backward (0.67 GB, 4.9 TB/s: two streams of reads and the arithmetic of the derivative).
+// 16384 x 8192 bf16: packing 71 us, unpacking 67 us (0.40 GB each, 5.7 and 6.0 TB/s), silu 117-125 us forward with the packing
+// (0.67 GB, 5.4-5.8 TB/s), 129-137 us backward (0.67 GB, 4.9-5.2 TB/s: two streams of reads and the arithmetic of the derivative).
 #include "common.h"
 #include "ckpt8.h"
 #include "scpair_hip.h"

@@ -12,10 +12,10 @@
 // 64 x 64 tiles straight from the tensors, without prepared copies, for the minibatch sizes, where a launch counts as much as
 // the product.  A cost model with measured rates chooses (step_us).
 //
-// Measured (products alone; in parentheses the library's on operands laid out for it): 16384 x 4096 x 4096 bf16 y 425-445
-// (441), dx 425-445 (436), dW 490 us (554 with a bf16 operand); 1024 x 900 x 1800 fp32 39, 38 and 29 us (32, 31, 35, in fp32 without the
-// checkpoint); 777 x 1801 x 901 bf16 25, 18, 16 us (19, 19, 19).  The large ones are bound by the matrix pipes at the clock
-// they hold (68 % busy at 1.8 GHz), the small ones by the latency of a tile's K-steps with one or two workgroups a CU.
+// Measured (products alone; in parentheses the library's on operands laid out for it): 16384 x 4096 x 4096 bf16 y 425-480
+// (441), dx 425-485 (436), dW 427-510 us (554 with a bf16 operand), by box and clock; 1024 x 900 x 1800 fp32 39, 37 and 29 us (32, 31, 35, in fp32 without the
+// checkpoint); 777 x 1801 x 901 bf16 25, 18, 16 us (19, 19, 19); 4096 x 4096 x 4096 fp32 y 806 (918).  The large ones are bound by the
+// matrix pipes at the clock they hold (busy 70-73 % of the cycles, dW 67 %, at 1.5-1.8 GHz), the small ones by the latency of a tile's K-steps with one or two workgroups a CU.
 #include <limits.h>
 #include "ckpt8.h"
 #include "common.h"

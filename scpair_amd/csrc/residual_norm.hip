@@ -22,9 +22,10 @@
 // alignment: the vector accesses are declared with the element's alignment, which the hardware takes as they are.
 // Column sums leave a workgroup as one partial row each; a second launch adds them in a fixed order (no atomics).
 //
-// Measured (32768 x 4096 bf16, rms norms, a gate per column): forward 200 us for 1.07 GB, 5.3 TB/s; backward 296 us for
-// 1.61 GB, 5.4 TB/s; a large copy reaches 5.1 TB/s.  4096 x 2048, fp32 stream beside bf16 blocks with a full gate: 22 and
+// Measured (32768 x 4096 bf16, rms norms, a gate per column): forward 200 us for 1.07 GB, 5.3 TB/s; backward 291-320 us
+// for 1.61 GB, 5.0-5.5 TB/s; a large copy reaches 5.1 TB/s.  4096 x 2048, fp32 stream beside bf16 blocks with a full gate: 22 and
 // 33 us, 5.4 and 5.6 TB/s.  1024 x 900 fp32, full gate: 9 and 12 us, and 9 us for the column sums: bound by latency.
+// 8192 x 6144 bf16, full gate: 93 and 155 us, 5.4 and 5.2 TB/s; 8192 x 8192 with biases: 132 and 227 us, 5.1 and 4.7 TB/s.
 #include "common.h"
 #include "scpair_hip.h"
 

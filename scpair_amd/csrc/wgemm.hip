@@ -99,8 +99,8 @@ enum { EPI_SLAB = 0, EPI_DIRECT = 1, EPI_ADAMW = 2 };
 
 // NW = 8 (default for the plain products): two waves per SIMD, wave tile 128 x 64; one wave's MFMA groups cover the other's
 // waits, and the tiles go from memory to LDS without passing through registers (a lane's 16 bytes land at LDS slot `lane` of
-// its wave's KB, so the swizzle is applied to what the lane fetches).  16384 x 4096 x 4096 bf16: 425-445 us (1240-1290 TFLOP/s)
-// with rows or columns for B; 516 and 512 us through registers, 437 and 499 us with the barrier at the step's end.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
+// its wave's KB, so the swizzle is applied to what the lane fetches).  16384 x 4096 x 4096 bf16: 425-485 us by box and clock
+// (1130-1290 TFLOP/s) with rows or columns for B; 516 and 512 us through registers, 437 and 499 us with the barrier at the step's end.  NW = 4 (the AdamW form; SCPAIR_WGEMM_NW=4
 // elsewhere): one wave per SIMD, wave tile 128 x 128, two register sets (loads two K-steps ahead).
 // BQ: the B operand (col) is an 8-bit activation checkpoint (ckpt8.hip): codes [K][ldb] int8 and one step byte per 64
 // columns.  A thread takes 16 codes with one 16-byte load, half the bytes of the bf16 operand, and takes them apart on the

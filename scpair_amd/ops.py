@@ -2219,7 +2219,9 @@ def linear8(x, W, b=None):
     """y = x W^T + b for x [..., K], W [N, K], b [N], keeping x for the backward pass as an 8-bit checkpoint: dW = dy^T
     unpack8(pack8(x)), while y, dx and db are what linear gives.  x float32 with W float32: y float32, products in the
     precision of set_precision.  x bfloat16 with W bfloat16 or float32 (rounded once per call): y bfloat16, bf16 products
-    with fp32 sums; dW has W's type.  Other derivatives and tracing are refused.  b may have any floating-point type.  W and its gradient stay below 2 GiB of bf16."""
+    with fp32 sums; dW has W's type.  Other derivatives and tracing are refused.  b may have any floating-point type.  W and its gradient stay below 2 GiB of bf16.  While a call runs, products too large for 64 x 64 tiles
+    take workspace: bf16 copies of operands that are not bf16 with a multiple of 8 columns, and in the fp32-equivalent precision 12 bytes an
+    element of x and W (backward: dy, W and again W).  float32 values beyond bfloat16's largest, 3.39e38, count as infinities."""
     _check_floats("linear8", x)
     _check_floats("linear8", W)
     K = x.shape[-1]

@@ -36,3 +36,18 @@ def test_parts_of_a_block_without_one(bad):
 def test_gradients_of_an_absent_block():
     L = _lib.lib()
     assert L.scp_residual_norm_bwd(norm_args(h=None, dh=64, dx=64), None) == -1 and b"absent" in L.scp_last_error()
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 4096), (16384, 4096, 4096)])
+def test_workspace_of_the_fp32_blocks(M, N, K):
+    """What the documentation says of the wide products in the fp32-equivalent precision: 12 bytes an element of x and W forward, of dy and W
+    backward, and three fp32 planes of dW."""
+    a = _lib.Linear8()
+    for k, v in dict(x=4096, W=4096, y=4096, dy=4096, dx=4096, dW=4096, codes=4096, steps=4096, M=M, N=N, K=K, ldx=K, lddy=N, ns=3).items():
+        setattr(a, k, v)
+    tiles, L = (C.c_int * 3)(), _lib.lib()
+    assert L.scp_linear8_tiles(C.byref(a), tiles) == 0 and list(tiles) == [256] * 3
+    assert L.scp_linear8_fwd_ws(C.byref(a)) == 12 * (M * K + N * K)
+    bwd = L.scp_linear8_bwd_ws(C.byref(a))
+    assert 0 <= bwd - (12 * (M * N + N * K) + 12 * N * K) <= 8 * N * K          # and slabs where a sum is divided
+    assert L.scp_linear8_tiles(None, tiles) == -1 and L.scp_linear8_tiles(C.byref(a), None) == -1
