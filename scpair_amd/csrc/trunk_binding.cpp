@@ -25,7 +25,7 @@ void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t
 
 void check(int rc, const char* what) {
   if (rc == 0) return;
-  TORCH_CHECK_VALUE(rc != -1, what, ": ", scp_last_error());
+  TORCH_CHECK_VALUE(rc != -1 && rc != -2, what, ": ", scp_last_error());
   TORCH_CHECK(false, what, ": error ", rc, ": ", scp_last_error());
 }
 

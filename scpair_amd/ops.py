@@ -2164,7 +2164,7 @@ def _check_floats(what, t):
 
 
 def pack8(x):
-    """The 8-bit checkpoint of a float32 or bfloat16 tensor [..., D] (a Packed8).  Every 64 columns of a row share a step
+    """The 8-bit checkpoint of a float32 or bfloat16 tensor [..., D], D at most 2^24 (a Packed8).  Every 64 columns of a row share a step
     2^k, the smallest power of two with max|x| <= 127 * 2^k (k >= -126; k <= 121, where codes saturate); a code is x / 2^k
     rounded to nearest even, so a value is off by at most max|x| / 127 of its group.  For autograd Functions of your own: no gradient flows through."""
     _check_floats("pack8", x)
@@ -2202,7 +2202,7 @@ _ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
 
 
 def act8(z, kind="gelu", slope=0.01):
-    """act(z) for z [..., D] float32 or bfloat16, keeping z for the backward pass as an 8-bit checkpoint that the same launch
+    """act(z) for z [..., D] float32 or bfloat16, D at most 2^24, keeping z for the backward pass as an 8-bit checkpoint that the same launch
     writes: dz = dout * act'(unpack8(pack8(z))); other derivatives and tracing are refused.  kind: 'gelu' (the erf form), 'silu', or 'leaky_relu' (slope; 0 is relu; a
     value whose code is 0 counts as not positive)."""
     _check_floats("act8", z)
