@@ -64,7 +64,7 @@ template <bool FAST> __device__ __forceinline__ float act_slope(float x, int kin
     const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
     return s * (1.f + x * (1.f - s));
   }
-  return x > 0.f ? 1.f : slope;
+  return x > 0.f ? 1.f : x <= 0.f ? slope : x;      // (a NaN group has no sign: NaN, like the others)
 }
 
 // ACT: also out = act(x), and codes may be null (no backward pass to come)

@@ -2204,7 +2204,7 @@ _ACTS8 = {"gelu": 0, "silu": 1, "leaky_relu": 2}
 def act8(z, kind="gelu", slope=0.01):
     """act(z) for z [..., D] float32 or bfloat16, D at most 2^24, keeping z for the backward pass as an 8-bit checkpoint that the same launch
     writes: dz = dout * act'(unpack8(pack8(z))); other derivatives and tracing are refused.  kind: 'gelu' (the erf form), 'silu', or 'leaky_relu' (slope; 0 is relu; a
-    value whose code is 0 counts as not positive)."""
+    value whose code is 0 counts as not positive).  Where 64 columns held an infinity or a NaN, dz of all of them is NaN."""
     _check_floats("act8", z)
     if kind not in _ACTS8:
         raise ValueError(f"act8: kind must be one of {sorted(_ACTS8)}, got {kind!r}")

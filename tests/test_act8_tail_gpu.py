@@ -68,3 +68,18 @@ def test_silu_of_every_bf16_is_the_nearest_bf16():
     x = x[torch.isfinite(x) & (x >= -87) & (x.abs() >= 2.0 ** -120)]
     want = act_ref(x.double(), "silu", 0.0).to(B16)
     assert x.numel() > 40000 and torch.equal(ops.act8(x.reshape(1, -1).cuda(), "silu").cpu()[0], want)
+
+
+@pytest.mark.parametrize("kind,slope", [("leaky_relu", 0.0), ("leaky_relu", 0.1), ("gelu", 0.0), ("silu", 0.0)])
+@pytest.mark.parametrize("dtype", [F32, B16])
+def test_a_group_without_values_has_no_derivatives(kind, slope, dtype):
+    """A group that held an infinity or a NaN reads as NaN, and so does the gradient of all its columns, for every activation: the sign
+    that a leaky relu would need is not there."""
+    from scpair_amd import ops
+    z = torch.randn(3, 130, generator=torch.Generator().manual_seed(2)).to(dtype)
+    z[0, 70], z[2, 129] = float("inf"), float("nan")
+    zg = z.cuda().requires_grad_()
+    d, = torch.autograd.grad(ops.act8(zg, kind, slope), zg, torch.ones(3, 130, dtype=dtype).cuda())
+    bad = torch.zeros(3, 130, dtype=torch.bool)
+    bad[0, 64:128], bad[2, 128:] = True, True
+    assert torch.equal(d.cpu().isnan(), bad)
